@@ -301,6 +301,116 @@ int scree_padded_lengths_ex(const void* mask, int mask_elem_bytes, int64_t B, in
 int scree_from_padded(const void* padded, const int32_t* offsets, int64_t B, int64_t max_len,
                       int64_t T, int64_t row_bytes, void* values, void* stream);
 
+/* ------------------------------------------------------------------ paged K/V cache
+ * No reference counterpart (docs/kernels.md:178 lists KV-cache support as
+ * planned).  A cache of L layers keeps its K and V in pools of shape
+ * (L, P, H, page, D), contiguous.  The bookkeeping is shared by the layers:
+ * table (S, M) int32, the pages of each slot in order and -1 beyond them;
+ * lengths (S,) int32, tokens of each slot (0 = free slot); refs (P,) int32,
+ * number of slots that hold each page (0 = free page).  A slot's part-filled
+ * last page is never shared.
+ *
+ * The calls read the bookkeeping from table / lengths / refs and write the new
+ * one to the *_out arrays, which must be other memory; the pools are updated in
+ * place.  Slots of one call must differ.  What a call cannot do (a slot, count or
+ * path out of range, too few free pages, a draft on shared pages) sets the device
+ * status word (SCREE_DEVERR_BAD_INPUT, sites 60-63); the bookkeeping is then
+ * copied through unchanged and no row moves.  Allocation takes the lowest free
+ * pages in the order of the call's entries.  At most 65536 slots.
+ * workspace: scree_paged_workspace_size() bytes, 16-byte aligned; calls that
+ * share one must be ordered (one stream). */
+typedef struct {
+  const int32_t *table, *lengths, *refs;
+  int32_t *table_out, *lengths_out, *refs_out;
+  int64_t S, M, P, page;
+} scree_paged_book;
+typedef struct {
+  void *k, *v;
+  int64_t L, H;
+  int64_t row_bytes; /* D elements */
+} scree_paged_pools;
+
+size_t scree_paged_workspace_size(int64_t S, int64_t P);
+/* Grows slot slots[i] by counts[i] tokens (allocates their pages). */
+int scree_paged_reserve(const scree_paged_book* book, const int32_t* slots, const int32_t* counts,
+                        int64_t n, void* workspace, size_t workspace_bytes, void* stream);
+/* Of the last drafted[i] tokens of slot slots[i], keeps those that row i of path
+ * (n, depth) names (ascending indices into the draft, ended by -1): their rows
+ * move to the front of the draft in every layer, the slot ends behind them and
+ * pages no longer needed are freed. */
+int scree_paged_accept(const scree_paged_book* book, const scree_paged_pools* pools,
+                       const int32_t* slots, const int32_t* drafted, const int32_t* path,
+                       int64_t depth, int64_t n, void* workspace, size_t workspace_bytes,
+                       void* stream);
+/* Slot children[i] (empty) becomes a copy of slot parents[i]: full pages are
+ * shared, the rows of a part-filled page are copied to a new one.  A parent may
+ * be named more than once and may not be a child. */
+int scree_paged_fork(const scree_paged_book* book, const scree_paged_pools* pools,
+                     const int32_t* parents, const int32_t* children, int64_t n, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* Empties the slots; pages that no other slot holds become free. */
+int scree_paged_free(const scree_paged_book* book, const int32_t* slots, int64_t n, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* Moves used pages to the front of the pools: with U used pages, the k-th used
+ * page at or above U goes to the k-th free page below U. */
+int scree_paged_compact(const scree_paged_book* book, const scree_paged_pools* pools,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* Writes K and V rows of one layer: rows [offsets[b], offsets[b+1]) of k / v
+ * (T, H, D) go to the last tokens of slot slots[b].  Strides in BYTES, unit
+ * stride inside a head. */
+int scree_paged_write(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
+                      int64_t S, int64_t M, int64_t P, int64_t page, int64_t layer,
+                      const int32_t* slots, const void* k, int64_t k_row_bytes,
+                      int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
+                      int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
+                      int64_t T, void* stream);
+/* Who sees whom in trees of drafted tokens: parents (T,) int32, index of each
+ * node's parent within its sequence (smaller than its own) or negative for a
+ * root; bit j of row t of mask (T, words) = node j is t or an ancestor of t. */
+int scree_tree_mask(const int32_t* parents, const void* offsets, int offs_is_i64, int64_t B,
+                    int64_t T, int64_t words, uint64_t* mask, void* stream);
+
+/* Attention of new tokens over the cache: q / o (T, H, D) fp16 / bf16 with
+ * offsets (B+1); the n_b queries of sequence b are the last n_b tokens of slot
+ * slots[b], whose K / V are already written.  Every query sees all tokens before
+ * those n_b; of the n_b, query i sees token j where bit j of its mask row
+ * (words x 64 bits) is set, or j <= i if mask is NULL.  A query that sees nothing gets
+ * O = 0 and LSE = -inf.  K/V head = query head / (H / H_kv).  D 32, 64 or 128;
+ * page a multiple of 16; at most 4096 sequences.  lse (T, H) fp32 or NULL.
+ * The pools' base and row strides must suit TMA (16-byte aligned base).
+ * workspace: 16-byte aligned. */
+size_t scree_attn_fwd_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t H_kv, int D);
+int scree_attn_fwd_paged(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                         const scree_paged_pools* pools, int64_t layer, const int32_t* table,
+                         const int32_t* lengths, int64_t S, int64_t M, int64_t P, int64_t page,
+                         const int32_t* slots, const void* offsets, int offs_is_i64, int64_t B,
+                         int64_t T, int64_t H, int D, int dtype, float scale,
+                         const uint64_t* mask, int64_t words, void* o, int64_t o_row_stride,
+                         int64_t o_head_stride, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ token log probabilities
+ * logits (N, V) in dtype with row stride row_stride (elements); targets (N,)
+ * int32 / int64.  Per row (fp32): lse; logp = logits[target] - lse, 0 for a
+ * negative target (no token given), a target >= V sets the status word
+ * (SCREE_DEVERR_BAD_INPUT, site 50); entropy in nats; the `top` (0..32) most
+ * likely tokens' log probabilities and indices, equal values by lower index,
+ * NaN above all.  A row of -inf alone has lse = logp = -inf and entropy 0.
+ * No reference counterpart. */
+size_t scree_token_logprobs_workspace_size(int64_t N, int64_t V, int top, int dtype);
+int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, const void* targets,
+                             int targets_is_i64, int64_t N, int64_t V, int top, int dtype,
+                             float* logp, float* entropy, float* lse, float* top_logp,
+                             int64_t* top_ids, void* workspace, size_t workspace_bytes,
+                             void* stream);
+/* d_logits (N, V) contiguous from the gradients of logp, entropy (N,) and
+ * top_logp (N, top), each fp32 contiguous or NULL. */
+int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, const void* targets,
+                             int targets_is_i64, const float* lse, const float* entropy,
+                             const int64_t* top_ids, const float* g_logp, const float* g_entropy,
+                             const float* g_top, int64_t N, int64_t V, int top, int dtype,
+                             void* d_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

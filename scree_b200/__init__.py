@@ -8,7 +8,7 @@ hand-written CUDA kernels from libscree_b200.so; there is no CPU path.
 """
 
 from ._core import Array, from_cu_seqlens, from_padded, pack, to_padded, unpack
-from . import kernels
+from . import kernels, paged
 
 __version__ = "0.1.0"
 
@@ -20,5 +20,6 @@ __all__ = [
     "from_padded",
     "from_cu_seqlens",
     "kernels",
+    "paged",
     "__version__",
 ]

@@ -84,6 +84,16 @@ class Array:
             return list(self._host)
         return _host_offsets(self.offsets)
 
+    def _with_values(self, values: Any) -> "Array":
+        """An Array of other values on the same offsets.  The offsets were checked against
+        the ragged size when this Array was made, so nothing is read from the device."""
+        assert values.shape[self.ragged_dim] == self.values.shape[self.ragged_dim]
+        out = object.__new__(Array)
+        for name, value in (("values", values), ("offsets", self.offsets), ("ragged_dim", self.ragged_dim),
+                            ("_host", self._host)):
+            object.__setattr__(out, name, value)
+        return out
+
     @property
     def batch_size(self) -> int:
         return len(self.offsets) - 1

@@ -29,6 +29,20 @@ _L = ctypes.c_int64
 _F = ctypes.c_float
 _S = ctypes.c_size_t
 
+
+class PagedBook(ctypes.Structure):
+    """scree_paged_book: a cache's bookkeeping, before and after a call."""
+
+    _fields_ = [("table", _P), ("lengths", _P), ("refs", _P), ("table_out", _P), ("lengths_out", _P),
+                ("refs_out", _P), ("S", _L), ("M", _L), ("P", _L), ("page", _L)]
+
+
+class PagedPools(ctypes.Structure):
+    """scree_paged_pools: a cache's K and V memory."""
+
+    _fields_ = [("k", _P), ("v", _P), ("L", _L), ("H", _L), ("row_bytes", _L)]
+
+
 # name -> (restype, argtypes); mirrors include/scree_b200.h
 _SIGNATURES = {
     "scree_last_error": (_I, [ctypes.c_char_p, _S]),
@@ -81,6 +95,25 @@ _SIGNATURES = {
     "scree_padded_lengths_ex": (_I, [_P, _I, _L, _L, _P, _P]),
     "scree_to_padded_ex": (_I, [_P, _P, _I, _L, _L, _L, _L, _P, _I, _P, _P, _I, _P]),
     "scree_from_padded": (_I, [_P, _P, _L, _L, _L, _L, _P, _P]),
+    "scree_paged_workspace_size": (_S, [_L, _L]),
+    "scree_paged_reserve": (_I, [_P, _P, _P, _L, _P, _S, _P]),
+    "scree_paged_accept": (_I, [_P, _P, _P, _P, _P, _L, _L, _P, _S, _P]),
+    "scree_paged_fork": (_I, [_P, _P, _P, _P, _L, _P, _S, _P]),
+    "scree_paged_free": (_I, [_P, _P, _L, _P, _S, _P]),
+    "scree_paged_compact": (_I, [_P, _P, _P, _S, _P]),
+    "scree_paged_write": (
+        _I,
+        [_P, _P, _P, _L, _L, _L, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _I, _L, _L, _P],
+    ),
+    "scree_tree_mask": (_I, [_P, _P, _I, _L, _L, _L, _P, _P]),
+    "scree_attn_fwd_paged_workspace_size": (_S, [_L, _L, _L, _L, _I]),
+    "scree_attn_fwd_paged": (
+        _I,
+        [_P, _L, _L, _P, _L, _P, _P, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _I, _I, _F, _P, _L, _P, _L, _L, _P, _P, _S, _P],
+    ),
+    "scree_token_logprobs_workspace_size": (_S, [_L, _L, _I, _I]),
+    "scree_token_logprobs_fwd": (_I, [_P, _L, _P, _I, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "scree_token_logprobs_bwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P, _P]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,747 @@
+// attn_paged.cu — attention of new tokens (single ones, chunks, trees of drafted
+// tokens) over a paged K/V cache.
+//
+//   S = Q K^T scale over the visible keys, P = softmax(S), O = P V, LSE = m + ln l
+//
+// The rows that share a K/V head (token i, query head h * G + g -> row i G + g)
+// form row tiles of R rows; a (sequence, K/V head, row tile) is a segment of
+// ceil(len / 16) groups of 16 keys.  All segments laid end to end are cut into
+// equal runs of groups, one run per worker, so the cache is read evenly by the
+// whole GPU whatever the lengths are: a long sequence is spread over many
+// workers, short ones share a worker.  A worker is one warp with a ring of
+// shared memory of its own, filled by TMA one group ahead of the next; the
+// warps of a CTA never wait for one another.  A segment that one worker holds
+// whole is written out by it; pieces of a split segment go to the workspace as
+// (m, l, O) and a second kernel joins them.
+//
+// Bound: HBM, 4 D bytes per key and K/V head (R <= 32 rows of mma.sync work per
+// key hide under that).  A group is 16 keys because that is the contraction of
+// one mma and pages hold multiples of it, so a group never spans pages.
+#include <algorithm>
+#include "attn_common.cuh"
+
+namespace scree {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kKeys = 16;            // keys of a group
+constexpr int kMaxSeqs = 4096;       // prefix of the segments in shared memory
+constexpr int kSitePagedAttn = 70, kSitePagedAttnPage = 71, kSitePagedAttnWait = 72;
+
+template <int D> struct Cfg {
+  static constexpr int ROWB = D >= 64 ? 128 : 64;  // bytes of a box row (= swizzle span)
+  static constexpr int NB = D * 2 / ROWB;          // boxes across D
+  static constexpr int BOX = kKeys * ROWB;
+  static constexpr int PART = NB * BOX;            // K (or V) of a group
+  static constexpr int STAGE = 2 * PART;
+  static constexpr int STAGES = 3 * 128 / D;       // 24 KB in flight per warp, 192 KB per SM
+  static constexpr int RING = kWarps * STAGES * STAGE;
+  static constexpr int smem(int64_t B) {
+    return 1024 + RING + kWarps * STAGES * 8 + 64 + (int)(B + 1) * 8;
+  }
+};
+
+struct Params {
+  const char* q;
+  int64_t q_rs, q_hs;  // bytes
+  const void* offs;
+  int is64;
+  const int32_t *slots, *table, *lengths;
+  const unsigned long long* mask;
+  int words;
+  int B, S, M, P, page;
+  int H, Hkv, G;
+  int64_t T;
+  int64_t layer_row;  // first row of the layer in the pools' row view
+  float sl2;          // scale log2 e
+  char* o;
+  int64_t o_rs, o_hs;
+  float* lse;
+  int* status;
+  struct Head* head;
+  struct Desc* desc;
+  float2* part_ml;  // [slot][R]
+  float* part_o;    // [slot][R][D]
+};
+struct Head {
+  int64_t U, N;
+};
+struct Desc {  // the segment that a worker's first piece continues
+  int64_t s0, s1;
+  int32_t b, h, rt, on;
+};
+
+// First unit of worker w and the worker that holds unit u.
+__device__ __forceinline__ int64_t worker_start(int64_t w, int64_t U, int64_t N) { return w * U / N; }
+__device__ __forceinline__ int64_t worker_of(int64_t u, int64_t U, int64_t N) {
+  return ((u + 1) * N - 1) / U;
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  T o[2];
+  const float f[2] = {a, b};
+  cvt_from_f<T, 2>(f, o);
+  return (uint32_t)*reinterpret_cast<uint16_t*>(&o[0]) | ((uint32_t)*reinterpret_cast<uint16_t*>(&o[1]) << 16);
+}
+// All ones in the exponent: infinity or NaN, of either half of a word.
+template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
+  constexpr uint32_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+  return ((w & E) == E ? 0xFFFFu : 0u) | (((w >> 16) & E) == E ? 0xFFFF0000u : 0u);
+}
+
+// 16-bit visibility of keys [k0, k0 + 16) for query i of a sequence: all keys
+// before c0 = len - n, of the n new ones those of the mask row (or j <= i).
+__device__ __forceinline__ uint32_t visible16(const Params& p, int64_t row, int i, int k0, int c0, int len) {
+  uint32_t v = 0xFFFFu;
+  const int t0 = k0 - c0;  // tree index of key k0
+  if (t0 > -kKeys) {
+    if (p.mask == nullptr) {
+      const int last = i - t0;  // last visible key of the group
+      v = last >= 15 ? 0xFFFFu : last < 0 ? 0u : (2u << last) - 1;
+    } else {
+      const unsigned long long* m = p.mask + row * p.words;
+      unsigned long long bits;
+      if (t0 < 0) {
+        bits = (m[0] << -t0) | ((1ull << -t0) - 1);
+      } else {
+        const int w = t0 >> 6, o = t0 & 63;
+        bits = w < p.words ? m[w] >> o : 0ull;
+        if (o > 48 && w + 1 < p.words) bits |= m[w + 1] << (64 - o);
+      }
+      v = (uint32_t)bits & 0xFFFFu;
+    }
+  }
+  const int left = len - k0;
+  return left >= 16 ? v : v & ((1u << left) - 1);
+}
+
+template <int D, typename T, int MT>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const Params p) {
+  using C = Cfg<D>;
+  constexpr int R = 16 * MT;
+  constexpr int KK = D / 16;  // k-steps of Q K^T = pairs of 8-column tiles of O
+  asm volatile("griddepcontrol.launch_dependents;");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kWarps * C::STAGES);
+  int64_t* pre = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars + kWarps * C::STAGES) + 64);
+  __shared__ int64_t warp_sum[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  if (threadIdx.x < kWarps * C::STAGES) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_mbar_init();
+  bool bad = p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0;
+  const bool stopped = bad;
+  // Units before each sequence, by every CTA for itself (a launch of its own
+  // would cost more than these few loads).
+  int64_t carry = 0;
+  for (int base = 0; base < p.B; base += kThreads) {
+    const int b = base + threadIdx.x;
+    int64_t units = 0;
+    if (b < p.B) {
+      const int s = p.slots[b];
+      const int64_t lo = load_offset(p.offs, p.is64, b), hi = load_offset(p.offs, p.is64, b + 1);
+      const int64_t n = hi - lo;
+      if ((unsigned)s >= (unsigned)p.S || lo < 0 || n < 0 || hi > p.T || (b == 0 && lo != 0) ||
+          (b == p.B - 1 && hi != p.T)) {
+        bad = true;
+      } else {
+        const int64_t len = p.lengths[s];
+        if (len < n || len > (int64_t)p.M * p.page || (p.mask != nullptr && n > (int64_t)p.words * 64)) bad = true;
+        else units = (n * p.G + R - 1) / R * ((len + kKeys - 1) / kKeys) * p.Hkv;
+      }
+    }
+    int64_t x = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int64_t before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < p.B) pre[b + 1] = before + x;
+    carry = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[0] = 0;
+  if (__syncthreads_or(bad)) {
+    if (bad && !stopped) record_device_error(p.status, SCREE_DEVERR_BAD_INPUT, kSitePagedAttn);
+    return;
+  }
+  const int64_t U = carry;
+  if (U == 0) return;  // (T = 0 does not launch; every row has a key: its own)
+  const int64_t N = min((int64_t)gridDim.x * kWarps, U);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.head = Head{U, N};
+  // Neighbouring runs go to different SMs, so few workers are spread out too.
+  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  if (w >= N) return;
+  const int64_t u0 = worker_start(w, U, N), u1 = worker_start(w + 1, U, N);
+
+  struct Seg {
+    int b, h, rt, slot, len;
+    int64_t s0, s1;
+  };
+  auto find = [&](int64_t u) {
+    int lo = 0, hi = p.B - 1;  // last b with pre[b] <= u (empty ones have no units)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    Seg g;
+    g.b = lo;
+    g.slot = p.slots[lo];
+    g.len = p.lengths[g.slot];
+    const int64_t groups = (g.len + kKeys - 1) / kKeys;
+    const int64_t at = (u - pre[lo]) / groups;             // segment within the sequence
+    const int64_t rts = (pre[lo + 1] - pre[lo]) / groups / p.Hkv;  // row tiles
+    g.h = (int)(at / rts);
+    g.rt = (int)(at % rts);
+    g.s0 = pre[lo] + at * groups;
+    g.s1 = g.s0 + groups;
+    return g;
+  };
+
+  uint8_t* ring = smem + warp * C::STAGES * C::STAGE;
+  const uint32_t ring_s = smem_u32(ring);
+  uint64_t* full = bars + warp * C::STAGES;
+
+  // Loads run ahead of the work, across segments.  The page ids of 32 groups
+  // at a time sit in the lanes.
+  int64_t ui = u0;
+  Seg gi = find(u0);
+  int64_t win = -1;  // first unit of the window of page ids
+  int my_page = 0;
+  int ist = 0;
+  auto issue = [&]() {
+    if (ui >= u1) return;
+    if (ui >= gi.s1) {
+      gi = find(ui);
+      win = -1;
+    }
+    if (win < 0 || ui >= win + 32) {
+      win = ui;
+      const int64_t g = ui - gi.s0 + lane;
+      my_page = 0;
+      if (g < gi.s1 - gi.s0) {
+        my_page = p.table[(int64_t)gi.slot * p.M + g * kKeys / p.page];
+        if ((unsigned)my_page >= (unsigned)p.P) {
+          record_device_error(p.status, SCREE_DEVERR_BAD_INPUT, kSitePagedAttnPage);
+          my_page = 0;
+        }
+      }
+    }
+    const int page = __shfl_sync(0xffffffffu, my_page, (int)(ui - win));
+    if (lane == 0) {
+      const int in_page = (int)((ui - gi.s0) * kKeys % p.page);
+      const int row = (int)(p.layer_row + ((int64_t)page * p.Hkv + gi.h) * p.page + in_page);
+      uint8_t* st = ring + ist * C::STAGE;
+      mbar_expect_tx(&full[ist], C::STAGE);
+#pragma unroll
+      for (int c = 0; c < C::NB; ++c) tma_load_2d(st + c * C::BOX, &tm_k, &full[ist], c * (C::ROWB / 2), row);
+#pragma unroll
+      for (int c = 0; c < C::NB; ++c)
+        tma_load_2d(st + C::PART + c * C::BOX, &tm_v, &full[ist], c * (C::ROWB / 2), row);
+    }
+    ist = ist + 1 == C::STAGES ? 0 : ist + 1;
+    ++ui;
+  };
+#pragma unroll 1
+  for (int i = 0; i < C::STAGES; ++i) issue();
+
+  // Byte offset of 16-byte chunk c of key k in a part (TMA's swizzle).
+  auto chunk = [](int k, int c) -> uint32_t {
+    constexpr int CPR = C::ROWB / 16;
+    const int sw = C::ROWB == 128 ? (k & 7) : ((k >> 1) & 3);
+    return (uint32_t)((c / CPR) * C::BOX + k * C::ROWB + (((c % CPR) ^ sw) << 4));
+  };
+  const int mi = lane >> 3;
+  const int k_key = (mi >> 1) * 8 + (lane & 7), k_c = mi & 1;  // ldmatrix rows of K
+  const int v_key = (mi & 1) * 8 + (lane & 7), v_c = mi >> 1;  // and of V
+  const int qr = lane >> 2, qc = (lane & 3) * 2;               // row and column in mma tiles
+
+  int cst = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int64_t u = u0; ok && u < u1;) {
+    const Seg g = find(u);
+    const int64_t begin = u, end = min(u1, g.s1);
+    const int64_t q0 = load_offset(p.offs, p.is64, g.b);
+    const int n = (int)(load_offset(p.offs, p.is64, g.b + 1) - q0);
+    const int c0 = g.len - n;
+    const int rows = min(R, n * p.G - g.rt * R);
+    // Rows of this lane: tile mt, half r -> row mt * 16 + r * 8 + qr of the tile.
+    auto row_of = [&](int mt, int r) { return mt * 16 + r * 8 + qr; };
+    uint32_t qf[MT][KK][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = row_of(mt, r);
+        const int a = g.rt * R + row;
+        const bool in = row < rows;
+        const char* src = p.q + (q0 + (in ? a / p.G : 0)) * p.q_rs + (int64_t)(g.h * p.G + (in ? a % p.G : 0)) * p.q_hs;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          qf[mt][kk][r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + qc) * 2) : 0u;
+          qf[mt][kk][2 + r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + 8 + qc) * 2) : 0u;
+        }
+      }
+    float o[MT][2 * KK][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2 * KK; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
+    }
+#pragma unroll 1
+    for (; u < end; ++u) {
+      ok = mbar_wait(&full[cst], phase, abort_flag, p.status, kSitePagedAttnWait);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      const uint32_t ks = ring_s + cst * C::STAGE, vs = ks + C::PART;
+      float s[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][t][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        uint32_t kf[4];
+        ldsm_x4(ks + chunk(k_key, kk * 2 + k_c), kf);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16816<T>(s[mt][0], qf[mt][kk], kf[0], kf[1]);
+          mma16816<T>(s[mt][1], qf[mt][kk], kf[2], kf[3]);
+        }
+      }
+      const int k0 = (int)(u - g.s0) * kKeys;
+      const bool edge = k0 + kKeys > c0;  // holds new tokens, or runs past the end
+      uint32_t vis[MT][2];
+      if (edge) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = row_of(mt, r), i = row < rows ? (g.rt * R + row) / p.G : 0;
+            vis[mt][r] = visible16(p, q0 + i, i, k0, c0, g.len);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (!(vis[mt][r] >> (t * 8 + qc + e) & 1)) s[mt][t][r * 2 + e] = -INFINITY;
+          }
+      }
+      // Running maximum; rescaled only when it grew by more than 2^8 (P stays <= 256).
+      float alpha[MT][2];
+      bool need = false;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float mx = fmaxf(fmaxf(s[mt][0][r * 2], s[mt][0][r * 2 + 1]), fmaxf(s[mt][1][r * 2], s[mt][1][r * 2 + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mc = mx * p.sl2;
+          alpha[mt][r] = 1.f;
+          if (mc > m[mt][r] + 8.f) {
+            alpha[mt][r] = ex2_approx(m[mt][r] - mc);
+            m[mt][r] = mc;
+            need = true;
+          }
+        }
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          l[mt][0] *= alpha[mt][0];
+          l[mt][1] *= alpha[mt][1];
+#pragma unroll
+          for (int j = 0; j < 2 * KK; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[mt][e >> 1];
+        }
+      }
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float mm = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float e0 = ex2_approx(fmaf(s[mt][t][r * 2], p.sl2, -mm));
+            const float e1 = ex2_approx(fmaf(s[mt][t][r * 2 + 1], p.sl2, -mm));
+            l[mt][r] += e0 + e1;
+            pf[mt][t * 2 + r] = pack2<T>(e0, e1);
+          }
+        }
+      if (!edge) {
+#pragma unroll
+        for (int j = 0; j < KK; ++j) {
+          uint32_t vf[4];
+          ldsm_x4_t(vs + chunk(v_key, j * 2 + v_c), vf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
+            mma16816<T>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+          }
+        }
+      } else {
+        // A key that a row does not see must not reach it even if its V is an
+        // infinity or NaN (0 * NaN): such elements, and the rows past the end of
+        // the sequence, are taken out of the product; the infinities and NaN are
+        // then added for the rows that do see them.
+        const int left = g.len - k0;
+        auto live = [&](int k) { return (k < left ? 0xFFFFu : 0u) | (k + 1 < left ? 0xFFFF0000u : 0u); };
+        const uint32_t live_lo = live(qc), live_hi = live(qc + 8);
+        bool special = false;
+#pragma unroll
+        for (int j = 0; j < KK; ++j) {
+          uint32_t vf[4];
+          ldsm_x4_t(vs + chunk(v_key, j * 2 + v_c), vf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            vf[e] &= (e & 1) ? live_hi : live_lo;
+            const uint32_t nf = nonfinite_halves<T>(vf[e]);
+            special |= nf != 0;
+            vf[e] &= ~nf;
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
+            mma16816<T>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+          }
+        }
+        if (__any_sync(0xffffffffu, special)) {
+#pragma unroll 1
+          for (int k = 0; k < min(left, kKeys); ++k) {
+            float pk[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                // P of key k: lane (k % 8) / 2 of the quad, word t = k / 8, half k % 2.
+                const uint32_t w0 = __shfl_sync(0xffffffffu, pf[mt][r], (lane & ~3) | ((k & 7) >> 1));
+                const uint32_t w1 = __shfl_sync(0xffffffffu, pf[mt][2 + r], (lane & ~3) | ((k & 7) >> 1));
+                const uint16_t h = (uint16_t)((k < 8 ? w0 : w1) >> (k & 1 ? 16 : 0));
+                pk[mt][r] = Cvt<T>::to_f(*reinterpret_cast<const T*>(&h));
+              }
+#pragma unroll
+            for (int j = 0; j < 2 * KK; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint8_t* at = ring + cst * C::STAGE + C::PART + chunk(k, j) + (qc + e) * 2;
+                const uint16_t h = *reinterpret_cast<const uint16_t*>(at);
+                if (nonfinite_halves<T>(h) & 0xFFFFu) {
+                  const float x = Cvt<T>::to_f(*reinterpret_cast<const T*>(&h));
+#pragma unroll
+                  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                      if (vis[mt][r] >> k & 1) o[mt][j][r * 2 + e] += pk[mt][r] * x;
+                }
+              }
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      issue();
+      cst = cst + 1 == C::STAGES ? 0 : cst + 1;
+      if (cst == 0) phase ^= 1;
+    }
+    if (!ok) break;
+    // ---------------------------------------------------------------- piece done
+    const bool whole = begin == g.s0 && end == g.s1;
+    const int64_t slot = 2 * w + (begin == u0 ? 0 : 1);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float sum = l[mt][r];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int row = row_of(mt, r);
+        if (row >= rows) continue;
+        if (whole) {
+          const int a = g.rt * R + row, hq = g.h * p.G + a % p.G;
+          const int64_t tok = q0 + a / p.G;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          char* dst = p.o + tok * p.o_rs + hq * p.o_hs;
+#pragma unroll
+          for (int j = 0; j < 2 * KK; ++j)
+            *reinterpret_cast<uint32_t*>(dst + (j * 8 + qc) * 2) =
+                pack2<T>(o[mt][j][r * 2] * inv, o[mt][j][r * 2 + 1] * inv);
+          if (p.lse != nullptr && (lane & 3) == 0)
+            p.lse[tok * p.H + hq] = sum == 0.f ? -INFINITY : (m[mt][r] + log2f(sum)) * 0.69314718055994531f;
+        } else {
+          float* dst = p.part_o + (slot * R + row) * D;
+#pragma unroll
+          for (int j = 0; j < 2 * KK; ++j)
+            *reinterpret_cast<float2*>(dst + j * 8 + qc) = make_float2(o[mt][j][r * 2], o[mt][j][r * 2 + 1]);
+          if ((lane & 3) == 0) p.part_ml[slot * R + row] = make_float2(m[mt][r], sum);
+        }
+      }
+    if (begin == u0 && lane == 0) p.desc[w] = Desc{g.s0, g.s1, g.b, g.h, g.rt, begin > g.s0 ? 1 : 0};
+  }
+}
+
+// Joins the pieces of a split segment: the block of the first worker that
+// continues it does so.  O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+template <int D, typename T>
+__global__ void __launch_bounds__(128) attn_paged_join_kernel(const Params p, int R) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const int64_t U = p.head->U, N = p.head->N;
+  const int64_t c = (int64_t)blockIdx.x + 1;
+  if (c >= N) return;
+  const Desc d = p.desc[c];
+  if (!d.on) return;
+  const int64_t w0 = worker_of(d.s0, U, N), w1 = worker_of(d.s1 - 1, U, N);
+  if (w0 != c - 1) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t q0 = load_offset(p.offs, p.is64, d.b);
+  const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
+  const int rows = min(R, n * p.G - d.rt * R);
+  const int64_t first = 2 * w0 + (worker_start(w0, U, N) == d.s0 ? 0 : 1);
+  auto slot_of = [&](int64_t i) { return i == 0 ? first : 2 * (w0 + i); };
+  const int64_t pieces = w1 - w0 + 1;
+  constexpr int E = D / 32;  // columns of a lane
+  for (int row = threadIdx.x >> 5; row < rows; row += 4) {
+    float mx = -INFINITY;
+    for (int64_t i = lane; i < pieces; i += 32) mx = fmaxf(mx, p.part_ml[slot_of(i) * R + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float acc[E], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int64_t i0 = 0; i0 < pieces; i0 += 32) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (i0 + lane < pieces) ml = p.part_ml[slot_of(i0 + lane) * R + row];
+      const float wt = ex2_approx(ml.x - ref);
+      sum += wt * ml.y;
+      const int here = (int)min((int64_t)32, pieces - i0);
+#pragma unroll 4
+      for (int i = 0; i < here; ++i) {
+        const float f = __shfl_sync(0xffffffffu, wt, i);
+        const float* src = p.part_o + (slot_of(i0 + i) * R + row) * D + lane * E;
+        float x[E];
+        if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+        else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+        else x[0] = *src;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int a = d.rt * R + row, hq = d.h * p.G + a % p.G;
+    const int64_t tok = q0 + a / p.G;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = Cvt<T>::from_f(acc[e] * inv);
+    char* dst = p.o + tok * p.o_rs + hq * p.o_hs + lane * E * 2;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+    else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(y);
+    else *reinterpret_cast<T*>(dst) = y[0];
+    if (p.lse != nullptr && lane == 0)
+      p.lse[tok * p.H + hq] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+  }
+}
+
+int tile_rows(int64_t B, int64_t T, int64_t H, int64_t H_kv) {
+  return T * (H / H_kv) <= 16 * B ? 16 : 32;
+}
+int64_t max_workers() { return (int64_t)num_sms() * kWarps; }
+size_t ws_bytes(int R, int D) {
+  const int64_t N = max_workers();
+  return 64 + (size_t)N * sizeof(Desc) + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
+}
+
+int make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, bool bf16) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) {
+    set_last_error("cuTensorMapEncodeTiled is unavailable from the driver");
+    return SCREE_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  cuuint32_t box[2] = {(cuuint32_t)std::min(D, 64), (cuuint32_t)kKeys};
+  cuuint32_t es[2] = {1u, 1u};
+  CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                   const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("cuTensorMapEncodeTiled failed (CUresult %d): pool of %lld rows, D=%d", (int)r,
+                   (long long)rows, D);
+    return SCREE_ERR_CUDA;
+  }
+  return SCREE_OK;
+}
+
+template <int D, typename T, int MT>
+int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t s) {
+  auto kern = attn_paged_kernel<D, T, MT>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    SCREE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem(kMaxSeqs)));
+    attr_set[dev & 63] = true;
+  }
+  ProfScope prof(PROF_ATTN_FWD, s);
+  kern<<<(unsigned)num_sms(), kThreads, Cfg<D>::smem(p.B), s>>>(tk, tv, p);
+  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(attn_paged_join_kernel<D, T>, dim3((unsigned)max_workers() - 1), dim3(128), 0, s,
+                                  p, 16 * MT));
+  count_launch();
+  return SCREE_OK;
+}
+
+}  // namespace
+}  // namespace scree
+
+using namespace scree;
+
+extern "C" size_t scree_attn_fwd_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t H_kv, int D) {
+  if (B < 1 || T < 0 || H < 1 || H_kv < 1 || H % H_kv != 0) return 0;
+  return ws_bytes(tile_rows(B, T, H, H_kv), D);
+}
+
+extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, const scree_paged_pools* pools,
+                                    int64_t layer, const int32_t* table, const int32_t* lengths, int64_t S,
+                                    int64_t M, int64_t P, int64_t page, const int32_t* slots,
+                                    const void* offsets, int offs_is_i64, int64_t B, int64_t T, int64_t H,
+                                    int D, int dtype, float scale, const uint64_t* mask, int64_t words,
+                                    void* o, int64_t o_rs, int64_t o_hs, float* lse, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  SCREE_CHECK_ARG(pools != nullptr, "attn_fwd_paged: null pools");
+  const int64_t H_kv = pools->H;
+  SCREE_CHECK_ARG(H_kv >= 1 && H >= 1 && H % H_kv == 0 && H < 65536,
+                  "attn_fwd_paged: query heads (%lld) must be a multiple of K/V heads (%lld)", (long long)H,
+                  (long long)H_kv);
+  SCREE_CHECK_ARG(B >= 1 && B <= kMaxSeqs && T >= 0 && T < (1ll << 31) && T * (H / H_kv) < (1ll << 31),
+                  "attn_fwd_paged: bad sizes B=%lld (at most %d) T=%lld", (long long)B, kMaxSeqs, (long long)T);
+  if (D != 32 && D != 64 && D != 128) {
+    set_last_error("attn_fwd_paged: head_dim %d unsupported (32, 64, 128)", D);
+    return SCREE_ERR_UNSUPPORTED;
+  }
+  if (dtype != SCREE_F16 && dtype != SCREE_BF16) {
+    set_last_error("attn_fwd_paged: fp16 / bf16 only");
+    return SCREE_ERR_UNSUPPORTED;
+  }
+  SCREE_CHECK_ARG(pools->row_bytes == 2 * D, "attn_fwd_paged: pool rows of %lld bytes for head_dim %d",
+                  (long long)pools->row_bytes, D);
+  SCREE_CHECK_ARG(S >= 1 && M >= 1 && P >= 1 && P < (1ll << 30) && page >= kKeys && page % kKeys == 0 &&
+                      M * page < (1ll << 31),
+                  "attn_fwd_paged: bad cache sizes S=%lld M=%lld P=%lld page=%lld (a multiple of %d)",
+                  (long long)S, (long long)M, (long long)P, (long long)page, kKeys);
+  SCREE_CHECK_ARG(layer >= 0 && layer < pools->L, "attn_fwd_paged: layer %lld of %lld", (long long)layer,
+                  (long long)pools->L);
+  const int64_t pool_rows = pools->L * P * H_kv * page;
+  SCREE_CHECK_ARG(pool_rows < (1ll << 31), "attn_fwd_paged: pools of %lld rows are too large", (long long)pool_rows);
+  SCREE_CHECK_ARG(mask == nullptr || (words >= 1 && words < (1 << 20)), "attn_fwd_paged: bad mask width");
+  if (T == 0) return SCREE_OK;
+  SCREE_CHECK_ARG(q && pools->k && pools->v && table && lengths && slots && offsets && o, "attn_fwd_paged: null pointer");
+  SCREE_CHECK_ARG((uintptr_t)pools->k % 16 == 0 && (uintptr_t)pools->v % 16 == 0,
+                  "attn_fwd_paged: pools must be 16-byte aligned");
+  SCREE_CHECK_ARG((uintptr_t)q % 4 == 0 && q_rs % 2 == 0 && q_hs % 2 == 0,
+                  "attn_fwd_paged: q must be 4-byte aligned with even strides");
+  SCREE_CHECK_ARG((uintptr_t)o % 8 == 0 && o_rs % 4 == 0 && o_hs % 4 == 0,
+                  "attn_fwd_paged: output must be 8-byte aligned with strides multiple of 4");
+  SCREE_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "attn_fwd_paged: workspace must be 16-byte aligned");
+  SCREE_BIND_DEVICE(stream, q);
+  const int R = tile_rows(B, T, H, H_kv);
+  SCREE_CHECK_ARG(workspace_bytes >= ws_bytes(R, D), "attn_fwd_paged: workspace too small");
+  const bool bf16 = dtype == SCREE_BF16;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, bf16))) return rc;
+  if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, bf16))) return rc;
+  Params p;
+  p.q = (const char*)q;
+  p.q_rs = q_rs * 2;
+  p.q_hs = q_hs * 2;
+  p.offs = offsets;
+  p.is64 = offs_is_i64;
+  p.slots = slots;
+  p.table = table;
+  p.lengths = lengths;
+  p.mask = reinterpret_cast<const unsigned long long*>(mask);
+  p.words = (int)words;
+  p.B = (int)B;
+  p.S = (int)S;
+  p.M = (int)M;
+  p.P = (int)P;
+  p.page = (int)page;
+  p.H = (int)H;
+  p.Hkv = (int)H_kv;
+  p.G = (int)(H / H_kv);
+  p.T = T;
+  p.layer_row = layer * P * H_kv * page;
+  p.sl2 = scale * 1.4426950408889634f;
+  p.o = (char*)o;
+  p.o_rs = o_rs * 2;
+  p.o_hs = o_hs * 2;
+  p.lse = lse;
+  p.status = device_status_ptr();
+  char* w = (char*)workspace;
+  const int64_t N = max_workers();
+  p.head = (Head*)w;
+  p.desc = (Desc*)(w + 64);
+  p.part_ml = (float2*)(w + 64 + N * sizeof(Desc));
+  p.part_o = (float*)(w + 64 + N * sizeof(Desc) + 2 * N * R * 8);
+  cudaStream_t s = (cudaStream_t)stream;
+#define SCREE_PAGED_CASE(DD)                                                                       \
+  if (D == DD) {                                                                                   \
+    if (bf16)                                                                                      \
+      return R == 16 ? launch_paged<DD, __nv_bfloat16, 1>(tk, tv, p, s)                            \
+                     : launch_paged<DD, __nv_bfloat16, 2>(tk, tv, p, s);                           \
+    return R == 16 ? launch_paged<DD, __half, 1>(tk, tv, p, s) : launch_paged<DD, __half, 2>(tk, tv, p, s); \
+  }
+  SCREE_PAGED_CASE(128)
+  SCREE_PAGED_CASE(64)
+  SCREE_PAGED_CASE(32)
+#undef SCREE_PAGED_CASE
+  return SCREE_ERR_UNSUPPORTED;
+}

@@ -55,6 +55,25 @@ void count_launch();
     ::scree::count_launch();            \
   } while (0)
 
+// Launch of a kernel that reads what the launch before it on the stream wrote,
+// started while that one drains: the kernel executes griddepcontrol.wait before
+// its first such read, and the one before it griddepcontrol.launch_dependents.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                                    cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // Optional per-kernel timing (scree_profile_enable): CUDA events recorded on the
 // launch stream around the main kernel of an entry point.
 enum ProfKernel : int { PROF_ATTN_FWD = 0, PROF_ATTN_BWD = 1, PROF_NORM_FWD = 2, PROF_NORM_BWD = 3, PROF_GATHER = 4, PROF_N = 5 };

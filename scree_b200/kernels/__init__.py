@@ -6,6 +6,8 @@ Same call shapes as scree/kernels/reference/__init__.py:7-17 for the hot path:
   varlen_layernorm(arr, weight=None, bias=None, eps=1e-5) -> Array
                                                       reference/varlen_layernorm.py:14
   varlen_softmax(arr) -> Array                        reference/varlen_softmax.py:13
+and, without a counterpart there,
+  varlen_token_logprobs(logits, targets, top_k=0) -> TokenLogprobs of Arrays
 Every call runs the sm_100a kernels of libscree_b200 and is differentiable
 (torch autograd), like the reference's torch branch.  Output Arrays reuse the
 input's offsets object (reference/varlen_attention.py:140).
@@ -16,7 +18,8 @@ from __future__ import annotations
 from .._core import Array, _is_torch
 from . import native
 
-__all__ = ["varlen_attention", "varlen_rmsnorm", "varlen_layernorm", "varlen_softmax", "native"]
+__all__ = ["varlen_attention", "varlen_rmsnorm", "varlen_layernorm", "varlen_softmax", "varlen_token_logprobs",
+           "native"]
 
 
 def _check_cuda(arr: Array, name: str) -> None:
@@ -64,3 +67,15 @@ def varlen_softmax(arr: Array) -> Array:
         raise NotImplementedError("varlen_softmax supports ragged_dim=0 only in v0.1")
     y = native.varlen_softmax_packed(arr.values, arr.offsets)
     return Array(values=y, offsets=arr.offsets, ragged_dim=0, _host=arr._host)
+
+
+def varlen_token_logprobs(logits: Array, targets, top_k: int = 0) -> native.TokenLogprobs:
+    """Log probabilities of given tokens, entropies and top alternatives of packed
+    (T, V) logits; ``targets`` (T,) is a tensor or an Array on the same offsets.  The
+    results are Arrays on logits' offsets; differentiable."""
+    _check_cuda(logits, "varlen_token_logprobs")
+    if logits.ragged_dim != 0:
+        raise NotImplementedError("varlen_token_logprobs supports ragged_dim=0 only in v0.1")
+    t = targets.values if isinstance(targets, Array) else targets
+    r = native.token_logprobs_autograd(logits.values, t, top_k)
+    return native.TokenLogprobs(*(logits._with_values(x) for x in r))

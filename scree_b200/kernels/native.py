@@ -18,6 +18,7 @@ here synchronises with the device.
 from __future__ import annotations
 
 import math
+from typing import Any, NamedTuple
 
 import torch
 
@@ -39,6 +40,9 @@ __all__ = [
     "varlen_attention_fp32_autograd",
     "rmsnorm_qkv",
     "rmsnorm_qkv_autograd",
+    "TokenLogprobs",
+    "token_logprobs",
+    "token_logprobs_autograd",
 ]
 
 
@@ -536,3 +540,82 @@ class _RMSNormQKV(torch.autograd.Function):
 def rmsnorm_qkv_autograd(x, gamma, weight, eps: float = 1e-6):
     """Differentiable rmsnorm_qkv."""
     return _RMSNormQKV.apply(x, gamma, weight, eps)
+
+
+# --------------------------------------------------------------------------- token log probabilities
+
+
+class TokenLogprobs(NamedTuple):
+    """logp (N,) of the given tokens (0 where none is given), entropy (N,) in nats,
+    top_logp (N, k) and top_ids (N, k) int64 of the most likely tokens; fp32."""
+
+    logp: Any
+    entropy: Any
+    top_logp: Any
+    top_ids: Any
+
+
+def _logprobs_fwd(logits, targets, top_k):
+    assert logits.is_cuda and logits.ndim == 2, "logits must be a (tokens, vocabulary) CUDA tensor"
+    assert logits.dtype in (torch.float16, torch.bfloat16, torch.float32), "fp16, bf16 or fp32 only"
+    N, V = logits.shape
+    assert targets.shape == (N,) and targets.device == logits.device, "targets must be (tokens,) on logits' device"
+    assert targets.dtype in (torch.int32, torch.int64), "targets must be int32 or int64"
+    if logits.stride(1) != 1 or (N > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    targets = targets.contiguous()
+    dev, top_k = logits.device, int(top_k)
+    logp, entropy, lse = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(3))
+    top_logp = torch.empty((N, max(top_k, 0)), dtype=torch.float32, device=dev)
+    top_ids = torch.empty((N, max(top_k, 0)), dtype=torch.int64, device=dev)
+    lib, code = _lib.load(), _lib.dtype_code(logits.dtype)
+    size = lib.scree_token_logprobs_workspace_size(N, V, top_k, code)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    rc = lib.scree_token_logprobs_fwd(
+        logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, N, V,
+        top_k, code, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
+        _ptr(ws), size, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "token_logprobs")
+    return logits, targets, logp, entropy, lse, top_logp, top_ids
+
+
+def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens, entropies and the top_k (0..32) most likely
+    tokens of (N, V) logits, fp16 / bf16 / fp32 with any row stride; one read of the
+    logits.  A negative target means that no token is given (logp 0); a target >= V
+    sets the device status word.  Equal logits rank by lower index; a row whose logits
+    are all -inf has logp -inf and entropy 0.  No reference counterpart."""
+    _, _, logp, entropy, _, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
+    return TokenLogprobs(logp, entropy, top_logp, top_ids)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k):
+        logits, targets, logp, entropy, lse, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
+        ctx.save_for_backward(logits, targets, lse, entropy, top_ids)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, targets, lse, entropy, top_ids = ctx.saved_tensors
+        N, V = logits.shape
+        f32 = lambda g: None if g is None else g.to(torch.float32).contiguous()  # noqa: E731
+        g_logp, g_entropy, g_top = f32(g_logp), f32(g_entropy), f32(g_top)
+        dx = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
+        rc = _lib.load().scree_token_logprobs_bwd(
+            logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0,
+            lse.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), _ptr(g_logp), _ptr(g_entropy), _ptr(g_top),
+            N, V, top_ids.shape[1], _lib.dtype_code(logits.dtype), dx.data_ptr(), _lib.stream_ptr(logits.device))
+        if rc:
+            _lib.check(rc, "token_logprobs backward")
+        return dx, None, None
+
+
+def token_logprobs_autograd(logits, targets, top_k: int = 0) -> TokenLogprobs:
+    """Differentiable token_logprobs: the gradient of the logits from those of logp,
+    entropy and top_logp, in one pass over the logits."""
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k))
