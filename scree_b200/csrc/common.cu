@@ -83,8 +83,14 @@ static CtxGetCurrentFn ctx_get_current() {
 
 int bind_device(cudaStream_t stream, const void* ptr, DeviceGuard* guard) {
   int dev = -1;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   if (stream != nullptr && stream != cudaStreamLegacy && stream != cudaStreamPerThread) {
-    SCREE_CUDA_TRY(cudaStreamGetDevice(stream, &dev));
+    // cudaStreamGetDevice is not permitted on a stream that is being captured;
+    // the memory's device is the stream's then.
+    SCREE_CUDA_TRY(cudaStreamIsCapturing(stream, &cap));
+    if (cap == cudaStreamCaptureStatusNone) SCREE_CUDA_TRY(cudaStreamGetDevice(stream, &dev));
+  }
+  if (dev >= 0) {
   } else if (ptr != nullptr) {
     cudaPointerAttributes a;
     SCREE_CUDA_TRY(cudaPointerGetAttributes(&a, ptr));
