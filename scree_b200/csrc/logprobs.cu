@@ -1,21 +1,30 @@
 // logprobs.cu — log probabilities of given tokens, entropies and top
 // alternatives of (N, V) logits, and the gradient of the logits.
 //
-//   lse = m + log s1,  s1 = sum e^(x - m),  s2 = sum e^(x - m) (x - m),  m = max x
-//   logp = x[target] - lse,  H = -sum p log p = log s1 - s2 / s1
+//   s1 = sum e^(x - m),  s2 = sum e^(x - m) (x - m),  m = max x
+//   log p = (x - m) - log s1,  H = -sum p log p = log s1 - s2 / s1
 //   dx_v = g_logp [v = target] + sum_j g_top_j [v = id_j]
 //          - p_v (g_logp + sum_j g_top_j) - g_H p_v (log p_v + H)
 //
-// Forward: each logit is read from HBM once.  A CTA takes a slice of a row
-// (kThreads x NV 16-byte vectors), keeps it in registers as it was loaded, and
-// forms per thread the maximum, then s1 and s2 against that maximum, so there
-// is no rescaling in the element loop.  The k-th largest of the threads' maxima
-// bounds the slice's k-th largest element from below; only elements that reach
-// it (about k of them) are ranked.  Slices are joined by a second kernel, one
-// warp per row, or in place when a row is one slice.
+// Forward: each logit is read from HBM once.  Persistent CTAs stream rows
+// (segments of rows when there are few) in chunks of 16 KB: one warp copies them
+// into a ring with bulk copies, running on into the CTA's next row while the
+// other eight finish one, so 3 CTAs keep up to 192 KB per SM in flight.  Each
+// thread keeps its own maximum, s1 and s2; they are rescaled only when a chunk
+// raises the maximum.
 //
-// Numerics: sums in fp32, in units of log2 (one FMA and one ex2 per element;
-// the product x log2e is not rounded before m is subtracted).
+// Alternatives: a thread notes the maximum of its elements of each chunk (a pair:
+// thread, chunk).  After kWin chunks or at the row's end the k-th largest pair
+// maximum is found; only the k pairs that reach it can hold one of the k best
+// elements, so their elements (k x 32) are read again, from L2, and ranked with
+// the list so far.  That is once per row of up to 131,000 16-bit logits, and the
+// streaming loop pays one store per chunk.  (Pushing elements above a running
+// bound as they stream past cost 4,000 cycles each time a warp met one, twice the
+// time of a chunk.)  Floods of equal values are taken in the order of their
+// indices by a scan that stops when it has enough.
+//
+// Numerics: sums in fp32, exponents in units of log2 (one FMA and one ex2 per
+// element; the product x log2e is not rounded before m is subtracted).
 #include <algorithm>
 #include "common.cuh"
 #include "sm100.cuh"
@@ -25,7 +34,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;     // one alternative per lane when lists are merged
-constexpr int kCand = 512;      // ranked candidates of a slice; more take the slow exact path
+constexpr int kU = 4;           // vectors of a thread per chunk
+constexpr int kPairs = 512;     // pairs noted at a merge before it counts as a flood
+constexpr int kAbove = 1024;    // elements above the k-th pair maximum: fewer than kMaxTop pairs x 32
+constexpr int kTies = 256;      // elements equal to it before they count as a flood
+constexpr int kCtasPerSm = 3;
+constexpr int kStages = 3;      // ring of chunks
+constexpr int kChunkBytes = kThreads * kU * 16;
+constexpr int kWinBytes = 32 * kThreads;
+constexpr int kRingSmem = kStages * kChunkBytes + kWinBytes + 128;
+constexpr int kSiteRing = 51;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kSiteTarget = 50;
 
@@ -75,6 +93,34 @@ template <typename T> __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
+// -inf must not meet its own weight, 0 * -inf = NaN: elements below kLow are
+// raised to it, two at a time for the 16-bit types.  With |m| < kMax their weight
+// is 0 either way and (x - m) log2e is finite.  NaN stays.
+template <typename T> struct Far;
+template <> struct Far<__nv_bfloat16> {
+  static constexpr float kMax = 1e36f;
+  static __device__ __forceinline__ uint32_t two(uint32_t w) {
+    const uint32_t low = 0xFE96FE96u;  // -9.97e37
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w)); }
+};
+template <> struct Far<__half> {
+  static constexpr float kMax = 60000.f;
+  static __device__ __forceinline__ uint32_t two(uint32_t w) {
+    const uint32_t low = 0xFBFFFBFFu;  // -65504
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&w), *reinterpret_cast<const __half2*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w)); }
+};
+template <> struct Far<float> {
+  static constexpr float kMax = 1e36f;
+  static __device__ __forceinline__ uint32_t one(uint32_t w) { return __float_as_uint(max_nan(__uint_as_float(w), -1e38f)); }
+  static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w)); }
+};
+
 // Order of the alternatives: larger value first (NaN above all, -0 = +0), then
 // lower index.  Keys of valid elements are never 0.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -90,29 +136,34 @@ __device__ __forceinline__ unsigned long long order_key(float x, uint32_t idx) {
   return ((unsigned long long)order_bits(x) << 32) | (0xFFFFFFFFu - idx);
 }
 
-// Running statistics: m2 = m log2e, s1, s2 (log2 units); s1 = 0 when empty.
+// Running statistics: m, s1, and s2 in units of log2; s1 = 0 when empty.
 struct Stat {
-  float m2, s1, s2;
+  float m, s1, s2;
 };
-__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
-  Stat r;
-  r.m2 = max_nan(a.m2, b.m2);
-  const float ref = r.m2 == -INFINITY ? 0.f : r.m2;
-  // An empty side has m2 = -inf: its weight is 0 and its (finite) shift is not used.
-  const float da = fmaxf(a.m2 - ref, -1000.f), db = fmaxf(b.m2 - ref, -1000.f);
-  const float wa = ex2_approx(a.m2 - ref), wb = ex2_approx(b.m2 - ref);
-  r.s1 = a.s1 * wa + b.s1 * wb;
-  r.s2 = wa * (a.s2 + da * a.s1) + wb * (b.s2 + db * b.s1);
-  return r;
+// s1 and s2 moved from maximum m to the maximum `to` >= m.
+__device__ __forceinline__ void stat_move(Stat& s, float to) {
+  const float d = (s.m - (to == -INFINITY ? 0.f : to)) * kLog2e;
+  const float w = ex2_approx(d);
+  // An empty side has d = -inf: its weight is 0 and its (bounded) shift is not used.
+  s.s2 = w * (s.s2 + fmaxf(d, -1000.f) * s.s1);
+  s.s1 *= w;
+  s.m = to;
+}
+__device__ __forceinline__ Stat stat_join(Stat a, Stat b) {
+  const float m = max_nan(a.m, b.m);
+  stat_move(a, m);
+  stat_move(b, m);
+  return Stat{m, a.s1 + b.s1, a.s2 + b.s2};
 }
 __device__ __forceinline__ Stat stat_warp(Stat s) {
+  float m = s.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  stat_move(s, m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    Stat t;
-    t.m2 = __shfl_xor_sync(0xffffffffu, s.m2, o);
-    t.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
-    t.s2 = __shfl_xor_sync(0xffffffffu, s.s2, o);
-    s = stat_join(s, t);
+    s.s1 += __shfl_xor_sync(0xffffffffu, s.s1, o);
+    s.s2 += __shfl_xor_sync(0xffffffffu, s.s2, o);
   }
   return s;
 }
@@ -126,17 +177,6 @@ template <typename K> __device__ __forceinline__ K lane_merge(K v, int lane) {
   }
   return v;
 }
-template <typename K> __device__ __forceinline__ K lane_sort(K v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 16; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const K o = __shfl_xor_sync(0xffffffffu, v, j);
-      const bool up = ((lane & k) == 0) == ((lane & j) == 0);
-      v = up == (v > o) ? v : o;
-    }
-  return lane_merge(v, lane);
-}
 // The 32 largest of two descending lists of 32.
 template <typename K> __device__ __forceinline__ K lane_join(K a, K b, int lane) {
   const K r = __shfl_sync(0xffffffffu, b, 31 - lane);
@@ -146,15 +186,17 @@ template <typename K> __device__ __forceinline__ K lane_join(K a, K b, int lane)
 struct FwdArgs {
   const void* x;
   int64_t row_stride, N;
-  uint32_t V;
-  int slices;
+  int V;
+  int chunks, segs;  // chunks of a row, segments that they are dealt to
   const void* targets;
   int t64;
   int top;
-  float *logp, *entropy, *lse, *top_logp;
+  float *logp, *entropy;
+  float2* norm;  // maximum and log of the sum: log p = (x - norm.x) - norm.y
+  float* top_logp;
   int64_t* top_ids;
-  Stat* part;                  // (N, slices)
-  unsigned long long* part_keys;  // (N, slices, top)
+  Stat* part;                     // (N, segs)
+  unsigned long long* part_keys;  // (N, segs, top)
   int* status;
 };
 
@@ -162,11 +204,11 @@ struct FwdArgs {
 template <typename T>
 __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const Stat& s,
                                            unsigned long long key, int lane) {
-  // A row with nothing left (every logit -inf): lse = logp = -inf, H = 0.
-  const bool empty = s.m2 == -INFINITY;
-  const float lse = empty ? -INFINITY : (s.m2 + log2f(s.s1)) * kLn2;
+  // A row with nothing left (every logit -inf): logp = -inf, H = 0.
+  const bool empty = s.m == -INFINITY;
+  const float ls = log2f(s.s1) * kLn2;
   if (lane == 0) {
-    a.lse[n] = lse;
+    a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
     a.entropy[n] = empty ? 0.f : (log2f(s.s1) - s.s2 / s.s1) * kLn2;
     const int64_t t = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[n]
                             : (int64_t)reinterpret_cast<const int32_t*>(a.targets)[n];
@@ -176,216 +218,451 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const St
       lp = __uint_as_float(0x7FFFFFFFu);
     } else if (t >= 0) {
       const float x = Cvt<T>::to_f(reinterpret_cast<const T*>(a.x)[n * a.row_stride + t]);
-      lp = empty ? -INFINITY : x - lse;
+      lp = empty ? -INFINITY : (x - s.m) - ls;
     }
     a.logp[n] = lp;
   }
   if (lane < a.top) {
     a.top_ids[n * a.top + lane] = (int64_t)(0xFFFFFFFFu - (uint32_t)key);
     const float x = order_value((uint32_t)(key >> 32));
-    a.top_logp[n * a.top + lane] = empty ? -INFINITY : x - lse;
+    a.top_logp[n * a.top + lane] = empty ? -INFINITY : (x - s.m) - ls;
   }
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(const FwdArgs a) {
-  constexpr int VE = Lv<T>::N;
-  __shared__ Stat sm_stat[kThreads / 32];
-  __shared__ uint32_t sm_max[kThreads / 32][32];
-  __shared__ unsigned long long sm_cand[kCand];
-  __shared__ unsigned long long sm_top[kMaxTop];
-  __shared__ unsigned long long sm_red[kThreads / 32];
-  __shared__ int sm_count;
-  __shared__ uint32_t sm_tau;
-  asm volatile("griddepcontrol.launch_dependents;");
-  const int64_t n = blockIdx.x / (unsigned)a.slices;
-  const int slice = blockIdx.x % (unsigned)a.slices;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* row = reinterpret_cast<const T*>(a.x) + n * a.row_stride;
-  // Vectors start at 16-byte boundaries: the row begins `mis` elements into its
-  // first vector.  A vector that crosses an end of the row is read element by element.
-  const int mis = (int)(((uintptr_t)row & 15) / sizeof(T));
-  const int64_t v0 = (int64_t)slice * kThreads * NV;  // first vector of the slice
-  uint4 d[NV];
-  // Index of element 0 of vector i of this thread (may be negative or past V).
-  auto first = [&](int i) { return (v0 + i * kThreads + threadIdx.x) * VE - mis; };
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t e0 = first(i);
-    if (e0 >= 0 && e0 + VE <= (int64_t)a.V) {
-      d[i] = __ldcs(reinterpret_cast<const uint4*>(row + e0));
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = neg_inf_word<T>();
-      if (e0 + VE > 0 && e0 < (int64_t)a.V) {
-        T* el = reinterpret_cast<T*>(w);
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-          if (e0 + u >= 0 && e0 + u < (int64_t)a.V) el[u] = row[e0 + u];
-      }
-      d[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  float vm[NV], m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    vm[i] = vec_max<T>(d[i]);
-    m = max_nan(m, vm[i]);
-  }
-  Stat st{-INFINITY, 0.f, 0.f};
-  if (m != -INFINITY) {
-    st.m2 = m * kLog2e;
-    const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m2, -st.m2);
-    uint64_t s1a = 0, s1b = 0, s2a = 0, s2b = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[VE];
-      unpack_vec<T>(d[i], f);
-#pragma unroll
-      for (int u = 0; u < VE; u += 4) {
-        auto two = [&](int j, uint64_t& s1, uint64_t& s2) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(f[j], f[j + 1]), l2, nm), x0, x1);
-          const uint64_t e = f2_pack(ex2_approx(x0), ex2_approx(x1));
-          s1 = f2_add(s1, e);
-          // -inf has e = 0; the bound keeps its term 0 instead of 0 * inf.
-          s2 = f2_fma(e, f2_pack(fmaxf(x0, -1000.f), fmaxf(x1, -1000.f)), s2);
-        };
-        two(u, s1a, s2a);
-        two(u + 2, s1b, s2b);
-      }
-    }
-    float p, q;
-    f2_unpack(f2_add(s1a, s1b), p, q);
-    st.s1 = p + q;
-    f2_unpack(f2_add(s2a, s2b), p, q);
-    st.s2 = p + q;
-  }
-  st = stat_warp(st);
-  if (lane == 0) sm_stat[warp] = st;
+// Wait on the ring.  It records its own time-out but does not stop for an error
+// that another row has recorded (a target out of range spoils no other row).
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+  const bool ok = mbar_wait_impl(bar, parity, abort, nullptr, kSiteRing);
+  if (!ok) record_device_error(status, SCREE_DEVERR_WAIT_TIMEOUT, kSiteRing);
+  return ok;
+}
 
-  if (a.top > 0) {
-    // Bound: the top-th largest thread maximum (threads without a valid element count as 0).
-    const bool any = first(0) + VE > 0 && first(0) < (int64_t)a.V;
-    sm_max[warp][lane] = lane_sort<uint32_t>(any ? order_bits(m) : 0u, lane);
-    if (threadIdx.x == 0) sm_count = 0;
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t best = sm_max[0][lane];
+// Barrier of the eight working warps.
+__device__ __forceinline__ void work_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
+
+// Vector at element e0 of a row (e0 a multiple of the vector size from a 16-byte
+// boundary); elements outside [0, V) read as -inf.
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const T* row, int e0, int V) {
+  constexpr int VE = Lv<T>::N;
+  if (e0 >= 0 && e0 + VE <= V) return __ldcs(reinterpret_cast<const uint4*>(row + e0));
+  uint32_t w[4];
 #pragma unroll
-      for (int w = 1; w < kThreads / 32; ++w) best = lane_join(best, sm_max[w][lane], lane);
-      if (lane == a.top - 1) sm_tau = best;
+  for (int u = 0; u < 4; ++u) w[u] = neg_inf_word<T>();
+  if (e0 + VE > 0 && e0 < V) {
+    T* el = reinterpret_cast<T*>(w);
+#pragma unroll
+    for (int u = 0; u < VE; ++u)
+      if (e0 + u >= 0 && e0 + u < V) el[u] = row[e0 + u];
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T> constexpr int kWin = 32 / (int)sizeof(T);  // chunks of a window
+
+// The list of the `top` best keys so far and the scratch of a merge.
+struct TopList {
+  unsigned long long best[2][kMaxTop];
+  unsigned long long cand[kAbove + kTies];
+  uint32_t pair_v[kPairs];  // order_bits of the pair's maximum
+  int pair_id[kPairs];      // chunk of the window * kThreads + thread
+  uint32_t bound[kThreads / 32];
+  uint32_t tau;
+  int pairs, above, ties;
+  int cur;  // which of best[] holds the list
+};
+
+// Sum over the working threads (a barrier before and after).
+__device__ __forceinline__ int work_sum(TopList& t, int v) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) t.bound[threadIdx.x >> 5] = (uint32_t)v;
+  work_sync();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) s += (int)t.bound[w];
+  work_sync();
+  return s;
+}
+
+// Merges the window of `nch` chunks from chunk c0 on into the list.  wm: the
+// window's maxima [chunk][thread]; tm: this thread's maximum over the window.
+template <typename T>
+__device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int mis, int V, const T* wm,
+                                          int c0, int nch, float tm) {
+  constexpr int VE = Lv<T>::N, CV = kThreads * kU, E = kU * VE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto first = [&](int q, int th, int i) { return ((c0 + q) * CV + i * kThreads + th) * VE - mis; };
+  // Whether the pair has elements, and its maximum.
+  auto pair_max = [&](int q) {
+    return first(q, tid, 0) < V ? order_bits(Cvt<T>::to_f(wm[q * kThreads + tid])) : 0u;
+  };
+  // A bound from below: of the w warps that hold elements each has r = ceil(top / w)
+  // thread maxima at or above its r-th, so `top` threads reach the smallest of these.
+  {
+    const int warps = min(kThreads / 32, max(1, ((V + mis + VE - 1) / VE - c0 * CV + 31) / 32));
+    uint32_t v = first(0, tid, 0) < V ? order_bits(tm) : 0u, r = 0;
+    for (int q = (top + warps - 1) / warps; q > 0; --q) {
+      r = __reduce_max_sync(0xffffffffu, v);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, v == r)) - 1) v = 0;
     }
-    __syncthreads();
-    const uint32_t tau = sm_tau;
-    if (any && order_bits(m) >= tau) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (order_bits(vm[i]) < tau) continue;
+    if (lane == 0) t.bound[warp] = r;
+    work_sync();
+    if (tid == 0) {
+      uint32_t tau = t.bound[0];
+      for (int w = 1; w < warps; ++w) tau = min(tau, t.bound[w]);
+      // An element equal to the list's last has a higher index: it must be above.
+      const uint32_t kth = (uint32_t)(t.best[t.cur][top - 1] >> 32);
+      t.tau = kth == 0xFFFFFFFFu ? kth : max(tau, kth + 1);
+    }
+    work_sync();
+  }
+  const int cur = t.cur;
+  const uint32_t tau = t.tau;
+  for (int q = 0; q < nch; ++q) {
+    const uint32_t o = pair_max(q);
+    if (o != 0 && o >= tau) {
+      const int at = atomicAdd(&t.pairs, 1);
+      if (at < kPairs) {
+        t.pair_v[at] = o;
+        t.pair_id[at] = q * kThreads + tid;
+      }
+    }
+  }
+  if (tid < kMaxTop) t.best[cur ^ 1][tid] = 0;
+  work_sync();
+  // t2: the top-th largest pair maximum (just below tau if there are fewer pairs).
+  int n = t.pairs;
+  const bool flood = n > kPairs;
+  uint32_t t2 = tau == 0 ? 0 : tau - 1;
+  if (flood) {
+    t2 = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t at_least = t2 | (1u << bit);
+      int c = 0;
+      for (int q = 0; q < nch; ++q) c += pair_max(q) >= at_least;
+      if (work_sum(t, c) >= top) t2 = at_least;
+    }
+    if (tid == 0) t.pairs = 0;
+    work_sync();
+    for (int q = 0; q < nch; ++q) {
+      const uint32_t o = pair_max(q);
+      if (o > t2) {  // fewer than `top` pairs
+        const int at = atomicAdd(&t.pairs, 1);
+        t.pair_v[at] = o;
+        t.pair_id[at] = q * kThreads + tid;
+      }
+    }
+    work_sync();
+    n = t.pairs;
+  } else if (n >= top) {
+    for (int j = tid; j < n; j += kThreads) {
+      const uint32_t v = t.pair_v[j];
+      int above = 0, reach = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        above += t.pair_v[i] > v;
+        reach += t.pair_v[i] >= v;
+      }
+      if (above < top && reach >= top) t.tau = v;
+    }
+    work_sync();
+    t2 = t.tau;
+  }
+  // Elements of the pairs that reach t2: those above it all, those equal to it
+  // unless they come in a flood.
+  for (int j = tid; j < n * E; j += kThreads) {
+    const int p = j / E;
+    if (t.pair_v[p] < t2) continue;
+    const int id = t.pair_id[p];
+    const int e = first(id / kThreads, id % kThreads, j % E / VE) + j % VE;
+    if (e < 0 || e >= V) continue;
+    const float x = Cvt<T>::to_f(row[e]);
+    const uint32_t o = order_bits(x);
+    if (o > t2) {
+      t.cand[min(atomicAdd(&t.above, 1), kAbove - 1)] = order_key(x, (uint32_t)e);
+    } else if (o == t2 && !flood) {
+      const int at = atomicAdd(&t.ties, 1);
+      if (at < kTies) t.cand[kAbove + at] = order_key(x, (uint32_t)e);
+    }
+  }
+  work_sync();
+  const int above = t.above;
+  int ties = t.ties;
+  if (flood || ties > kTies) {
+    // Elements equal to t2 in the order of their indices, as many as can count.
+    ties = 0;
+    for (int q = 0; q < nch && ties < top; ++q)
+      for (int i = 0; i < kU && ties < top; ++i) {
+        const int e0 = first(q, tid, i);
         float f[VE];
-        unpack_vec<T>(d[i], f);
-        const int64_t e0 = first(i);
+        int mine = 0;
+        if (pair_max(q) >= t2) {
+          unpack_vec<T>(load_vec<T>(row, e0, V), f);
 #pragma unroll
-        for (int u = 0; u < VE; ++u) {
-          if (order_bits(f[u]) >= tau && e0 + u >= 0 && e0 + u < (int64_t)a.V) {
-            const int at = atomicAdd(&sm_count, 1);
-            if (at < kCand) sm_cand[at] = order_key(f[u], (uint32_t)(e0 + u));
-          }
+          for (int u = 0; u < VE; ++u) mine += e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2;
+        }
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        if (lane == 31) t.bound[warp] = (uint32_t)before;
+        work_sync();
+        int at = ties + before - mine, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+          if (w < warp) at += (int)t.bound[w];
+          all += (int)t.bound[w];
+        }
+        if (mine > 0) {
+#pragma unroll
+          for (int u = 0; u < VE; ++u)
+            if (e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2) {
+              if (at < top) t.cand[kAbove + at] = order_key(f[u], (uint32_t)(e0 + u));
+              ++at;
+            }
+        }
+        ties = min(top, ties + all);
+        work_sync();
+      }
+  }
+  // Keys differ, so a key's rank is the number of larger ones, whatever order
+  // they were noted in.
+  for (int i = tid; i < above + ties + kMaxTop; i += kThreads) {
+    const unsigned long long key = i < above          ? t.cand[i]
+                                   : i < above + ties ? t.cand[kAbove + i - above]
+                                                      : t.best[cur][i - above - ties];
+    if (key == 0) continue;
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < kMaxTop; ++j) rank += t.best[cur][j] > key;
+#pragma unroll 4
+    for (int j = 0; j < above; ++j) rank += t.cand[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < ties; ++j) rank += t.cand[kAbove + j] > key;
+    if (rank < top) t.best[cur ^ 1][rank] = key;
+  }
+  work_sync();
+  if (tid == 0) {
+    t.cur = cur ^ 1;
+    t.pairs = t.above = t.ties = 0;
+  }
+  work_sync();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(const FwdArgs a) {
+  constexpr int VE = Lv<T>::N, CV = kThreads * kU;  // elements of a vector, vectors of a chunk
+  extern __shared__ __align__(16) uint8_t ring[];
+  T* wm = reinterpret_cast<T*>(ring + kStages * kChunkBytes);  // a window's maxima
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kChunkBytes + kWinBytes);
+  uint64_t* empty = full + kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  __shared__ Stat sm_stat[2][kThreads / 32];
+  __shared__ TopList tl;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kThreads / 32);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int64_t items = a.N * a.segs;
+  // Vectors start at 16-byte boundaries: a row begins `mis` elements into its
+  // first vector; vectors [1 if mis, (V + mis) / VE) lie inside the row and go
+  // through the ring, the two at its ends are read element by element.
+  auto row_of = [&](int64_t n) { return reinterpret_cast<const T*>(a.x) + n * a.row_stride; };
+  auto mis_of = [](const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); };
+  auto seg_begin = [&](int64_t seg) { return (int)((int64_t)a.chunks * seg / a.segs); };
+
+  if (warp == kThreads / 32) {
+    // ---------------------------------------------------------------- copies
+    if (lane != 0) return;
+    int k = 0;  // chunks issued
+    bool ok = true;
+    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const T* row = row_of(item / a.segs);
+      const int seg = (int)(item % a.segs), mis = mis_of(row);
+      const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
+      for (int c = seg_begin(seg); c < seg_begin(seg + 1); ++c, ++k) {
+        const int st = k % kStages;
+        if (k >= kStages &&
+            !(ok = ring_wait(&empty[st], ((k / kStages) - 1) & 1, abort_flag, a.status)))
+          break;
+        const int lo = max(c * CV, v_lo), hi = min((c + 1) * CV, v_hi);
+        if (lo < hi) {
+          mbar_expect_tx(&full[st], (uint32_t)(hi - lo) * 16);
+          bulk_load_1d(ring + st * kChunkBytes + (lo - c * CV) * 16, row + (int64_t)lo * VE - mis,
+                       (uint32_t)(hi - lo) * 16, &full[st]);
+        } else {
+          mbar_arrive(&full[st]);
         }
       }
     }
-    __syncthreads();
-    const int cnt = sm_count;
-    if (threadIdx.x < kMaxTop) sm_top[threadIdx.x] = 0;
-    __syncthreads();
-    if (cnt <= kCand) {
-      // Keys differ, so a candidate's rank is the number of larger ones, whatever
-      // order the candidates arrived in.
-      for (int i = threadIdx.x; i < cnt; i += kThreads) {
-        const unsigned long long key = sm_cand[i];
-        int rank = 0;
-        for (int j = 0; j < cnt; ++j) rank += sm_cand[j] > key;
-        if (rank < a.top) sm_top[rank] = key;
-      }
-      __syncthreads();
-    } else {
-      // Many equal elements: take the largest remaining key, `top` times.
-      unsigned long long last = ~0ull;
-      for (int r = 0; r < a.top; ++r) {
-        unsigned long long best = 0;
+    if (!ok) {  // give copies in flight time to land before the CTA ends
+      volatile int quiet = 0;
+      for (int i = max(0, k - kStages); i < k; ++i)
+        mbar_wait_impl(&full[i % kStages], (i / kStages) & 1, &quiet, nullptr, kSiteRing);
+    }
+    return;
+  }
+
+  int k = 0;  // chunks taken
+  int parity = 0;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t n = item / a.segs;
+    const int seg = (int)(item % a.segs);
+    const int c0 = seg_begin(seg), c1 = seg_begin(seg + 1);
+    const T* row = row_of(n);
+    const int mis = mis_of(row);
+    const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
+    Stat st{-INFINITY, 0.f, 0.f};
+    // Warp 0, which has read the item before's list, starts this one's; the others
+    // touch it behind the first chunk's barrier.
+    if (a.top > 0 && warp == 0) {
+      tl.best[0][lane] = 0;
+      if (lane == 0) tl.pairs = tl.above = tl.ties = tl.cur = 0;
+    }
+    float tm = -INFINITY;  // this thread's maximum over the window
+    int wn = 0;            // chunks of the window so far
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c, ++k) {
+      // A wait that gives up has set the status word; the work runs on (its
+      // results do not count) so that all threads meet at the barriers.
+      const int slot = k % kStages;
+      ring_wait(&full[slot], (k / kStages) & 1, abort_flag, a.status);
+      const uint4* src = reinterpret_cast<const uint4*>(ring + slot * kChunkBytes);
+      auto vec = [&](int i) {
+        const int v = c * CV + i * kThreads + (int)threadIdx.x;
+        return v >= v_lo && v < v_hi ? src[i * kThreads + threadIdx.x] : load_vec<T>(row, v * VE - mis, a.V);
+      };
+      uint4 d[kU];
+      if (c * CV >= v_lo && (c + 1) * CV <= v_hi) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        for (int i = 0; i < kU; ++i) d[i] = src[i * kThreads + threadIdx.x];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kU; ++i) d[i] = vec(i);
+      }
+      float cm = vec_max<T>(d[0]);
+#pragma unroll
+      for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
+      if (!(cm <= st.m)) stat_move(st, cm);
+      if (!(fabsf(st.m) >= Far<T>::kMax)) {
+        const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
+        uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < kU; ++i) {
           float f[VE];
-          unpack_vec<T>(d[i], f);
-          const int64_t e0 = first(i);
+          unpack_vec<T>(Far<T>::raise(d[i]), f);
+#pragma unroll
+          for (int u = 0; u < VE; u += 2) {
+            const uint64_t t = f2_fma(f2_pack(f[u], f[u + 1]), l2, nm);
+            float t0, t1;
+            f2_unpack(t, t0, t1);
+            const uint64_t e = f2_pack(ex2_approx(t0), ex2_approx(t1));
+            s1[(u >> 1) & 1] = f2_add(s1[(u >> 1) & 1], e);
+            s2[(u >> 1) & 1] = f2_fma(e, t, s2[(u >> 1) & 1]);
+          }
+        }
+        float x, y;
+        f2_unpack(f2_add(s1[0], s1[1]), x, y);
+        st.s1 += x + y;
+        f2_unpack(f2_add(s2[0], s2[1]), x, y);
+        st.s2 += x + y;
+      } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
+        // A maximum near the type's lowest value (a masked row), where m log2e may
+        // overflow and -inf differs from the lowest value; or an infinity.
+#pragma unroll 1
+        for (int i = 0; i < kU; ++i) {
+          float f[VE];
+          unpack_vec<T>(vec(i), f);
 #pragma unroll
           for (int u = 0; u < VE; ++u) {
-            if (e0 + u < 0 || e0 + u >= (int64_t)a.V) continue;
-            const unsigned long long key = order_key(f[u], (uint32_t)(e0 + u));
-            if (key < last && key > best) best = key;
+            const float t = (f[u] - st.m) * kLog2e, e = ex2_approx(t);
+            st.s1 += e;
+            st.s2 = fmaf(e, fmaxf(t, -1000.f), st.s2);
           }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const unsigned long long t = __shfl_xor_sync(0xffffffffu, best, o);
-          best = t > best ? t : best;
-        }
-        if (lane == 0) sm_red[warp] = best;
-        __syncthreads();
-        best = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) best = sm_red[w] > best ? sm_red[w] : best;
-        if (threadIdx.x == 0) sm_top[r] = best;
-        last = best;
-        __syncthreads();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+      if (a.top == 0) continue;
+      wm[wn * kThreads + threadIdx.x] = Cvt<T>::from_f(cm);  // exact: an element's value
+      tm = max_nan(tm, cm);
+      if (++wn == kWin<T> || c + 1 == c1) {
+        merge_window<T>(tl, a.top, row, mis, a.V, wm, c + 1 - wn, wn, tm);
+        wn = 0;
+        tm = -INFINITY;
       }
     }
-  } else {
-    __syncthreads();
-  }
-  if (warp == 0) {
-    Stat s = lane < kThreads / 32 ? sm_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-    s = stat_warp(s);
-    if (a.slices == 1) {
-      finish_row<T>(a, n, s, lane < a.top ? sm_top[lane] : 0, lane);
-    } else {
-      if (lane == 0) a.part[n * a.slices + slice] = s;
-      if (lane < a.top) a.part_keys[(n * a.slices + slice) * a.top + lane] = sm_top[lane];
+    st = stat_warp(st);
+    if (lane == 0) sm_stat[parity][warp] = st;
+    work_sync();
+    // Warp 0 finishes the item while the others begin the next (they write the
+    // other half of sm_stat, and this half only behind that item's barrier).
+    if (warp == 0) {
+      Stat s = lane < kThreads / 32 ? sm_stat[parity][lane] : Stat{-INFINITY, 0.f, 0.f};
+      s = stat_warp(s);
+      const unsigned long long key = lane < a.top ? tl.best[tl.cur][lane] : 0;
+      if (a.segs == 1) {
+        finish_row<T>(a, n, s, key, lane);
+      } else {
+        if (lane == 0) a.part[n * a.segs + seg] = s;
+        if (lane < a.top) a.part_keys[(n * a.segs + seg) * a.top + lane] = key;
+      }
+      __syncwarp();
     }
+    parity ^= 1;
   }
 }
 
-// One warp per row joins the slices.
+// Joins a row's segments, the lists dealt to four warps.
+constexpr int kJoinWarps = 4;
 template <typename T>
-__global__ void __launch_bounds__(128) logprobs_join_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) logprobs_join_kernel(const FwdArgs a) {
+  __shared__ unsigned long long lists[kJoinWarps][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (n >= a.N) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = blockIdx.x;
   Stat s{-INFINITY, 0.f, 0.f};
-  for (int j = lane; j < a.slices; j += 32) s = stat_join(s, a.part[n * a.slices + j]);
-  s = stat_warp(s);
+  if (warp == 0) {
+    for (int j = lane; j < a.segs; j += 32) s = stat_join(s, a.part[n * a.segs + j]);
+    s = stat_warp(s);
+  }
   unsigned long long best = 0;
   if (a.top > 0) {
-    const unsigned long long* keys = a.part_keys + n * a.slices * a.top;
-    for (int j = 0; j < a.slices; ++j) {
+    const unsigned long long* keys = a.part_keys + n * a.segs * a.top;
+    for (int j = warp; j < a.segs; j += kJoinWarps) {
       const unsigned long long k = lane < a.top ? keys[(int64_t)j * a.top + lane] : 0;
-      best = j == 0 ? k : lane_join(best, k, lane);
+      best = j == warp ? k : lane_join(best, k, lane);
     }
+    lists[warp][lane] = best;
+    __syncthreads();
+    if (warp == 0)
+      for (int w = 1; w < kJoinWarps; ++w) best = lane_join(best, lists[w][lane], lane);
   }
-  finish_row<T>(a, n, s, best, lane);
+  if (warp == 0) finish_row<T>(a, n, s, best, lane);
 }
 
 struct BwdArgs {
   const void* x;
   int64_t row_stride, N;
-  uint32_t V;
+  int V;
   int slices;
   const void* targets;
   int t64;
   int top;
-  const float *lse, *entropy;
+  const float2* norm;
+  const float* entropy;
   const int64_t* top_ids;
   const float *g_logp, *g_entropy, *g_top;  // each may be null
   void* dx;                                 // (N, V) contiguous
@@ -403,33 +680,17 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   T* out = reinterpret_cast<T*>(a.dx) + n * (int64_t)a.V;
   const int mis = (int)(((uintptr_t)row & 15) / sizeof(T));
   const bool same = (((uintptr_t)row ^ (uintptr_t)out) & 15) == 0;
-  const int64_t v0 = (int64_t)slice * kThreads * NV;
+  const int v0 = slice * kThreads * NV;  // first vector of the slice
   uint4 d[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t e0 = (v0 + i * kThreads + threadIdx.x) * VE - mis;
-    if (e0 >= 0 && e0 + VE <= (int64_t)a.V) {
-      d[i] = __ldcs(reinterpret_cast<const uint4*>(row + e0));
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = neg_inf_word<T>();
-      if (e0 + VE > 0 && e0 < (int64_t)a.V) {
-        T* el = reinterpret_cast<T*>(w);
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-          if (e0 + u >= 0 && e0 + u < (int64_t)a.V) el[u] = row[e0 + u];
-      }
-      d[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
+  for (int i = 0; i < NV; ++i) d[i] = load_vec<T>(row, (v0 + i * kThreads + (int)threadIdx.x) * VE - mis, a.V);
   // The given token and the alternatives as one list of (index, weight): entry 0
   // is the target, entry 1 + j alternative j; index -1 has no weight.
   auto entry = [&](int j, int64_t& idx) -> float {
     if (j == 0) {
       idx = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[n]
                   : (int64_t)reinterpret_cast<const int32_t*>(a.targets)[n];
-      if (idx < 0 || idx >= (int64_t)a.V || a.g_logp == nullptr) idx = -1;
+      if (idx < 0 || idx >= a.V || a.g_logp == nullptr) idx = -1;
       return idx < 0 ? 0.f : a.g_logp[n];
     }
     idx = a.top_ids[n * a.top + j - 1];
@@ -445,32 +706,33 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
     if (threadIdx.x == 0) sm_gs = g;
   }
   __syncthreads();
-  const float lse = a.lse[n];
+  const float2 nm = a.norm[n];
   const float gh = a.g_entropy != nullptr ? a.g_entropy[n] : 0.f;
-  const bool empty = lse == -INFINITY;  // nothing left in the row: no gradient
+  const bool empty = nm.x == -INFINITY;  // nothing left in the row: no gradient
   const float base = sm_gs + gh * a.entropy[n];
-  const float l2 = lse * kLog2e;
+  const float l2 = (nm.x + nm.y) * kLog2e, s2 = nm.y * kLog2e;
+  const bool far = fabsf(nm.x) >= 1e37f;  // the product with log2e may overflow (rows of the lowest value)
   auto grad = [&](float x) {
-    const float d2 = fmaf(x, kLog2e, -l2);  // log2 p
+    const float d2 = far ? fmaf(x - nm.x, kLog2e, -s2) : fmaf(x, kLog2e, -l2);  // log2 p
     // The bound only matters at p = 0, where it keeps 0 * inf out.
     return -ex2_approx(d2) * fmaf(gh, fmaxf(d2, -1000.f) * kLn2, base);
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t e0 = (v0 + i * kThreads + threadIdx.x) * VE - mis;
-    if (e0 + VE <= 0 || e0 >= (int64_t)a.V) continue;
+    const int e0 = (v0 + i * kThreads + (int)threadIdx.x) * VE - mis;
+    if (e0 + VE <= 0 || e0 >= a.V) continue;
     float f[VE];
     unpack_vec<T>(d[i], f);
 #pragma unroll
     for (int u = 0; u < VE; ++u) f[u] = empty ? 0.f : grad(f[u]);
     __align__(16) T o[VE];
     cvt_from_f<T, VE>(f, o);
-    if (same && e0 >= 0 && e0 + VE <= (int64_t)a.V) {
+    if (same && e0 >= 0 && e0 + VE <= a.V) {
       __stcs(reinterpret_cast<uint4*>(out + e0), *reinterpret_cast<const uint4*>(o));
     } else {
 #pragma unroll
       for (int u = 0; u < VE; ++u)
-        if (e0 + u >= 0 && e0 + u < (int64_t)a.V) out[e0 + u] = o[u];
+        if (e0 + u >= 0 && e0 + u < a.V) out[e0 + u] = o[u];
     }
   }
   // The listed elements of this slice, written again with their weights (after
@@ -479,8 +741,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   if (threadIdx.x < entries && !empty) {
     int64_t idx;
     entry(threadIdx.x, idx);
-    const int64_t lo = v0 * VE - mis;
-    if (idx >= 0 && idx >= lo && idx < lo + (int64_t)kThreads * NV * VE) {
+    const int lo = v0 * VE - mis;
+    if (idx >= 0 && idx >= lo && idx < lo + kThreads * NV * VE) {
       float g = 0.f;
       for (int j = 0; j < entries; ++j) {
         int64_t other;
@@ -492,34 +754,48 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   }
 }
 
-constexpr int kNV = 8;
-template <typename T> int64_t slice_elems() { return (int64_t)kThreads * kNV * Lv<T>::N; }
-int64_t row_slices(int64_t V, int dtype) {
-  const int64_t per = dtype == SCREE_F32 ? slice_elems<float>() : slice_elems<__half>();
-  const int64_t lead = dtype == SCREE_F32 ? 3 : 7;  // a row may begin inside its first vector
-  return (V + lead + per - 1) / per;
+// Vectors of a row (which may begin inside its first one).
+int64_t row_vecs(int64_t V, int dtype) {
+  const int64_t ve = 16 / (int64_t)dtype_size(dtype);
+  return (V + ve - 1 + ve - 1) / ve;
 }
+int64_t row_chunks(int64_t V, int dtype) { return (row_vecs(V, dtype) + kThreads * kU - 1) / (kThreads * kU); }
+// A CTA per row once there are four rounds of them; fewer rows are cut so that
+// there are as many segments (or chunks of one).
+int64_t row_segs(int64_t N, int64_t V, int dtype) {
+  const int64_t want = 4 * kCtasPerSm * (int64_t)num_sms();
+  return std::max<int64_t>(1, std::min(row_chunks(V, dtype), (want + N - 1) / std::max<int64_t>(N, 1)));
+}
+constexpr int kNV = 8;  // vectors of a thread, backward
+int64_t bwd_slices(int64_t V, int dtype) { return (row_vecs(V, dtype) + kThreads * kNV - 1) / (kThreads * kNV); }
 
 int check_sizes(const char* what, int64_t N, int64_t V, int64_t row_stride, int top, int dtype) {
   SCREE_CHECK_ARG(dtype == SCREE_F16 || dtype == SCREE_BF16 || dtype == SCREE_F32,
                   "%s: fp16, bf16 or fp32 only", what);
-  SCREE_CHECK_ARG(N >= 0 && V >= 1 && V < (1ll << 31), "%s: bad sizes N=%lld V=%lld", what,
+  SCREE_CHECK_ARG(N >= 0 && V >= 1 && V < (1ll << 30), "%s: bad sizes N=%lld V=%lld", what,
                   (long long)N, (long long)V);
   SCREE_CHECK_ARG(row_stride >= V || N <= 1, "%s: rows overlap (row stride %lld, V=%lld)", what,
                   (long long)row_stride, (long long)V);
   SCREE_CHECK_ARG(top >= 0 && top <= kMaxTop && top <= V,
                   "%s: top must be between 0 and %d and at most V (got %d)", what, kMaxTop, top);
-  SCREE_CHECK_ARG(N * row_slices(V, dtype) < (1ll << 31), "%s: N=%lld too large", what,
+  SCREE_CHECK_ARG(N * row_chunks(V, dtype) < (1ll << 31), "%s: N=%lld too large", what,
                   (long long)N);
   return SCREE_OK;
 }
 
 template <typename T> int launch_fwd(const FwdArgs& a, cudaStream_t s) {
-  logprobs_slice_kernel<T, kNV><<<(unsigned)(a.N * a.slices), kThreads, 0, s>>>(a);
-  SCREE_LAUNCH_CHECK();
-  if (a.slices > 1) {
-    SCREE_CUDA_TRY(launch_dependent(logprobs_join_kernel<T>, dim3((unsigned)((a.N + 3) / 4)),
-                                    dim3(128), 0, s, a));
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    SCREE_CUDA_TRY(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    attr_set[dev & 63] = true;
+  }
+  const unsigned grid = (unsigned)std::min<int64_t>(a.N * a.segs, (int64_t)kCtasPerSm * num_sms());
+  SCREE_CUDA_TRY(launch_dependent(logprobs_kernel<T>, dim3(grid), dim3(kThreads + 32), kRingSmem, s, a));
+  count_launch();
+  if (a.segs > 1) {
+    SCREE_CUDA_TRY(launch_dependent(logprobs_join_kernel<T>, dim3((unsigned)a.N), dim3(kJoinWarps * 32), 0, s, a));
     count_launch();
   }
   return SCREE_OK;
@@ -536,22 +812,23 @@ template <typename T> int launch_bwd(const BwdArgs& a, cudaStream_t s) {
 using namespace scree;
 
 extern "C" size_t scree_token_logprobs_workspace_size(int64_t N, int64_t V, int top, int dtype) {
-  const int64_t sl = row_slices(V, dtype);
-  if (N <= 0 || V <= 0 || sl == 1) return 0;
-  return (size_t)(N * sl) * (16 + 8 * (size_t)(top > 0 ? top : 0));
+  if (N <= 0 || V <= 0 || dtype_size(dtype) == 0) return 0;
+  const int64_t segs = row_segs(N, V, dtype);
+  return segs == 1 ? 0 : (size_t)(N * segs) * (16 + 8 * (size_t)(top > 0 ? top : 0));
 }
 
 extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, const void* targets,
                                         int targets_is_i64, int64_t N, int64_t V, int top,
-                                        int dtype, float* logp, float* entropy, float* lse,
+                                        int dtype, float* logp, float* entropy, float* norm,
                                         float* top_logp, int64_t* top_ids, void* workspace,
                                         size_t workspace_bytes, void* stream) {
   int rc = check_sizes("token_logprobs", N, V, row_stride, top, dtype);
   if (rc != SCREE_OK) return rc;
   if (N == 0) return SCREE_OK;
-  SCREE_CHECK_ARG(logits && targets && logp && entropy && lse && (top == 0 || (top_logp && top_ids)),
+  SCREE_CHECK_ARG(logits && targets && logp && entropy && norm && (top == 0 || (top_logp && top_ids)),
                   "token_logprobs: null pointer");
-  SCREE_CHECK_ARG((uintptr_t)logits % dtype_size(dtype) == 0, "token_logprobs: misaligned logits");
+  SCREE_CHECK_ARG((uintptr_t)logits % dtype_size(dtype) == 0 && (uintptr_t)norm % 8 == 0,
+                  "token_logprobs: misaligned logits or norm");
   const size_t need = scree_token_logprobs_workspace_size(N, V, top, dtype);
   SCREE_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
                   "token_logprobs: workspace too small");
@@ -560,18 +837,19 @@ extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, 
   a.x = logits;
   a.row_stride = row_stride;
   a.N = N;
-  a.V = (uint32_t)V;
-  a.slices = (int)row_slices(V, dtype);
+  a.V = (int)V;
+  a.chunks = (int)row_chunks(V, dtype);
+  a.segs = (int)row_segs(N, V, dtype);
   a.targets = targets;
   a.t64 = targets_is_i64;
   a.top = top;
   a.logp = logp;
   a.entropy = entropy;
-  a.lse = lse;
+  a.norm = (float2*)norm;
   a.top_logp = top_logp;
   a.top_ids = top_ids;
   a.part_keys = reinterpret_cast<unsigned long long*>(workspace);
-  a.part = reinterpret_cast<Stat*>(reinterpret_cast<char*>(workspace) + 8 * (size_t)(N * a.slices) * top);
+  a.part = reinterpret_cast<Stat*>(reinterpret_cast<char*>(workspace) + 8 * (size_t)(N * a.segs) * top);
   a.status = device_status_ptr();
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == SCREE_F32) return launch_fwd<float>(a, s);
@@ -579,7 +857,7 @@ extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, 
 }
 
 extern "C" int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, const void* targets,
-                                        int targets_is_i64, const float* lse, const float* entropy,
+                                        int targets_is_i64, const float* norm, const float* entropy,
                                         const int64_t* top_ids, const float* g_logp,
                                         const float* g_entropy, const float* g_top, int64_t N,
                                         int64_t V, int top, int dtype, void* d_logits,
@@ -587,21 +865,22 @@ extern "C" int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, 
   int rc = check_sizes("token_logprobs backward", N, V, row_stride, top, dtype);
   if (rc != SCREE_OK) return rc;
   if (N == 0) return SCREE_OK;
-  SCREE_CHECK_ARG(logits && targets && lse && entropy && d_logits && (top == 0 || g_top == nullptr || top_ids),
+  SCREE_CHECK_ARG(logits && targets && norm && entropy && d_logits && (top == 0 || g_top == nullptr || top_ids),
                   "token_logprobs backward: null pointer");
-  SCREE_CHECK_ARG((uintptr_t)logits % dtype_size(dtype) == 0 && (uintptr_t)d_logits % dtype_size(dtype) == 0,
-                  "token_logprobs backward: misaligned logits");
+  SCREE_CHECK_ARG((uintptr_t)logits % dtype_size(dtype) == 0 && (uintptr_t)d_logits % dtype_size(dtype) == 0 &&
+                      (uintptr_t)norm % 8 == 0,
+                  "token_logprobs backward: misaligned logits or norm");
   SCREE_BIND_DEVICE(stream, logits);
   BwdArgs a;
   a.x = logits;
   a.row_stride = row_stride;
   a.N = N;
-  a.V = (uint32_t)V;
-  a.slices = (int)row_slices(V, dtype);
+  a.V = (int)V;
+  a.slices = (int)bwd_slices(V, dtype);
   a.targets = targets;
   a.t64 = targets_is_i64;
   a.top = top;
-  a.lse = lse;
+  a.norm = (const float2*)norm;
   a.entropy = entropy;
   a.top_ids = top_ids;
   a.g_logp = g_logp;

@@ -565,7 +565,8 @@ def _logprobs_fwd(logits, targets, top_k):
         logits = logits.contiguous()
     targets = targets.contiguous()
     dev, top_k = logits.device, int(top_k)
-    logp, entropy, lse = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(3))
+    logp, entropy = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
+    norm = torch.empty((N, 2), dtype=torch.float32, device=dev)  # kept for the gradient
     top_logp = torch.empty((N, max(top_k, 0)), dtype=torch.float32, device=dev)
     top_ids = torch.empty((N, max(top_k, 0)), dtype=torch.int64, device=dev)
     lib, code = _lib.load(), _lib.dtype_code(logits.dtype)
@@ -573,11 +574,11 @@ def _logprobs_fwd(logits, targets, top_k):
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     rc = lib.scree_token_logprobs_fwd(
         logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, N, V,
-        top_k, code, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
+        top_k, code, logp.data_ptr(), entropy.data_ptr(), norm.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
         _ptr(ws), size, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "token_logprobs")
-    return logits, targets, logp, entropy, lse, top_logp, top_ids
+    return logits, targets, logp, entropy, norm, top_logp, top_ids
 
 
 def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
@@ -593,22 +594,22 @@ def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
-        logits, targets, logp, entropy, lse, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
-        ctx.save_for_backward(logits, targets, lse, entropy, top_ids)
+        logits, targets, logp, entropy, norm, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
+        ctx.save_for_backward(logits, targets, norm, entropy, top_ids)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
     def backward(ctx, g_logp, g_entropy, g_top, _):
-        logits, targets, lse, entropy, top_ids = ctx.saved_tensors
+        logits, targets, norm, entropy, top_ids = ctx.saved_tensors
         N, V = logits.shape
         f32 = lambda g: None if g is None else g.to(torch.float32).contiguous()  # noqa: E731
         g_logp, g_entropy, g_top = f32(g_logp), f32(g_entropy), f32(g_top)
         dx = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
         rc = _lib.load().scree_token_logprobs_bwd(
             logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0,
-            lse.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), _ptr(g_logp), _ptr(g_entropy), _ptr(g_top),
+            norm.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), _ptr(g_logp), _ptr(g_entropy), _ptr(g_top),
             N, V, top_ids.shape[1], _lib.dtype_code(logits.dtype), dx.data_ptr(), _lib.stream_ptr(logits.device))
         if rc:
             _lib.check(rc, "token_logprobs backward")

@@ -29,9 +29,10 @@ def _status():
 def _ref(x, t, k):
     """x (N, V) float64 on any device, t (N,) -> logp, H, lse, top ids (definition, NaN first)."""
     m = x.amax(1)
-    lse = torch.logsumexp(x, 1)
     empty = m == -np.inf
-    lp = x - lse[:, None]
+    rest = torch.logsumexp(x - m[:, None], 1)  # apart from m: it may be too large to add to in 64 bits
+    lse = m + rest
+    lp = (x - m[:, None]) - rest[:, None]
     lp[empty] = -np.inf
     p = torch.where(empty[:, None], torch.zeros_like(lp), lp.exp())
     H = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(1)
@@ -119,14 +120,27 @@ def test_ties_rank_by_lower_index(cuda):
     _check(x, t, 32, r, x.double())
 
 
-def test_masked_infinite_and_nan_logits(cuda):
+def test_rows_that_rise_along_the_vocabulary(cuda):
+    """Every element beats all before it: the candidate buffer overflows."""
+    from scree_b200.kernels.native import token_logprobs
+
+    x = torch.arange(60000, dtype=torch.float32, device=cuda).mul(1e-3).repeat(3, 1)
+    x[1] = x[1].flip(0)
+    t = torch.tensor([59999, 0, 5], device=cuda)
+    _check(x, t, 32, token_logprobs(x, t, top_k=32), x.double())
+    y = x.to(torch.bfloat16)  # steps of equal values
+    _check(y, t, 32, token_logprobs(y, t, top_k=32), y.double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_masked_infinite_and_nan_logits(cuda, dtype):
     from scree_b200.kernels.native import token_logprobs, token_logprobs_autograd
 
-    x, t = _logits(8, 20000, torch.float16, cuda, seed=5)
+    x, t = _logits(8, 20000, dtype, cuda, seed=5)
     x[0, 100:] = -np.inf          # most of the vocabulary masked
     x[1] = -np.inf                # nothing left
-    x[2] = torch.finfo(torch.float16).min  # masked by the type's lowest value throughout
-    x[3, 7:] = torch.finfo(torch.float16).min
+    x[2] = torch.finfo(dtype).min  # masked by the type's lowest value throughout
+    x[3, 7:] = torch.finfo(dtype).min
     x[4, 5] = np.nan
     x[5, 19999] = np.inf
     x[6, :] = -np.inf
