@@ -18,16 +18,14 @@
 // key hide under that).  A group is 16 keys because that is the contraction of
 // one mma and pages hold multiples of it, so a group never spans pages.
 #include <algorithm>
-#include "attn_common.cuh"
+#include "attn_paged.cuh"
 
 namespace scree {
 namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kKeys = 16;            // keys of a group
-constexpr int kMaxSeqs = 4096;       // prefix of the segments in shared memory
-constexpr int kSitePagedAttn = 70, kSitePagedAttnPage = 71, kSitePagedAttnWait = 72;
+constexpr int kKeys = kPagedKeys;    // keys of a group
 
 template <int D> struct Cfg {
   static constexpr int ROWB = D >= 64 ? 128 : 64;  // bytes of a box row (= swizzle span)
@@ -41,42 +39,6 @@ template <int D> struct Cfg {
     return 1024 + RING + kWarps * STAGES * 8 + 64 + (int)(B + 1) * 8;
   }
 };
-
-struct Params {
-  const char* q;
-  int64_t q_rs, q_hs;  // bytes
-  const void* offs;
-  int is64;
-  const int32_t *slots, *table, *lengths;
-  const unsigned long long* mask;
-  int words;
-  int B, S, M, P, page;
-  int H, Hkv, G;
-  int64_t T;
-  int64_t layer_row;  // first row of the layer in the pools' row view
-  float sl2;          // scale log2 e
-  char* o;
-  int64_t o_rs, o_hs;
-  float* lse;
-  int* status;
-  struct Head* head;
-  struct Desc* desc;
-  float2* part_ml;  // [slot][R]
-  float* part_o;    // [slot][R][D]
-};
-struct Head {
-  int64_t U, N;
-};
-struct Desc {  // the segment that a worker's first piece continues
-  int64_t s0, s1;
-  int32_t b, h, rt, on;
-};
-
-// First unit of worker w and the worker that holds unit u.
-__device__ __forceinline__ int64_t worker_start(int64_t w, int64_t U, int64_t N) { return w * U / N; }
-__device__ __forceinline__ int64_t worker_of(int64_t u, int64_t U, int64_t N) {
-  return ((u + 1) * N - 1) / U;
-}
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -103,105 +65,34 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
   cvt_from_f<T, 2>(f, o);
   return (uint32_t)*reinterpret_cast<uint16_t*>(&o[0]) | ((uint32_t)*reinterpret_cast<uint16_t*>(&o[1]) << 16);
 }
-// All ones in the exponent: infinity or NaN, of either half of a word.
-template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
-  constexpr uint32_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
-  return ((w & E) == E ? 0xFFFFu : 0u) | (((w >> 16) & E) == E ? 0xFFFF0000u : 0u);
-}
-
-// 16-bit visibility of keys [k0, k0 + 16) for query i of a sequence: all keys
-// before c0 = len - n, of the n new ones those of the mask row (or j <= i).
-__device__ __forceinline__ uint32_t visible16(const Params& p, int64_t row, int i, int k0, int c0, int len) {
-  uint32_t v = 0xFFFFu;
-  const int t0 = k0 - c0;  // tree index of key k0
-  if (t0 > -kKeys) {
-    if (p.mask == nullptr) {
-      const int last = i - t0;  // last visible key of the group
-      v = last >= 15 ? 0xFFFFu : last < 0 ? 0u : (2u << last) - 1;
-    } else {
-      const unsigned long long* m = p.mask + row * p.words;
-      unsigned long long bits;
-      if (t0 < 0) {
-        bits = (m[0] << -t0) | ((1ull << -t0) - 1);
-      } else {
-        const int w = t0 >> 6, o = t0 & 63;
-        bits = w < p.words ? m[w] >> o : 0ull;
-        if (o > 48 && w + 1 < p.words) bits |= m[w + 1] << (64 - o);
-      }
-      v = (uint32_t)bits & 0xFFFFu;
-    }
-  }
-  const int left = len - k0;
-  return left >= 16 ? v : v & ((1u << left) - 1);
-}
-
 template <int D, typename T, int MT>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const Params p) {
+                      const PagedParams p) {
   using C = Cfg<D>;
   constexpr int R = 16 * MT;
   constexpr int KK = D / 16;  // k-steps of Q K^T = pairs of 8-column tiles of O
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kWarps * C::STAGES);
   int64_t* pre = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars + kWarps * C::STAGES) + 64);
-  __shared__ int64_t warp_sum[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
   if (threadIdx.x < kWarps * C::STAGES) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) *abort_flag = 0;
   fence_mbar_init();
-  bool bad = p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0;
-  const bool stopped = bad;
   // Units before each sequence, by every CTA for itself (a launch of its own
   // would cost more than these few loads).
-  int64_t carry = 0;
-  for (int base = 0; base < p.B; base += kThreads) {
-    const int b = base + threadIdx.x;
-    int64_t units = 0;
-    if (b < p.B) {
-      const int s = p.slots[b];
-      const int64_t lo = load_offset(p.offs, p.is64, b), hi = load_offset(p.offs, p.is64, b + 1);
-      const int64_t n = hi - lo;
-      if ((unsigned)s >= (unsigned)p.S || lo < 0 || n < 0 || hi > p.T || (b == 0 && lo != 0) ||
-          (b == p.B - 1 && hi != p.T)) {
-        bad = true;
-      } else {
-        const int64_t len = p.lengths[s];
-        if (len < n || len > (int64_t)p.M * p.page || (p.mask != nullptr && n > (int64_t)p.words * 64)) bad = true;
-        else units = (n * p.G + R - 1) / R * ((len + kKeys - 1) / kKeys) * p.Hkv;
-      }
-    }
-    int64_t x = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) warp_sum[warp] = x;
-    __syncthreads();
-    int64_t before = carry, all = carry;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += warp_sum[w];
-      all += warp_sum[w];
-    }
-    if (b < p.B) pre[b + 1] = before + x;
-    carry = all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) pre[0] = 0;
-  if (__syncthreads_or(bad)) {
-    if (bad && !stopped) record_device_error(p.status, SCREE_DEVERR_BAD_INPUT, kSitePagedAttn);
+  if (!paged_prefix<kWarps>(p, pre, [&](int64_t n, int64_t len) {
+        return (n * p.G + R - 1) / R * ((len + kKeys - 1) / kKeys) * p.Hkv;
+      }))
     return;
-  }
-  const int64_t U = carry;
-  if (U == 0) return;  // (T = 0 does not launch; every row has a key: its own)
+  const int64_t U = pre[p.B];  // > 0: T = 0 does not launch, and a new token is a key
   const int64_t N = min((int64_t)gridDim.x * kWarps, U);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.head = Head{U, N};
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.head = PagedHead{U, N};
   // Neighbouring runs go to different SMs, so few workers are spread out too.
   const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
   if (w >= N) return;
@@ -212,12 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t s0, s1;
   };
   auto find = [&](int64_t u) {
-    int lo = 0, hi = p.B - 1;  // last b with pre[b] <= u (empty ones have no units)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= u) lo = mid;
-      else hi = mid - 1;
-    }
+    const int lo = paged_find(pre, p.B, u);
     Seg g;
     g.b = lo;
     g.slot = p.slots[lo];
@@ -253,13 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       win = ui;
       const int64_t g = ui - gi.s0 + lane;
       my_page = 0;
-      if (g < gi.s1 - gi.s0) {
-        my_page = p.table[(int64_t)gi.slot * p.M + g * kKeys / p.page];
-        if ((unsigned)my_page >= (unsigned)p.P) {
-          record_device_error(p.status, SCREE_DEVERR_BAD_INPUT, kSitePagedAttnPage);
-          my_page = 0;
-        }
-      }
+      if (g < gi.s1 - gi.s0) my_page = paged_page(p, gi.slot, g);
     }
     const int page = __shfl_sync(0xffffffffu, my_page, (int)(ui - win));
     if (lane == 0) {
@@ -330,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 #pragma unroll 1
     for (; u < end; ++u) {
-      ok = mbar_wait(&full[cst], phase, abort_flag, p.status, kSitePagedAttnWait);
+      ok = paged_wait(p, &full[cst], phase, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -362,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int row = row_of(mt, r), i = row < rows ? (g.rt * R + row) / p.G : 0;
-            vis[mt][r] = visible16(p, q0 + i, i, k0, c0, g.len);
+            vis[mt][r] = (uint32_t)paged_visible<16>(p, q0 + i, i, k0, c0, g.len);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -453,17 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, special)) {
 #pragma unroll 1
           for (int k = 0; k < min(left, kKeys); ++k) {
-            float pk[MT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                // P of key k: lane (k % 8) / 2 of the quad, word t = k / 8, half k % 2.
-                const uint32_t w0 = __shfl_sync(0xffffffffu, pf[mt][r], (lane & ~3) | ((k & 7) >> 1));
-                const uint32_t w1 = __shfl_sync(0xffffffffu, pf[mt][2 + r], (lane & ~3) | ((k & 7) >> 1));
-                const uint16_t h = (uint16_t)((k < 8 ? w0 : w1) >> (k & 1 ? 16 : 0));
-                pk[mt][r] = Cvt<T>::to_f(*reinterpret_cast<const T*>(&h));
-              }
 #pragma unroll
             for (int j = 0; j < 2 * KK; ++j)
 #pragma unroll
@@ -476,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                      if (vis[mt][r] >> k & 1) o[mt][j][r * 2 + e] += pk[mt][r] * x;
+                      if (vis[mt][r] >> k & 1) o[mt][j][r * 2 + e] += x;  // P > 0
                 }
               }
           }
@@ -519,60 +388,80 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((lane & 3) == 0) p.part_ml[slot * R + row] = make_float2(m[mt][r], sum);
         }
       }
-    if (begin == u0 && lane == 0) p.desc[w] = Desc{g.s0, g.s1, g.b, g.h, g.rt, begin > g.s0 ? 1 : 0};
+    if (begin == u0 && lane == 0) p.desc[w] = PagedDesc{g.s0, g.s1, g.b, g.h, g.rt, begin > g.s0 ? 1 : 0};
   }
 }
 
-// Joins the pieces of a split segment: the block of the first worker that
-// continues it does so.  O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+// Joins the pieces of a split segment: O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+// The workers that continue a segment (all of its pieces but the first) lend a
+// block each; they deal its rows among them.  Where a segment has many pieces
+// (one long sequence over the whole GPU) the warps of a block share a row's
+// pieces, else each warp takes rows of its own.
+constexpr int kJoinWarps = 8;
+constexpr int64_t kManyPieces = 16;
 template <int D, typename T>
-__global__ void __launch_bounds__(128) attn_paged_join_kernel(const Params p, int R) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedParams p, int R) {
+  constexpr int E = D / 32;  // columns of a lane
+  __shared__ float sm_o[kJoinWarps][D];
+  __shared__ float sm_l[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const int64_t U = p.head->U, N = p.head->N;
   const int64_t c = (int64_t)blockIdx.x + 1;
-  if (c >= N) return;
-  const Desc d = p.desc[c];
-  if (!d.on) return;
-  const int64_t w0 = worker_of(d.s0, U, N), w1 = worker_of(d.s1 - 1, U, N);
-  if (w0 != c - 1) return;
-  const int lane = threadIdx.x & 31;
+  const PagedHead hd = *p.head;
+  const PagedDesc d = p.desc[c];  // garbage past the last worker, not used then
+  const int64_t U = hd.U, N = hd.N;
+  if (c >= N || !d.on) return;
+  const int64_t w0 = worker_of(d.s0, U, N);
+  const int np = (int)(worker_of(d.s1 - 1, U, N) - w0) + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t q0 = load_offset(p.offs, p.is64, d.b);
   const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
   const int rows = min(R, n * p.G - d.rt * R);
   const int64_t first = 2 * w0 + (worker_start(w0, U, N) == d.s0 ? 0 : 1);
-  auto slot_of = [&](int64_t i) { return i == 0 ? first : 2 * (w0 + i); };
-  const int64_t pieces = w1 - w0 + 1;
-  constexpr int E = D / 32;  // columns of a lane
-  for (int row = threadIdx.x >> 5; row < rows; row += 4) {
+  auto slot_of = [&](int i) { return i == 0 ? first : 2 * (w0 + i); };
+  const int share = np >= kManyPieces ? kJoinWarps : 1;  // warps of one row
+  const int sub = warp % share;
+  const int step = (np - 1) * (kJoinWarps / share);
+  for (int row = (int)(c - w0 - 1) * (kJoinWarps / share) + warp / share; row < rows; row += step) {
     float mx = -INFINITY;
-    for (int64_t i = lane; i < pieces; i += 32) mx = fmaxf(mx, p.part_ml[slot_of(i) * R + row].x);
+    for (int i = lane; i < np; i += 32) mx = fmaxf(mx, p.part_ml[slot_of(i) * R + row].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float ref = mx == -INFINITY ? 0.f : mx;
     float acc[E], sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int64_t i0 = 0; i0 < pieces; i0 += 32) {
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (i0 + lane < pieces) ml = p.part_ml[slot_of(i0 + lane) * R + row];
-      const float wt = ex2_approx(ml.x - ref);
-      sum += wt * ml.y;
-      const int here = (int)min((int64_t)32, pieces - i0);
-#pragma unroll 4
-      for (int i = 0; i < here; ++i) {
-        const float f = __shfl_sync(0xffffffffu, wt, i);
-        const float* src = p.part_o + (slot_of(i0 + i) * R + row) * D + lane * E;
-        float x[E];
-        if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-        else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
-        else x[0] = *src;
+#pragma unroll 8
+    for (int i = sub; i < np; i += share) {
+      const int64_t at = slot_of(i) * R + row;
+      const float2 ml = p.part_ml[at];
+      const float* src = p.part_o + at * D + lane * E;
+      float x[E];
+      if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+      else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+      else x[0] = *src;
+      const float f = ex2_approx(ml.x - ref);
+      sum = fmaf(f, ml.y, sum);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+    }
+    if (share > 1) {
+      __syncthreads();  // the row before has been read
+#pragma unroll
+      for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = acc[e];
+      if (lane == 0) sm_l[warp] = sum;
+      __syncthreads();
+      if (warp > 0) continue;
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        sum += sm_l[w];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += sm_o[w][lane * E + e];
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int a = d.rt * R + row, hq = d.h * p.G + a % p.G;
     const int64_t tok = q0 + a / p.G;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -588,16 +477,41 @@ __global__ void __launch_bounds__(128) attn_paged_join_kernel(const Params p, in
   }
 }
 
+// Rows of a tile; 0: the tensor-core kernel's 2 x 128.  See scree_attn_fwd_paged.
 int tile_rows(int64_t B, int64_t T, int64_t H, int64_t H_kv) {
-  return T * (H / H_kv) <= 16 * B ? 16 : 32;
+  const int64_t rows = T * (H / H_kv);
+  return rows <= 16 * B ? 16 : rows <= 32 * B || H / H_kv > 128 ? 32 : 0;
 }
 int64_t max_workers() { return (int64_t)num_sms() * kWarps; }
 size_t ws_bytes(int R, int D) {
+  if (R == 0) return attn_paged_tc_workspace(D);
   const int64_t N = max_workers();
-  return 64 + (size_t)N * sizeof(Desc) + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
+  return 64 + (size_t)N * sizeof(PagedDesc) + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
 }
 
-int make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, bool bf16) {
+template <int D, typename T, int MT>
+int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, cudaStream_t s) {
+  auto kern = attn_paged_kernel<D, T, MT>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    SCREE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem(kPagedMaxSeqs)));
+    attr_set[dev & 63] = true;
+  }
+  ProfScope prof(PROF_ATTN_FWD, s);
+  SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), Cfg<D>::smem(p.B), s, tk, tv, p));
+  count_launch();
+  SCREE_CUDA_TRY(launch_dependent(attn_paged_join_kernel<D, T>, dim3((unsigned)max_workers() - 1),
+                                  dim3(kJoinWarps * 32), 0, s,
+                                  p, 16 * MT));
+  count_launch();
+  return SCREE_OK;
+}
+
+}  // namespace
+
+int make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, int box_rows, bool bf16) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) {
     set_last_error("cuTensorMapEncodeTiled is unavailable from the driver");
@@ -605,7 +519,7 @@ int make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, bool 
   }
   cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-  cuuint32_t box[2] = {(cuuint32_t)std::min(D, 64), (cuuint32_t)kKeys};
+  cuuint32_t box[2] = {(cuuint32_t)std::min(D, 64), (cuuint32_t)box_rows};
   cuuint32_t es[2] = {1u, 1u};
   CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                    const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -619,26 +533,6 @@ int make_pool_map(CUtensorMap* map, const void* base, int64_t rows, int D, bool 
   return SCREE_OK;
 }
 
-template <int D, typename T, int MT>
-int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t s) {
-  auto kern = attn_paged_kernel<D, T, MT>;
-  static bool attr_set[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!attr_set[dev & 63]) {
-    SCREE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem(kMaxSeqs)));
-    attr_set[dev & 63] = true;
-  }
-  ProfScope prof(PROF_ATTN_FWD, s);
-  kern<<<(unsigned)num_sms(), kThreads, Cfg<D>::smem(p.B), s>>>(tk, tv, p);
-  SCREE_LAUNCH_CHECK();
-  SCREE_CUDA_TRY(launch_dependent(attn_paged_join_kernel<D, T>, dim3((unsigned)max_workers() - 1), dim3(128), 0, s,
-                                  p, 16 * MT));
-  count_launch();
-  return SCREE_OK;
-}
-
-}  // namespace
 }  // namespace scree
 
 using namespace scree;
@@ -660,8 +554,8 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   SCREE_CHECK_ARG(H_kv >= 1 && H >= 1 && H % H_kv == 0 && H < 65536,
                   "attn_fwd_paged: query heads (%lld) must be a multiple of K/V heads (%lld)", (long long)H,
                   (long long)H_kv);
-  SCREE_CHECK_ARG(B >= 1 && B <= kMaxSeqs && T >= 0 && T < (1ll << 31) && T * (H / H_kv) < (1ll << 31),
-                  "attn_fwd_paged: bad sizes B=%lld (at most %d) T=%lld", (long long)B, kMaxSeqs, (long long)T);
+  SCREE_CHECK_ARG(B >= 1 && B <= kPagedMaxSeqs && T >= 0 && T < (1ll << 31) && T * (H / H_kv) < (1ll << 31),
+                  "attn_fwd_paged: bad sizes B=%lld (at most %d) T=%lld", (long long)B, kPagedMaxSeqs, (long long)T);
   if (D != 32 && D != 64 && D != 128) {
     set_last_error("attn_fwd_paged: head_dim %d unsupported (32, 64, 128)", D);
     return SCREE_ERR_UNSUPPORTED;
@@ -685,20 +579,16 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   SCREE_CHECK_ARG(q && pools->k && pools->v && table && lengths && slots && offsets && o, "attn_fwd_paged: null pointer");
   SCREE_CHECK_ARG((uintptr_t)pools->k % 16 == 0 && (uintptr_t)pools->v % 16 == 0,
                   "attn_fwd_paged: pools must be 16-byte aligned");
-  SCREE_CHECK_ARG((uintptr_t)q % 4 == 0 && q_rs % 2 == 0 && q_hs % 2 == 0,
-                  "attn_fwd_paged: q must be 4-byte aligned with even strides");
-  SCREE_CHECK_ARG((uintptr_t)o % 8 == 0 && o_rs % 4 == 0 && o_hs % 4 == 0,
-                  "attn_fwd_paged: output must be 8-byte aligned with strides multiple of 4");
+  SCREE_CHECK_ARG((uintptr_t)q % 16 == 0 && q_rs % 8 == 0 && q_hs % 8 == 0,
+                  "attn_fwd_paged: q must be 16-byte aligned with strides multiple of 8");
+  SCREE_CHECK_ARG((uintptr_t)o % 16 == 0 && o_rs % 8 == 0 && o_hs % 8 == 0,
+                  "attn_fwd_paged: output must be 16-byte aligned with strides multiple of 8");
   SCREE_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "attn_fwd_paged: workspace must be 16-byte aligned");
   SCREE_BIND_DEVICE(stream, q);
   const int R = tile_rows(B, T, H, H_kv);
   SCREE_CHECK_ARG(workspace_bytes >= ws_bytes(R, D), "attn_fwd_paged: workspace too small");
   const bool bf16 = dtype == SCREE_BF16;
-  CUtensorMap tk, tv;
-  int rc;
-  if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, bf16))) return rc;
-  if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, bf16))) return rc;
-  Params p;
+  PagedParams p;
   p.q = (const char*)q;
   p.q_rs = q_rs * 2;
   p.q_hs = q_hs * 2;
@@ -719,19 +609,25 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   p.G = (int)(H / H_kv);
   p.T = T;
   p.layer_row = layer * P * H_kv * page;
+  p.v = pools->v;
   p.sl2 = scale * 1.4426950408889634f;
   p.o = (char*)o;
   p.o_rs = o_rs * 2;
   p.o_hs = o_hs * 2;
   p.lse = lse;
   p.status = device_status_ptr();
+  cudaStream_t s = (cudaStream_t)stream;
+  if (R == 0) return attn_paged_tc(p, pools->k, pools->v, pool_rows, D, bf16, workspace, s);
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, kKeys, bf16))) return rc;
+  if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, kKeys, bf16))) return rc;
   char* w = (char*)workspace;
   const int64_t N = max_workers();
-  p.head = (Head*)w;
-  p.desc = (Desc*)(w + 64);
-  p.part_ml = (float2*)(w + 64 + N * sizeof(Desc));
-  p.part_o = (float*)(w + 64 + N * sizeof(Desc) + 2 * N * R * 8);
-  cudaStream_t s = (cudaStream_t)stream;
+  p.head = (PagedHead*)w;
+  p.desc = (PagedDesc*)(w + 64);
+  p.part_ml = (float2*)(w + 64 + N * sizeof(PagedDesc));
+  p.part_o = (float*)(w + 64 + N * sizeof(PagedDesc) + 2 * N * R * 8);
 #define SCREE_PAGED_CASE(DD)                                                                       \
   if (D == DD) {                                                                                   \
     if (bf16)                                                                                      \

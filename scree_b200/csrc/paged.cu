@@ -68,6 +68,13 @@ template <> struct Vec<1> { using T = uint8_t; };
 
 // ------------------------------------------------------------------ plan pieces
 
+// A plan waits for what came before it on the stream (it may be the apply of an
+// earlier call on the same cache) and lets its own apply be launched meanwhile.
+__device__ __forceinline__ void begin_plan() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+
 // Exclusive sum over the block (1024 threads) and its total.
 __device__ int block_scan(int v, int* total) {
   __shared__ int warp_sum[32];
@@ -198,7 +205,7 @@ __device__ bool plan_stopped(const Book& b) {
 __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(const Book b, const int32_t* slots,
                                                                     const int32_t* counts, int n) {
   __shared__ SlotSet set;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_plan();
   if (plan_stopped(b)) return;
   int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
   int64_t want = 0;
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(const Book b
 __global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(const Book b, const int32_t* parents,
                                                                  const int32_t* children, int n) {
   __shared__ SlotSet set;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_plan();
   if (plan_stopped(b)) return;
   int bad = mark_slots(b, children, n, &set) ? 0 : kSitePagedArgs;
   __syncthreads();
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(const Book b, c
 
 __global__ void __launch_bounds__(kPlanThreads) plan_free_kernel(const Book b, const int32_t* slots, int n) {
   __shared__ SlotSet set;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_plan();
   if (plan_stopped(b)) return;
   int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b,
                                                                    const int32_t* drafted,
                                                                    const int32_t* path, int depth, int n) {
   __shared__ SlotSet set;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_plan();
   if (plan_stopped(b)) return;
   int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
   // One warp per entry: lanes read the path and the draft's pages side by side.
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b,
 
 // list = new id of each page, then the holes and the pages that fill them.
 __global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(const Book b) {
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_plan();
   if (plan_stopped(b)) return;
   int32_t *to = b.list(0), *hole = to + b.P, *mover = hole + b.P;
   const int lane = threadIdx.x & 31;
@@ -450,6 +457,7 @@ __global__ void __launch_bounds__(kThreads)
     apply_kernel(const Book b, const Pools pl, const int32_t* slots, const int32_t* aux,
                  const int32_t* path, int depth, int n, int table_blocks) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   const bool ok = b.plan()->ok != 0;
   if ((int)blockIdx.x < table_blocks) {
     const int64_t all = (int64_t)b.S * b.M;
@@ -741,8 +749,8 @@ extern "C" int scree_paged_reserve(const scree_paged_book* book, const int32_t* 
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  plan_reserve_kernel<<<1, kPlanThreads, 0, s>>>(b, slots, counts, (int)n);
-  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(plan_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, counts, (int)n));
+  count_launch();
   return launch_apply<kReserve>(b, Pools{}, slots, counts, nullptr, 0, (int)n, 0, s);
 }
 
@@ -759,8 +767,8 @@ extern "C" int scree_paged_accept(const scree_paged_book* book, const scree_page
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  plan_accept_kernel<<<1, kPlanThreads, 0, s>>>(b, slots, drafted, path, (int)depth, (int)n);
-  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(plan_accept_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, drafted, path, (int)depth, (int)n));
+  count_launch();
   const int w = pick_width(pl.row_bytes, {(uintptr_t)pl.k, (uintptr_t)pl.v});
   const int64_t threads = n * pl.L * 2 * pl.H * (pl.row_bytes / w);
   return launch_apply<kAccept>(b, pl, slots, drafted, path, (int)depth, (int)n,
@@ -778,8 +786,8 @@ extern "C" int scree_paged_fork(const scree_paged_book* book, const scree_paged_
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  plan_fork_kernel<<<1, kPlanThreads, 0, s>>>(b, parents, children, (int)n);
-  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(plan_fork_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, parents, children, (int)n));
+  count_launch();
   return launch_apply<kFork>(b, pl, parents, parents, nullptr, 0, (int)n, n * pl.L * 2 * pl.H, s);
 }
 
@@ -791,8 +799,8 @@ extern "C" int scree_paged_free(const scree_paged_book* book, const int32_t* slo
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  plan_free_kernel<<<1, kPlanThreads, 0, s>>>(b, slots, (int)n);
-  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(plan_free_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, (int)n));
+  count_launch();
   return launch_apply<kFree>(b, Pools{}, slots, nullptr, nullptr, 0, (int)n, 0, s);
 }
 
@@ -805,8 +813,8 @@ extern "C" int scree_paged_compact(const scree_paged_book* book, const scree_pag
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  plan_compact_kernel<<<1, kPlanThreads, 0, s>>>(b);
-  SCREE_LAUNCH_CHECK();
+  SCREE_CUDA_TRY(launch_dependent(plan_compact_kernel, dim3(1), dim3(kPlanThreads), 0, s, b));
+  count_launch();
   // At most half of the pages can move.
   return launch_apply<kCompact>(b, pl, nullptr, nullptr, nullptr, 0, 0, (book->P / 2 + 1) * pl.L * 2 * 8, s);
 }
