@@ -392,18 +392,16 @@ int scree_attn_fwd_paged(const void* q, int64_t q_row_stride, int64_t q_head_str
 /* ------------------------------------------------------------------ token log probabilities
  * logits (N, V) in dtype with row stride row_stride (elements); targets (N,)
  * int32 / int64.  Per row (fp32): norm (N, 2) = the maximum m and
- * log sum e^(logits - m) (8-byte aligned; for the gradient); logp = log
+ * log sum e^(logits - m) (8-byte aligned; for the gradient, or NULL); logp = log
  * softmax(logits)[target], 0 for a negative target (no token given), a target >= V sets the status word
  * (SCREE_DEVERR_BAD_INPUT, site 50); entropy in nats; the `top` (0..32) most
  * likely tokens' log probabilities and indices, equal values by lower index,
  * NaN above all.  A row of -inf alone has logp -inf and entropy 0.  V < 2^30.
  * No reference counterpart. */
-size_t scree_token_logprobs_workspace_size(int64_t N, int64_t V, int top, int dtype);
 int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, const void* targets,
                              int targets_is_i64, int64_t N, int64_t V, int top, int dtype,
                              float* logp, float* entropy, float* norm, float* top_logp,
-                             int64_t* top_ids, void* workspace, size_t workspace_bytes,
-                             void* stream);
+                             int64_t* top_ids, void* stream);
 /* d_logits (N, V) contiguous from the gradients of logp, entropy (N,) and
  * top_logp (N, top), each fp32 contiguous or NULL. */
 int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, const void* targets,

@@ -89,9 +89,7 @@ class Array:
         the ragged size when this Array was made, so nothing is read from the device."""
         assert values.shape[self.ragged_dim] == self.values.shape[self.ragged_dim]
         out = object.__new__(Array)
-        for name, value in (("values", values), ("offsets", self.offsets), ("ragged_dim", self.ragged_dim),
-                            ("_host", self._host)):
-            object.__setattr__(out, name, value)
+        out.__dict__.update(self.__dict__, values=values)
         return out
 
     @property

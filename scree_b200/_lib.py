@@ -111,8 +111,7 @@ _SIGNATURES = {
         _I,
         [_P, _L, _L, _P, _L, _P, _P, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _I, _I, _F, _P, _L, _P, _L, _L, _P, _P, _S, _P],
     ),
-    "scree_token_logprobs_workspace_size": (_S, [_L, _L, _I, _I]),
-    "scree_token_logprobs_fwd": (_I, [_P, _L, _P, _I, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "scree_token_logprobs_fwd": (_I, [_P, _L, _P, _I, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P]),
     "scree_token_logprobs_bwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P, _P]),
 }
 

@@ -500,10 +500,10 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams
     attr_set[dev & 63] = true;
   }
   ProfScope prof(PROF_ATTN_FWD, s);
-  SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), Cfg<D>::smem(p.B), s, tk, tv, p));
+  SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), Cfg<D>::smem(p.B), s, 1, tk, tv, p));
   count_launch();
   SCREE_CUDA_TRY(launch_dependent(attn_paged_join_kernel<D, T>, dim3((unsigned)max_workers() - 1),
-                                  dim3(kJoinWarps * 32), 0, s,
+                                  dim3(kJoinWarps * 32), 0, s, 1,
                                   p, 16 * MT));
   count_launch();
   return SCREE_OK;

@@ -691,10 +691,10 @@ int launch_tc(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& t
     attr_set[dev & 63] = true;
   }
   ProfScope prof(PROF_ATTN_FWD, s);
-  SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), smem, s, tq, tk, tv, p, box));
+  SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), smem, s, 1, tq, tk, tv, p, box));
   count_launch();
   SCREE_CUDA_TRY(launch_dependent(attn_paged_tc_join_kernel<D, T>, dim3((unsigned)std::max(1, num_sms() - 1), 8),
-                                  dim3(kJoinWarps * 32), 0, s, p));
+                                  dim3(kJoinWarps * 32), 0, s, 1, p));
   count_launch();
   return SCREE_OK;
 }

@@ -58,19 +58,23 @@ void count_launch();
 // Launch of a kernel that reads what the launch before it on the stream wrote,
 // started while that one drains: the kernel executes griddepcontrol.wait before
 // its first such read, and the one before it griddepcontrol.launch_dependents.
+// `cluster` CTAs form a cluster.
 template <typename... P, typename... A>
 inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
-                                    cudaStream_t s, A... args) {
+                                    cudaStream_t s, int cluster, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 

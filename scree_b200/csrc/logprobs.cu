@@ -6,12 +6,12 @@
 //   dx_v = g_logp [v = target] + sum_j g_top_j [v = id_j]
 //          - p_v (g_logp + sum_j g_top_j) - g_H p_v (log p_v + H)
 //
-// Forward: each logit is read from HBM once.  Persistent CTAs stream rows
-// (segments of rows when there are few) in chunks of 16 KB: one warp copies them
+// Forward: each logit is read from HBM once.  Persistent CTAs stream rows in chunks of 16 KB: one warp copies them
 // into a ring with bulk copies, running on into the CTA's next row while the
 // other eight finish one, so 3 CTAs keep up to 192 KB per SM in flight.  Each
 // thread keeps its own maximum, s1 and s2; they are rescaled only when a chunk
-// raises the maximum.
+// raises the maximum.  Of few rows each is cut into segments for the CTAs of a
+// cluster, which hand their results to its first CTA through shared memory.
 //
 // Alternatives: a thread notes the maximum of its elements of each chunk (a pair:
 // thread, chunk).  After kWin chunks or at the row's end the k-th largest pair
@@ -43,6 +43,7 @@ constexpr int kStages = 3;      // ring of chunks
 constexpr int kChunkBytes = kThreads * kU * 16;
 constexpr int kWinBytes = 32 * kThreads;
 constexpr int kRingSmem = kStages * kChunkBytes + kWinBytes + 128;
+constexpr int kMaxSegs = 8;     // a portable cluster
 constexpr int kSiteRing = 51;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kSiteTarget = 50;
@@ -187,7 +188,7 @@ struct FwdArgs {
   const void* x;
   int64_t row_stride, N;
   int V;
-  int chunks, segs;  // chunks of a row, segments that they are dealt to
+  int chunks, segs;  // chunks of a row, segments that they are dealt to (= CTAs of a cluster)
   const void* targets;
   int t64;
   int top;
@@ -195,8 +196,6 @@ struct FwdArgs {
   float2* norm;  // maximum and log of the sum: log p = (x - norm.x) - norm.y
   float* top_logp;
   int64_t* top_ids;
-  Stat* part;                     // (N, segs)
-  unsigned long long* part_keys;  // (N, segs, top)
   int* status;
 };
 
@@ -208,7 +207,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const St
   const bool empty = s.m == -INFINITY;
   const float ls = log2f(s.s1) * kLn2;
   if (lane == 0) {
-    a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
+    if (a.norm != nullptr) a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
     a.entropy[n] = empty ? 0.f : (log2f(s.s1) - s.s2 / s.s1) * kLn2;
     const int64_t t = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[n]
                             : (int64_t)reinterpret_cast<const int32_t*>(a.targets)[n];
@@ -453,6 +452,18 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
   work_sync();
 }
 
+// What a row's other segments hand to its first CTA.
+struct SegOut {
+  Stat stat[kMaxSegs];
+  unsigned long long keys[kMaxSegs][kMaxTop];
+};
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(const FwdArgs a) {
   constexpr int VE = Lv<T>::N, CV = kThreads * kU;  // elements of a vector, vectors of a chunk
@@ -463,6 +474,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
   __shared__ Stat sm_stat[2][kThreads / 32];
   __shared__ TopList tl;
+  __shared__ SegOut so;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -473,8 +485,11 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
     fence_mbar_init();
   }
   __syncthreads();
+  if (a.segs > 1) cluster_sync();  // the first CTA is there to be written to
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
+  // Item = segment of a row; with several segments a CTA has one item, and the
+  // segment is its rank in the cluster.
   const int64_t items = a.N * a.segs;
   // Vectors start at 16-byte boundaries: a row begins `mis` elements into its
   // first vector; vectors [1 if mis, (V + mis) / VE) lie inside the row and go
@@ -485,10 +500,9 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
 
   if (warp == kThreads / 32) {
     // ---------------------------------------------------------------- copies
-    if (lane != 0) return;
     int k = 0;  // chunks issued
     bool ok = true;
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+    for (int64_t item = blockIdx.x; lane == 0 && ok && item < items; item += gridDim.x) {
       const T* row = row_of(item / a.segs);
       const int seg = (int)(item % a.segs), mis = mis_of(row);
       const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
@@ -507,11 +521,13 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
         }
       }
     }
-    if (!ok) {  // give copies in flight time to land before the CTA ends
+    if (lane == 0 && !ok) {  // give copies in flight time to land before the CTA ends
       volatile int quiet = 0;
       for (int i = max(0, k - kStages); i < k; ++i)
         mbar_wait_impl(&full[i % kStages], (i / kStages) & 1, &quiet, nullptr, kSiteRing);
     }
+    __syncwarp();
+    if (a.segs > 1) cluster_sync();
     return;
   }
 
@@ -616,41 +632,31 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
       if (a.segs == 1) {
         finish_row<T>(a, n, s, key, lane);
       } else {
-        if (lane == 0) a.part[n * a.segs + seg] = s;
-        if (lane < a.top) a.part_keys[(n * a.segs + seg) * a.top + lane] = key;
+        if (seg > 0) {
+          const uint32_t at = smem_peer(smem_u32(&so.stat[seg]), 0);
+          if (lane == 0) {
+            st_cluster(at, s.m);
+            st_cluster(at + 4, s.s1);
+            st_cluster(at + 8, s.s2);
+          }
+          if (a.top > 0) st_cluster(smem_peer(smem_u32(&so.keys[seg][lane]), 0), key);
+        }
+        cluster_sync();
+        if (seg == 0) {
+          const Stat o = lane > 0 && lane < a.segs ? so.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+          s = stat_warp(lane == 0 ? s : o);
+          unsigned long long best = key;
+          if (a.top > 0)
+            for (int j = 1; j < a.segs; ++j) best = lane_join(best, so.keys[j][lane], lane);
+          finish_row<T>(a, n, s, best, lane);
+        }
       }
       __syncwarp();
+    } else if (a.segs > 1) {
+      cluster_sync();
     }
     parity ^= 1;
   }
-}
-
-// Joins a row's segments, the lists dealt to four warps.
-constexpr int kJoinWarps = 4;
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) logprobs_join_kernel(const FwdArgs a) {
-  __shared__ unsigned long long lists[kJoinWarps][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n = blockIdx.x;
-  Stat s{-INFINITY, 0.f, 0.f};
-  if (warp == 0) {
-    for (int j = lane; j < a.segs; j += 32) s = stat_join(s, a.part[n * a.segs + j]);
-    s = stat_warp(s);
-  }
-  unsigned long long best = 0;
-  if (a.top > 0) {
-    const unsigned long long* keys = a.part_keys + n * a.segs * a.top;
-    for (int j = warp; j < a.segs; j += kJoinWarps) {
-      const unsigned long long k = lane < a.top ? keys[(int64_t)j * a.top + lane] : 0;
-      best = j == warp ? k : lane_join(best, k, lane);
-    }
-    lists[warp][lane] = best;
-    __syncthreads();
-    if (warp == 0)
-      for (int w = 1; w < kJoinWarps; ++w) best = lane_join(best, lists[w][lane], lane);
-  }
-  if (warp == 0) finish_row<T>(a, n, s, best, lane);
 }
 
 struct BwdArgs {
@@ -761,10 +767,12 @@ int64_t row_vecs(int64_t V, int dtype) {
 }
 int64_t row_chunks(int64_t V, int dtype) { return (row_vecs(V, dtype) + kThreads * kU - 1) / (kThreads * kU); }
 // A CTA per row once there are four rounds of them; fewer rows are cut so that
-// there are as many segments (or chunks of one).
-int64_t row_segs(int64_t N, int64_t V, int dtype) {
+// there are about as many segments.
+int row_segs(int64_t N, int64_t V, int dtype) {
   const int64_t want = 4 * kCtasPerSm * (int64_t)num_sms();
-  return std::max<int64_t>(1, std::min(row_chunks(V, dtype), (want + N - 1) / std::max<int64_t>(N, 1)));
+  int segs = 1;
+  while (segs < kMaxSegs && N * segs < want && 2 * segs <= row_chunks(V, dtype)) segs *= 2;
+  return segs;
 }
 constexpr int kNV = 8;  // vectors of a thread, backward
 int64_t bwd_slices(int64_t V, int dtype) { return (row_vecs(V, dtype) + kThreads * kNV - 1) / (kThreads * kNV); }
@@ -791,13 +799,9 @@ template <typename T> int launch_fwd(const FwdArgs& a, cudaStream_t s) {
     SCREE_CUDA_TRY(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
     attr_set[dev & 63] = true;
   }
-  const unsigned grid = (unsigned)std::min<int64_t>(a.N * a.segs, (int64_t)kCtasPerSm * num_sms());
-  SCREE_CUDA_TRY(launch_dependent(logprobs_kernel<T>, dim3(grid), dim3(kThreads + 32), kRingSmem, s, a));
+  const int64_t grid = a.segs > 1 ? a.N * a.segs : std::min<int64_t>(a.N, (int64_t)kCtasPerSm * num_sms());
+  SCREE_CUDA_TRY(launch_dependent(logprobs_kernel<T>, dim3((unsigned)grid), dim3(kThreads + 32), kRingSmem, s, a.segs, a));
   count_launch();
-  if (a.segs > 1) {
-    SCREE_CUDA_TRY(launch_dependent(logprobs_join_kernel<T>, dim3((unsigned)a.N), dim3(kJoinWarps * 32), 0, s, a));
-    count_launch();
-  }
   return SCREE_OK;
 }
 template <typename T> int launch_bwd(const BwdArgs& a, cudaStream_t s) {
@@ -811,27 +815,17 @@ template <typename T> int launch_bwd(const BwdArgs& a, cudaStream_t s) {
 
 using namespace scree;
 
-extern "C" size_t scree_token_logprobs_workspace_size(int64_t N, int64_t V, int top, int dtype) {
-  if (N <= 0 || V <= 0 || dtype_size(dtype) == 0) return 0;
-  const int64_t segs = row_segs(N, V, dtype);
-  return segs == 1 ? 0 : (size_t)(N * segs) * (16 + 8 * (size_t)(top > 0 ? top : 0));
-}
-
 extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, const void* targets,
                                         int targets_is_i64, int64_t N, int64_t V, int top,
                                         int dtype, float* logp, float* entropy, float* norm,
-                                        float* top_logp, int64_t* top_ids, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
+                                        float* top_logp, int64_t* top_ids, void* stream) {
   int rc = check_sizes("token_logprobs", N, V, row_stride, top, dtype);
   if (rc != SCREE_OK) return rc;
   if (N == 0) return SCREE_OK;
-  SCREE_CHECK_ARG(logits && targets && logp && entropy && norm && (top == 0 || (top_logp && top_ids)),
+  SCREE_CHECK_ARG(logits && targets && logp && entropy && (top == 0 || (top_logp && top_ids)),
                   "token_logprobs: null pointer");
   SCREE_CHECK_ARG((uintptr_t)logits % dtype_size(dtype) == 0 && (uintptr_t)norm % 8 == 0,
                   "token_logprobs: misaligned logits or norm");
-  const size_t need = scree_token_logprobs_workspace_size(N, V, top, dtype);
-  SCREE_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
-                  "token_logprobs: workspace too small");
   SCREE_BIND_DEVICE(stream, logits);
   FwdArgs a;
   a.x = logits;
@@ -839,7 +833,7 @@ extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, 
   a.N = N;
   a.V = (int)V;
   a.chunks = (int)row_chunks(V, dtype);
-  a.segs = (int)row_segs(N, V, dtype);
+  a.segs = row_segs(N, V, dtype);
   a.targets = targets;
   a.t64 = targets_is_i64;
   a.top = top;
@@ -848,8 +842,6 @@ extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, 
   a.norm = (float2*)norm;
   a.top_logp = top_logp;
   a.top_ids = top_ids;
-  a.part_keys = reinterpret_cast<unsigned long long*>(workspace);
-  a.part = reinterpret_cast<Stat*>(reinterpret_cast<char*>(workspace) + 8 * (size_t)(N * a.segs) * top);
   a.status = device_status_ptr();
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == SCREE_F32) return launch_fwd<float>(a, s);

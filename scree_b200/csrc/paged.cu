@@ -8,10 +8,10 @@
 // lowest free pages in the order of the call's entries, so results do not depend
 // on any hidden list.  A part-filled page is never shared.
 //
-// Every operation is two launches: a plan of one CTA (checks everything, scans
-// refs, and leaves its decisions in the workspace) and an apply over all SMs
-// that writes the new table and lengths and moves rows.  If the plan rejects the
-// call, it sets the status word and the apply copies the bookkeeping through.
+// Every operation is a plan of one CTA (checks everything, scans refs, and leaves
+// its decisions in the workspace) and an apply that writes the new table and
+// lengths and moves rows: over all SMs in a second launch, or, for small calls, by
+// the plan's own CTA.  If the plan rejects the call, it sets the status word and the apply copies the bookkeeping through.
 //
 // Bound: the moves are HBM copies; the plan is latency (a few dependent loads and
 // block scans), which is why it is one CTA and the apply starts while it drains.
@@ -24,6 +24,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kThreads = 256;
 constexpr int kMaxSlots = 65536;
+constexpr int kHereEntries = 8192, kHereWarps = 128;  // see apply_by_plan
 constexpr int kSitePagedArgs = 60;    // a slot, count, length or path out of range
 constexpr int kSitePagedFull = 61;    // not enough free pages
 constexpr int kSitePagedShared = 62;  // a draft on pages that other slots hold
@@ -200,184 +201,6 @@ __device__ bool plan_stopped(const Book& b) {
   return true;
 }
 
-// ------------------------------------------------------------------ plans
-
-__global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(const Book b, const int32_t* slots,
-                                                                    const int32_t* counts, int n) {
-  __shared__ SlotSet set;
-  begin_plan();
-  if (plan_stopped(b)) return;
-  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
-  int64_t want = 0;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
-    int need = 0, f = 0;
-    if (i < n) {
-      const int s = slots[i];
-      const int64_t cnt = counts[i];
-      if ((unsigned)s < (unsigned)b.S) {
-        const int64_t len = b.lengths[s];
-        if (cnt < 0 || !length_ok(b, len) || !length_ok(b, len + cnt)) {
-          bad = kSitePagedArgs;
-        } else {
-          f = pages_of(len, b.page);
-          need = pages_of(len + cnt, b.page) - f;
-        }
-      }
-    }
-    int total;
-    const int before = block_scan(need, &total);
-    if (i < n) {
-      b.first()[i] = f;
-      b.last(n)[i] = f + need;
-      b.start(n)[i] = (int)min(want + before, (int64_t)b.P);
-    }
-    want += total;
-  }
-  const bool fits = list_free(b, (int)min(want, (int64_t)b.P), b.list(n)) && want <= b.P;
-  if (!fits && bad == 0) bad = kSitePagedFull;
-  end_plan(b, bad, 0);
-}
-
-__global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(const Book b, const int32_t* parents,
-                                                                 const int32_t* children, int n) {
-  __shared__ SlotSet set;
-  begin_plan();
-  if (plan_stopped(b)) return;
-  int bad = mark_slots(b, children, n, &set) ? 0 : kSitePagedArgs;
-  __syncthreads();
-  int64_t want = 0;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
-    int need = 0, full = 0;
-    if (i < n) {
-      const int p = parents[i], c = children[i];
-      if ((unsigned)p >= (unsigned)b.S || (unsigned)c >= (unsigned)b.S || b.lengths[c] != 0 ||
-          (set.bits[p >> 5] >> (p & 31) & 1) || !length_ok(b, b.lengths[p])) {
-        bad = kSitePagedArgs;
-      } else {
-        full = b.lengths[p] / b.page;
-        need = b.lengths[p] % b.page != 0;
-      }
-    }
-    int total;
-    const int before = block_scan(need, &total);
-    if (i < n) {
-      b.first()[i] = full;
-      b.last(n)[i] = full + need;
-      b.start(n)[i] = (int)min(want + before, (int64_t)b.P);
-    }
-    want += total;
-  }
-  const bool fits = list_free(b, (int)min(want, (int64_t)b.P), b.list(n)) && want <= b.P;
-  if (!fits && bad == 0) bad = kSitePagedFull;
-  end_plan(b, bad, 0);
-}
-
-__global__ void __launch_bounds__(kPlanThreads) plan_free_kernel(const Book b, const int32_t* slots, int n) {
-  __shared__ SlotSet set;
-  begin_plan();
-  if (plan_stopped(b)) return;
-  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int s = slots[i];
-    if ((unsigned)s < (unsigned)b.S && !length_ok(b, b.lengths[s])) bad = kSitePagedArgs;
-  }
-  copy_and_count(b, false);
-  end_plan(b, bad, 0);
-}
-
-// last[i] = pages before, first[i] = pages after, start[i] = rows kept of the draft.
-__global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b, const int32_t* slots,
-                                                                   const int32_t* drafted,
-                                                                   const int32_t* path, int depth, int n) {
-  __shared__ SlotSet set;
-  begin_plan();
-  if (plan_stopped(b)) return;
-  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
-  // One warp per entry: lanes read the path and the draft's pages side by side.
-  const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
-    const int s = slots[i];
-    if ((unsigned)s >= (unsigned)b.S) continue;  // reported above
-    const int64_t len = b.lengths[s], m = drafted[i];
-    if (m < 0 || m > len || !length_ok(b, len)) {
-      bad = kSitePagedArgs;
-      continue;
-    }
-    int kept = 0, prev = -1;
-    for (int d0 = 0; d0 < depth; d0 += 32) {
-      const int node = d0 + lane < depth ? path[(int64_t)i * depth + d0 + lane] : -1;
-      const unsigned ends = __ballot_sync(0xffffffffu, node < 0);
-      const int here = ends ? __ffs(ends) - 1 : 32;  // nodes before the first -1
-      int before = __shfl_up_sync(0xffffffffu, node, 1);
-      if (lane == 0) before = prev;
-      if (lane < here && (node <= before || node >= m)) bad = kSitePagedArgs;
-      prev = __shfl_sync(0xffffffffu, node, 31);
-      kept += here;
-      if (here < 32) break;
-    }
-    const int64_t begin = len - m;
-    const int pages = pages_of(len, b.page);
-    for (int c = (int)(begin / b.page) + lane; c < pages; c += 32) {
-      const int p = b.table[(int64_t)s * b.M + c];
-      if ((unsigned)p >= (unsigned)b.P) bad = kSitePagedTable;
-      else if (m > 0 && b.refs[p] != 1) bad = kSitePagedShared;
-    }
-    if (lane == 0) {
-      b.last(n)[i] = pages;
-      b.first()[i] = pages_of(begin + kept, b.page);
-      b.start(n)[i] = kept;
-    }
-  }
-  copy_and_count(b, false);
-  end_plan(b, bad, 0);
-}
-
-// list = new id of each page, then the holes and the pages that fill them.
-__global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(const Book b) {
-  begin_plan();
-  if (plan_stopped(b)) return;
-  int32_t *to = b.list(0), *hole = to + b.P, *mover = hole + b.P;
-  const int lane = threadIdx.x & 31;
-  const int mine = copy_and_count(b, true);
-  int used;
-  block_scan(lane == 0 ? mine : 0, &used);
-  int lo, hi;
-  warp_pages(b.P, lo, hi);
-  int nh = 0, nm = 0;
-  for (int p0 = lo; p0 < hi; p0 += 32) {
-    const int p = p0 + lane, r = p < hi ? b.refs[p] : 0;
-    nh += __popc(__ballot_sync(0xffffffffu, p < hi && r <= 0 && p < used));
-    nm += __popc(__ballot_sync(0xffffffffu, p < hi && r > 0 && p >= used));
-  }
-  int holes, movers;
-  int rh = block_scan(lane == 0 ? nh : 0, &holes);
-  int rm = block_scan(lane == 0 ? nm : 0, &movers);
-  rh = __shfl_sync(0xffffffffu, rh, 0);
-  rm = __shfl_sync(0xffffffffu, rm, 0);
-  for (int p0 = lo; p0 < hi; p0 += 32) {
-    const int p = p0 + lane, r = p < hi ? b.refs[p] : 0;
-    const bool h = p < hi && r <= 0 && p < used, m = p < hi && r > 0 && p >= used;
-    const unsigned bh = __ballot_sync(0xffffffffu, h), bm = __ballot_sync(0xffffffffu, m);
-    const unsigned lt = (1u << lane) - 1;
-    if (p < hi) to[p] = p;
-    if (h) hole[rh + __popc(bh & lt)] = p;
-    if (m) mover[rm + __popc(bm & lt)] = p;
-    rh += __popc(bh);
-    rm += __popc(bm);
-  }
-  __syncthreads();  // also orders the lists for this block's readers
-  // As many used pages stand above `used` as free ones below it.
-  for (int i = threadIdx.x; i < movers; i += blockDim.x) {
-    const int src = mover[i], dst = hole[i];
-    to[src] = dst;
-    b.refs_out[dst] = b.refs[src];
-    b.refs_out[src] = 0;
-  }
-  end_plan(b, 0, movers);
-}
-
 // ------------------------------------------------------------------ apply
 
 // Rows of `bytes` bytes as W-byte vectors by one warp.
@@ -451,25 +274,19 @@ __device__ __forceinline__ void book_entry(const Book& b, bool ok, const int32_t
   if (c == 0) b.lengths_out[s] = len;
 }
 
-// Blocks [0, table_blocks) write the table, the others move rows.
+// The whole new table by threads [thread, ...) of `threads`.
+template <int OP>
+__device__ __forceinline__ void apply_table(const Book& b, bool ok, const int32_t* aux, int n, int64_t thread,
+                                            int64_t threads) {
+  const int64_t all = (int64_t)b.S * b.M;
+  for (int64_t at = thread; at < all; at += threads) book_entry<OP>(b, ok, aux, n, at);
+}
+
+// The rows that an accepted call moves, by warp `warp` of `warps`.
 template <int OP, int W>
-__global__ void __launch_bounds__(kThreads)
-    apply_kernel(const Book b, const Pools pl, const int32_t* slots, const int32_t* aux,
-                 const int32_t* path, int depth, int n, int table_blocks) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;");
-  const bool ok = b.plan()->ok != 0;
-  if ((int)blockIdx.x < table_blocks) {
-    const int64_t all = (int64_t)b.S * b.M;
-    for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < all;
-         at += (int64_t)table_blocks * kThreads)
-      book_entry<OP>(b, ok, aux, n, at);
-    return;
-  }
-  if (!ok) return;
+__device__ __forceinline__ void apply_moves(const Book& b, const Pools& pl, const int32_t* slots, const int32_t* aux,
+                                            const int32_t* path, int depth, int n, int64_t warp, int64_t warps) {
   const int lane = threadIdx.x & 31;
-  const int64_t warps = (int64_t)(gridDim.x - table_blocks) * (kThreads / 32);
-  const int64_t warp = (int64_t)(blockIdx.x - table_blocks) * (kThreads / 32) + (threadIdx.x >> 5);
   if constexpr (OP == kFork) {
     // Filled rows of the parent's last page, one head at a time.
     const int64_t tasks = (int64_t)n * pl.L * 2 * pl.H;
@@ -541,6 +358,231 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   }
+}
+
+// Blocks [0, table_blocks) write the table, the others move rows.
+template <int OP, int W>
+__global__ void __launch_bounds__(kThreads)
+    apply_kernel(const Book b, const Pools pl, const int32_t* slots, const int32_t* aux,
+                 const int32_t* path, int depth, int n, int table_blocks) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const bool ok = b.plan()->ok != 0;
+  if ((int)blockIdx.x < table_blocks) {
+    apply_table<OP>(b, ok, aux, n, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)table_blocks * kThreads);
+  } else if (ok) {
+    apply_moves<OP, W>(b, pl, slots, aux, path, depth, n,
+                       (int64_t)(blockIdx.x - table_blocks) * (kThreads / 32) + (threadIdx.x >> 5),
+                       (int64_t)(gridDim.x - table_blocks) * (kThreads / 32));
+  }
+}
+
+// A small call's apply, by its plan's own CTA (rows in 16-byte vectors).
+template <int OP, bool MOVES>
+__device__ __forceinline__ void apply_here(const Book& b, const Pools& pl, const int32_t* slots, const int32_t* aux,
+                                           const int32_t* path, int depth, int n) {
+  __syncthreads();
+  const bool ok = b.plan()->ok != 0;
+  apply_table<OP>(b, ok, aux, n, threadIdx.x, blockDim.x);
+  if (MOVES && ok) apply_moves<OP, 16>(b, pl, slots, aux, path, depth, n, threadIdx.x >> 5, blockDim.x >> 5);
+}
+
+// ------------------------------------------------------------------ plans
+
+template <bool HERE>
+__global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(const Book b, const int32_t* slots,
+                                                                    const int32_t* counts, int n) {
+  __shared__ SlotSet set;
+  begin_plan();
+  if (plan_stopped(b)) {
+    if (HERE) apply_here<kReserve, false>(b, Pools{}, slots, counts, nullptr, 0, n);
+    return;
+  }
+  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
+  int64_t want = 0;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, f = 0;
+    if (i < n) {
+      const int s = slots[i];
+      const int64_t cnt = counts[i];
+      if ((unsigned)s < (unsigned)b.S) {
+        const int64_t len = b.lengths[s];
+        if (cnt < 0 || !length_ok(b, len) || !length_ok(b, len + cnt)) {
+          bad = kSitePagedArgs;
+        } else {
+          f = pages_of(len, b.page);
+          need = pages_of(len + cnt, b.page) - f;
+        }
+      }
+    }
+    int total;
+    const int before = block_scan(need, &total);
+    if (i < n) {
+      b.first()[i] = f;
+      b.last(n)[i] = f + need;
+      b.start(n)[i] = (int)min(want + before, (int64_t)b.P);
+    }
+    want += total;
+  }
+  const bool fits = list_free(b, (int)min(want, (int64_t)b.P), b.list(n)) && want <= b.P;
+  if (!fits && bad == 0) bad = kSitePagedFull;
+  end_plan(b, bad, 0);
+  if (HERE) apply_here<kReserve, false>(b, Pools{}, slots, counts, nullptr, 0, n);
+}
+
+template <bool HERE>
+__global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(const Book b, const Pools pl, const int32_t* parents,
+                                                                 const int32_t* children, int n) {
+  __shared__ SlotSet set;
+  begin_plan();
+  if (plan_stopped(b)) {
+    if (HERE) apply_here<kFork, true>(b, pl, parents, parents, nullptr, 0, n);
+    return;
+  }
+  int bad = mark_slots(b, children, n, &set) ? 0 : kSitePagedArgs;
+  __syncthreads();
+  int64_t want = 0;
+  for (int base = 0; base < n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, full = 0;
+    if (i < n) {
+      const int p = parents[i], c = children[i];
+      if ((unsigned)p >= (unsigned)b.S || (unsigned)c >= (unsigned)b.S || b.lengths[c] != 0 ||
+          (set.bits[p >> 5] >> (p & 31) & 1) || !length_ok(b, b.lengths[p])) {
+        bad = kSitePagedArgs;
+      } else {
+        full = b.lengths[p] / b.page;
+        need = b.lengths[p] % b.page != 0;
+      }
+    }
+    int total;
+    const int before = block_scan(need, &total);
+    if (i < n) {
+      b.first()[i] = full;
+      b.last(n)[i] = full + need;
+      b.start(n)[i] = (int)min(want + before, (int64_t)b.P);
+    }
+    want += total;
+  }
+  const bool fits = list_free(b, (int)min(want, (int64_t)b.P), b.list(n)) && want <= b.P;
+  if (!fits && bad == 0) bad = kSitePagedFull;
+  end_plan(b, bad, 0);
+  if (HERE) apply_here<kFork, true>(b, pl, parents, parents, nullptr, 0, n);
+}
+
+template <bool HERE>
+__global__ void __launch_bounds__(kPlanThreads) plan_free_kernel(const Book b, const int32_t* slots, int n) {
+  __shared__ SlotSet set;
+  begin_plan();
+  if (plan_stopped(b)) {
+    if (HERE) apply_here<kFree, false>(b, Pools{}, slots, nullptr, nullptr, 0, n);
+    return;
+  }
+  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int s = slots[i];
+    if ((unsigned)s < (unsigned)b.S && !length_ok(b, b.lengths[s])) bad = kSitePagedArgs;
+  }
+  copy_and_count(b, false);
+  end_plan(b, bad, 0);
+  if (HERE) apply_here<kFree, false>(b, Pools{}, slots, nullptr, nullptr, 0, n);
+}
+
+// last[i] = pages before, first[i] = pages after, start[i] = rows kept of the draft.
+template <bool HERE>
+__global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b, const Pools pl, const int32_t* slots,
+                                                                   const int32_t* drafted,
+                                                                   const int32_t* path, int depth, int n) {
+  __shared__ SlotSet set;
+  begin_plan();
+  if (plan_stopped(b)) {
+    if (HERE) apply_here<kAccept, true>(b, pl, slots, drafted, path, depth, n);
+    return;
+  }
+  int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
+  // One warp per entry: lanes read the path and the draft's pages side by side.
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+    const int s = slots[i];
+    if ((unsigned)s >= (unsigned)b.S) continue;  // reported above
+    const int64_t len = b.lengths[s], m = drafted[i];
+    if (m < 0 || m > len || !length_ok(b, len)) {
+      bad = kSitePagedArgs;
+      continue;
+    }
+    int kept = 0, prev = -1;
+    for (int d0 = 0; d0 < depth; d0 += 32) {
+      const int node = d0 + lane < depth ? path[(int64_t)i * depth + d0 + lane] : -1;
+      const unsigned ends = __ballot_sync(0xffffffffu, node < 0);
+      const int here = ends ? __ffs(ends) - 1 : 32;  // nodes before the first -1
+      int before = __shfl_up_sync(0xffffffffu, node, 1);
+      if (lane == 0) before = prev;
+      if (lane < here && (node <= before || node >= m)) bad = kSitePagedArgs;
+      prev = __shfl_sync(0xffffffffu, node, 31);
+      kept += here;
+      if (here < 32) break;
+    }
+    const int64_t begin = len - m;
+    const int pages = pages_of(len, b.page);
+    for (int c = (int)(begin / b.page) + lane; c < pages; c += 32) {
+      const int p = b.table[(int64_t)s * b.M + c];
+      if ((unsigned)p >= (unsigned)b.P) bad = kSitePagedTable;
+      else if (m > 0 && b.refs[p] != 1) bad = kSitePagedShared;
+    }
+    if (lane == 0) {
+      b.last(n)[i] = pages;
+      b.first()[i] = pages_of(begin + kept, b.page);
+      b.start(n)[i] = kept;
+    }
+  }
+  copy_and_count(b, false);
+  end_plan(b, bad, 0);
+  if (HERE) apply_here<kAccept, true>(b, pl, slots, drafted, path, depth, n);
+}
+
+// list = new id of each page, then the holes and the pages that fill them.
+__global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(const Book b) {
+  begin_plan();
+  if (plan_stopped(b)) return;
+  int32_t *to = b.list(0), *hole = to + b.P, *mover = hole + b.P;
+  const int lane = threadIdx.x & 31;
+  const int mine = copy_and_count(b, true);
+  int used;
+  block_scan(lane == 0 ? mine : 0, &used);
+  int lo, hi;
+  warp_pages(b.P, lo, hi);
+  int nh = 0, nm = 0;
+  for (int p0 = lo; p0 < hi; p0 += 32) {
+    const int p = p0 + lane, r = p < hi ? b.refs[p] : 0;
+    nh += __popc(__ballot_sync(0xffffffffu, p < hi && r <= 0 && p < used));
+    nm += __popc(__ballot_sync(0xffffffffu, p < hi && r > 0 && p >= used));
+  }
+  int holes, movers;
+  int rh = block_scan(lane == 0 ? nh : 0, &holes);
+  int rm = block_scan(lane == 0 ? nm : 0, &movers);
+  rh = __shfl_sync(0xffffffffu, rh, 0);
+  rm = __shfl_sync(0xffffffffu, rm, 0);
+  for (int p0 = lo; p0 < hi; p0 += 32) {
+    const int p = p0 + lane, r = p < hi ? b.refs[p] : 0;
+    const bool h = p < hi && r <= 0 && p < used, m = p < hi && r > 0 && p >= used;
+    const unsigned bh = __ballot_sync(0xffffffffu, h), bm = __ballot_sync(0xffffffffu, m);
+    const unsigned lt = (1u << lane) - 1;
+    if (p < hi) to[p] = p;
+    if (h) hole[rh + __popc(bh & lt)] = p;
+    if (m) mover[rm + __popc(bm & lt)] = p;
+    rh += __popc(bh);
+    rm += __popc(bm);
+  }
+  __syncthreads();  // also orders the lists for this block's readers
+  // As many used pages stand above `used` as free ones below it.
+  for (int i = threadIdx.x; i < movers; i += blockDim.x) {
+    const int src = mover[i], dst = hole[i];
+    to[src] = dst;
+    b.refs_out[dst] = b.refs[src];
+    b.refs_out[src] = 0;
+  }
+  end_plan(b, 0, movers);
 }
 
 // ------------------------------------------------------------------ write
@@ -710,10 +752,16 @@ template <int OP, int W>
 int launch_apply_w(const Book& b, const Pools& pl, const int32_t* slots, const int32_t* aux,
                    const int32_t* path, int depth, int n, int table_blocks, int move_blocks, cudaStream_t s) {
   SCREE_CUDA_TRY(launch_dependent(apply_kernel<OP, W>, dim3((unsigned)(table_blocks + move_blocks)),
-                                  dim3(kThreads), 0, s, b, pl, slots, aux, path, depth, n, table_blocks));
+                                  dim3(kThreads), 0, s, 1, b, pl, slots, aux, path, depth, n, table_blocks));
   count_launch();
   return SCREE_OK;
 }
+// A call is applied by its plan's CTA if that takes it no longer than a second
+// launch: measured, XXMEASURE.
+bool apply_by_plan(const Book& b, int64_t units, int w) {
+  return (int64_t)b.S * b.M <= kHereEntries && units <= kHereWarps && w == 16;
+}
+
 // `units`: warps of row-moving work (an upper bound where only the device knows).
 template <int OP>
 int launch_apply(const Book& b, const Pools& pl, const int32_t* slots, const int32_t* aux,
@@ -749,8 +797,11 @@ extern "C" int scree_paged_reserve(const scree_paged_book* book, const int32_t* 
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  SCREE_CUDA_TRY(launch_dependent(plan_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, counts, (int)n));
+  const bool here = apply_by_plan(b, 0, 16);
+  SCREE_CUDA_TRY(launch_dependent(here ? plan_reserve_kernel<true> : plan_reserve_kernel<false>, dim3(1),
+                                  dim3(kPlanThreads), 0, s, 1, b, slots, counts, (int)n));
   count_launch();
+  if (here) return SCREE_OK;
   return launch_apply<kReserve>(b, Pools{}, slots, counts, nullptr, 0, (int)n, 0, s);
 }
 
@@ -767,12 +818,14 @@ extern "C" int scree_paged_accept(const scree_paged_book* book, const scree_page
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  SCREE_CUDA_TRY(launch_dependent(plan_accept_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, drafted, path, (int)depth, (int)n));
-  count_launch();
   const int w = pick_width(pl.row_bytes, {(uintptr_t)pl.k, (uintptr_t)pl.v});
-  const int64_t threads = n * pl.L * 2 * pl.H * (pl.row_bytes / w);
-  return launch_apply<kAccept>(b, pl, slots, drafted, path, (int)depth, (int)n,
-                               depth == 0 ? 0 : (threads + 31) / 32, s);
+  const int64_t threads = depth == 0 ? 0 : n * pl.L * 2 * pl.H * (pl.row_bytes / w);
+  const bool here = apply_by_plan(b, (threads + 31) / 32, w);
+  SCREE_CUDA_TRY(launch_dependent(here ? plan_accept_kernel<true> : plan_accept_kernel<false>, dim3(1),
+                                  dim3(kPlanThreads), 0, s, 1, b, pl, slots, drafted, path, (int)depth, (int)n));
+  count_launch();
+  if (here) return SCREE_OK;
+  return launch_apply<kAccept>(b, pl, slots, drafted, path, (int)depth, (int)n, (threads + 31) / 32, s);
 }
 
 extern "C" int scree_paged_fork(const scree_paged_book* book, const scree_paged_pools* pools,
@@ -786,9 +839,13 @@ extern "C" int scree_paged_fork(const scree_paged_book* book, const scree_paged_
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  SCREE_CUDA_TRY(launch_dependent(plan_fork_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, parents, children, (int)n));
+  const int64_t units = n * pl.L * 2 * pl.H;
+  const bool here = apply_by_plan(b, units, pick_width(pl.row_bytes, {(uintptr_t)pl.k, (uintptr_t)pl.v}));
+  SCREE_CUDA_TRY(launch_dependent(here ? plan_fork_kernel<true> : plan_fork_kernel<false>, dim3(1),
+                                  dim3(kPlanThreads), 0, s, 1, b, pl, parents, children, (int)n));
   count_launch();
-  return launch_apply<kFork>(b, pl, parents, parents, nullptr, 0, (int)n, n * pl.L * 2 * pl.H, s);
+  if (here) return SCREE_OK;
+  return launch_apply<kFork>(b, pl, parents, parents, nullptr, 0, (int)n, units, s);
 }
 
 extern "C" int scree_paged_free(const scree_paged_book* book, const int32_t* slots, int64_t n, void* workspace,
@@ -799,8 +856,11 @@ extern "C" int scree_paged_free(const scree_paged_book* book, const int32_t* slo
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  SCREE_CUDA_TRY(launch_dependent(plan_free_kernel, dim3(1), dim3(kPlanThreads), 0, s, b, slots, (int)n));
+  const bool here = apply_by_plan(b, 0, 16);
+  SCREE_CUDA_TRY(launch_dependent(here ? plan_free_kernel<true> : plan_free_kernel<false>, dim3(1),
+                                  dim3(kPlanThreads), 0, s, 1, b, slots, (int)n));
   count_launch();
+  if (here) return SCREE_OK;
   return launch_apply<kFree>(b, Pools{}, slots, nullptr, nullptr, 0, (int)n, 0, s);
 }
 
@@ -813,7 +873,7 @@ extern "C" int scree_paged_compact(const scree_paged_book* book, const scree_pag
   SCREE_BIND_DEVICE(stream, book->table);
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
-  SCREE_CUDA_TRY(launch_dependent(plan_compact_kernel, dim3(1), dim3(kPlanThreads), 0, s, b));
+  SCREE_CUDA_TRY(launch_dependent(plan_compact_kernel, dim3(1), dim3(kPlanThreads), 0, s, 1, b));
   count_launch();
   // At most half of the pages can move.
   return launch_apply<kCompact>(b, pl, nullptr, nullptr, nullptr, 0, 0, (book->P / 2 + 1) * pl.L * 2 * 8, s);

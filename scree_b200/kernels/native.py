@@ -555,27 +555,28 @@ class TokenLogprobs(NamedTuple):
     top_ids: Any
 
 
-def _logprobs_fwd(logits, targets, top_k):
+def _logprobs_fwd(logits, targets, top_k, want_norm):
     assert logits.is_cuda and logits.ndim == 2, "logits must be a (tokens, vocabulary) CUDA tensor"
     assert logits.dtype in (torch.float16, torch.bfloat16, torch.float32), "fp16, bf16 or fp32 only"
     N, V = logits.shape
-    assert targets.shape == (N,) and targets.device == logits.device, "targets must be (tokens,) on logits' device"
+    dev = logits.device
+    assert targets.shape == (N,) and targets.device == dev, "targets must be (tokens,) on logits' device"
     assert targets.dtype in (torch.int32, torch.int64), "targets must be int32 or int64"
-    if logits.stride(1) != 1 or (N > 1 and logits.stride(0) < V):
+    sr, sv = logits.stride()
+    if sv != 1 or (N > 1 and sr < V):
         logits = logits.contiguous()
-    targets = targets.contiguous()
-    dev, top_k = logits.device, int(top_k)
-    logp, entropy = (torch.empty(N, dtype=torch.float32, device=dev) for _ in range(2))
-    norm = torch.empty((N, 2), dtype=torch.float32, device=dev)  # kept for the gradient
-    top_logp = torch.empty((N, max(top_k, 0)), dtype=torch.float32, device=dev)
+        sr = V
+    if not targets.is_contiguous():
+        targets = targets.contiguous()
+    f32 = torch.float32
+    logp, entropy = torch.empty(N, dtype=f32, device=dev), torch.empty(N, dtype=f32, device=dev)
+    norm = torch.empty((N, 2), dtype=f32, device=dev) if want_norm else None  # for the gradient
+    top_logp = torch.empty((N, max(top_k, 0)), dtype=f32, device=dev)
     top_ids = torch.empty((N, max(top_k, 0)), dtype=torch.int64, device=dev)
-    lib, code = _lib.load(), _lib.dtype_code(logits.dtype)
-    size = lib.scree_token_logprobs_workspace_size(N, V, top_k, code)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    rc = lib.scree_token_logprobs_fwd(
-        logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, N, V,
-        top_k, code, logp.data_ptr(), entropy.data_ptr(), norm.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
-        _ptr(ws), size, _lib.stream_ptr(dev))
+    rc = _lib.load().scree_token_logprobs_fwd(
+        logits.data_ptr(), sr, targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, N, V, top_k,
+        _lib.dtype_code(logits.dtype), logp.data_ptr(), entropy.data_ptr(), _ptr(norm), top_logp.data_ptr(),
+        top_ids.data_ptr(), _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "token_logprobs")
     return logits, targets, logp, entropy, norm, top_logp, top_ids
@@ -587,14 +588,14 @@ def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
     logits.  A negative target means that no token is given (logp 0); a target >= V
     sets the device status word.  Equal logits rank by lower index; a row whose logits
     are all -inf has logp -inf and entropy 0.  No reference counterpart."""
-    _, _, logp, entropy, _, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
+    _, _, logp, entropy, _, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k, False)
     return TokenLogprobs(logp, entropy, top_logp, top_ids)
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
-        logits, targets, logp, entropy, norm, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k)
+        logits, targets, logp, entropy, norm, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k, True)
         ctx.save_for_backward(logits, targets, norm, entropy, top_ids)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
@@ -604,7 +605,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy, g_top, _):
         logits, targets, norm, entropy, top_ids = ctx.saved_tensors
         N, V = logits.shape
-        f32 = lambda g: None if g is None else g.to(torch.float32).contiguous()  # noqa: E731
+        f32 = lambda g: g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) \
+            else g.to(torch.float32).contiguous()  # noqa: E731
         g_logp, g_entropy, g_top = f32(g_logp), f32(g_entropy), f32(g_top)
         dx = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
         rc = _lib.load().scree_token_logprobs_bwd(

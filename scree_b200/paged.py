@@ -67,11 +67,16 @@ class PagedCache:
                 raise ValueError("table, lengths and refs must be contiguous int32")
         if len({t.device for t in (self.k, self.v, self.table, self.lengths, self.refs)}) != 1:
             raise ValueError("all tensors of a cache must be on one device")
-        L, P, H, _, D = self.k.shape
-        size = _lib.load().scree_paged_workspace_size(self.table.shape[0], P)
-        object.__setattr__(self, "_work", torch.empty(size, dtype=torch.uint8, device=self.k.device))
-        object.__setattr__(self, "_pools", _lib.PagedPools(self.k.data_ptr(), self.v.data_ptr(), L, H,
-                                                           D * self.k.element_size()))
+        L, P, H, page, D = self.k.shape
+        S, M = self.table.shape
+        work = torch.empty(_lib.load().scree_paged_workspace_size(S, P), dtype=torch.uint8, device=self.k.device)
+        pools = _lib.PagedPools(self.k.data_ptr(), self.v.data_ptr(), L, H, D * self.k.element_size())
+        # What every call of this cache and those derived from it passes on.
+        pools.sizes = (S, M, P, page, H, D)
+        pools.dtype, pools.device = self.k.dtype, self.k.device
+        pools.ref, pools.work = ctypes.byref(pools), (work.data_ptr(), work.numel())
+        object.__setattr__(self, "_work", work)
+        object.__setattr__(self, "_pools", pools)
 
     @property
     def page_size(self) -> int:
@@ -92,103 +97,109 @@ def paged_cache(layers: int, pages: int, page_size: int, kv_heads: int, head_dim
                       refs=torch.zeros(pages, **i32))
 
 
-def _ints(t, n, what, cache):
+def _ints(t, n, what, device):
     """An int32 CUDA vector (of n entries, if n is given) next to the cache."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == cache.k.device):
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device):
         raise TypeError(f"{what} must be an int32 tensor on the cache's device")
     if t.ndim != 1 or (n is not None and t.shape[0] != n):
         raise ValueError(f"{what} must be 1-D" + (f" with {n} entries" if n is not None else ""))
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _book_call(cache: PagedCache, name: str, *args) -> PagedCache:
-    table, lengths, refs = torch.empty_like(cache.table), torch.empty_like(cache.lengths), torch.empty_like(cache.refs)
-    S, M = cache.table.shape
-    book = _lib.PagedBook(cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(), table.data_ptr(),
-                          lengths.data_ptr(), refs.data_ptr(), S, M, cache.refs.shape[0], cache.k.shape[3])
-    rc = getattr(_lib.load(), name)(ctypes.byref(book), *args, cache._work.data_ptr(), cache._work.numel(),
-                                    _lib.stream_ptr(cache.k.device))
+def _book_call(cache: PagedCache, fn, name: str, *args) -> PagedCache:
+    t, le, r, pools = cache.table, cache.lengths, cache.refs, cache._pools
+    table, lengths, refs = torch.empty_like(t), torch.empty_like(le), torch.empty_like(r)
+    S, M, P, page, _, _ = pools.sizes
+    book = _lib.PagedBook(t.data_ptr(), le.data_ptr(), r.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+                          refs.data_ptr(), S, M, P, page)
+    rc = fn(ctypes.byref(book), *args, *pools.work, _lib.stream_ptr(pools.device))
     if rc:
         _lib.check(rc, name)
-    return PagedCache(k=cache.k, v=cache.v, table=table, lengths=lengths, refs=refs, _work=cache._work,
-                      _pools=cache._pools)
+    return PagedCache(cache.k, cache.v, table, lengths, refs, cache._work, pools)
 
 
 def paged_reserve(cache: PagedCache, slots, counts) -> PagedCache:
     """Grows slot slots[i] by counts[i] tokens, from the lowest free pages."""
-    slots = _ints(slots, None, "slots", cache)
-    counts = _ints(counts, slots.shape[0], "counts", cache)
-    return _book_call(cache, "scree_paged_reserve", slots.data_ptr(), counts.data_ptr(), slots.shape[0])
+    dev = cache._pools.device
+    slots = _ints(slots, None, "slots", dev)
+    n = slots.shape[0]
+    counts = _ints(counts, n, "counts", dev)
+    return _book_call(cache, _lib.load().scree_paged_reserve, "paged_reserve", slots.data_ptr(), counts.data_ptr(), n)
 
 
 def paged_accept(cache: PagedCache, slots, drafted, path) -> PagedCache:
     """Of the last drafted[i] tokens of slot slots[i], keeps those whose indices into the
     draft row i of ``path`` (n, depth) lists, ascending and ended by -1; their rows move to
     the front of the draft in every layer, the others are dropped and their pages freed."""
-    slots = _ints(slots, None, "slots", cache)
-    drafted = _ints(drafted, slots.shape[0], "drafted", cache)
-    if not (isinstance(path, torch.Tensor) and path.dtype == torch.int32 and path.device == cache.k.device):
+    dev = cache._pools.device
+    slots = _ints(slots, None, "slots", dev)
+    n = slots.shape[0]
+    drafted = _ints(drafted, n, "drafted", dev)
+    if not (isinstance(path, torch.Tensor) and path.dtype == torch.int32 and path.device == dev):
         raise TypeError("path must be an int32 tensor on the cache's device")
-    if path.ndim != 2 or path.shape[0] != slots.shape[0]:
+    if path.ndim != 2 or path.shape[0] != n:
         raise ValueError("path must be (slots, depth)")
     path = path.contiguous()
-    return _book_call(cache, "scree_paged_accept", ctypes.byref(cache._pools), slots.data_ptr(), drafted.data_ptr(),
-                      path.data_ptr(), path.shape[1], slots.shape[0])
+    return _book_call(cache, _lib.load().scree_paged_accept, "paged_accept", cache._pools.ref, slots.data_ptr(),
+                      drafted.data_ptr(), path.data_ptr(), path.shape[1], n)
 
 
 def paged_fork(cache: PagedCache, parents, children) -> PagedCache:
     """The empty slots children[i] become copies of parents[i] (which may repeat, and may not
     be children): full pages are shared, a part-filled page is copied."""
-    parents = _ints(parents, None, "parents", cache)
-    children = _ints(children, parents.shape[0], "children", cache)
-    return _book_call(cache, "scree_paged_fork", ctypes.byref(cache._pools), parents.data_ptr(), children.data_ptr(),
-                      parents.shape[0])
+    dev = cache._pools.device
+    parents = _ints(parents, None, "parents", dev)
+    n = parents.shape[0]
+    children = _ints(children, n, "children", dev)
+    return _book_call(cache, _lib.load().scree_paged_fork, "paged_fork", cache._pools.ref, parents.data_ptr(),
+                      children.data_ptr(), n)
 
 
 def paged_free(cache: PagedCache, slots) -> PagedCache:
     """Empties the slots; pages that no other slot holds become free."""
-    slots = _ints(slots, None, "slots", cache)
-    return _book_call(cache, "scree_paged_free", slots.data_ptr(), slots.shape[0])
+    slots = _ints(slots, None, "slots", cache._pools.device)
+    return _book_call(cache, _lib.load().scree_paged_free, "paged_free", slots.data_ptr(), slots.shape[0])
 
 
 def paged_compact(cache: PagedCache) -> PagedCache:
     """Moves used pages so that they are the first of the pools; of the pages above their
     count, the k-th used one goes to the k-th hole below it."""
-    return _book_call(cache, "scree_paged_compact", ctypes.byref(cache._pools))
+    return _book_call(cache, _lib.load().scree_paged_compact, "paged_compact", cache._pools.ref)
 
 
-def _offsets(arr: Array):
+def _offsets(arr: Array, device):
+    """Offsets on the device, whether they are int64, sequences."""
     offs = arr.offsets
-    if not (isinstance(offs, torch.Tensor) and offs.device == arr.values.device
-            and offs.dtype in (torch.int32, torch.int64)):
-        offs = torch.as_tensor(arr.host_offsets(), dtype=torch.int64, device=arr.values.device)
-    return offs.contiguous()
+    if not (isinstance(offs, torch.Tensor) and offs.device == device and offs.dtype in (torch.int32, torch.int64)):
+        offs = torch.as_tensor(arr.host_offsets(), dtype=torch.int64, device=device)
+    if not offs.is_contiguous():
+        offs = offs.contiguous()
+    return offs, 1 if offs.dtype == torch.int64 else 0, offs.shape[0] - 1
 
 
 def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> None:
     """Writes the rows of sequence b of k / v (T, kv_heads, head_dim) as the K / V of the last
     tokens of slot slots[b] in one layer."""
-    slots = _ints(slots, k.batch_size, "slots", cache)
-    kt, vt = k.values, v.values
-    L, P, H, page, D = cache.k.shape
-    if tuple(kt.shape[1:]) != (H, D) or kt.shape != vt.shape:
+    kt, vt, pools = k.values, v.values, cache._pools
+    S, M, P, page, H, D = pools.sizes
+    dev = pools.device
+    if kt.ndim != 3 or kt.shape[1] != H or kt.shape[2] != D or kt.shape != vt.shape:
         raise ValueError(f"k and v must be (tokens, {H}, {D})")
-    if kt.dtype != cache.k.dtype or vt.dtype != cache.k.dtype:
+    if kt.dtype != pools.dtype or vt.dtype != pools.dtype:
         raise ValueError("k and v must have the cache's dtype")
-    if kt.device != cache.k.device or vt.device != cache.k.device:
+    if kt.device != dev or vt.device != dev:
         raise TypeError("k and v must be on the cache's device")
-    if kt.stride(2) != 1:
-        kt = kt.contiguous()
-    if vt.stride(2) != 1:
-        vt = vt.contiguous()
-    offs = _offsets(k)
+    offs, is64, B = _offsets(k, dev)
+    slots = _ints(slots, B, "slots", dev)
+    (kr, kh, kd), (vr, vh, vd) = kt.stride(), vt.stride()
+    if kd != 1 or vd != 1:
+        kt, vt = kt.contiguous(), vt.contiguous()
+        (kr, kh, _), (vr, vh, _) = kt.stride(), vt.stride()
     es = kt.element_size()
-    S, M = cache.table.shape
     rc = _lib.load().scree_paged_write(
-        ctypes.byref(cache._pools), cache.table.data_ptr(), cache.lengths.data_ptr(), S, M, P, page, int(layer),
-        slots.data_ptr(), kt.data_ptr(), kt.stride(0) * es, kt.stride(1) * es, vt.data_ptr(), vt.stride(0) * es,
-        vt.stride(1) * es, offs.data_ptr(), 1 if offs.dtype == torch.int64 else 0, k.batch_size, kt.shape[0],
-        _lib.stream_ptr(kt.device))
+        pools.ref, cache.table.data_ptr(), cache.lengths.data_ptr(), S, M, P, page, layer, slots.data_ptr(),
+        kt.data_ptr(), kr * es, kh * es, vt.data_ptr(), vr * es, vh * es, offs.data_ptr(), is64, B, kt.shape[0],
+        _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "paged_write")
 
@@ -205,12 +216,12 @@ def tree_mask(parents: Array, max_nodes: int = None):
     if max_nodes is None:
         host = parents.host_offsets()
         max_nodes = max(b - a for a, b in zip(host, host[1:]))
-    vals, offs = parents.values.contiguous(), _offsets(parents)
+    vals = parents.values.contiguous()
+    offs, is64, B = _offsets(parents, vals.device)
     words = max(1, -(-int(max_nodes) // 64))
     mask = torch.empty((vals.shape[0], words), dtype=torch.int64, device=vals.device)
-    rc = _lib.load().scree_tree_mask(vals.data_ptr(), offs.data_ptr(), 1 if offs.dtype == torch.int64 else 0,
-                                     parents.batch_size, vals.shape[0], words, mask.data_ptr(),
-                                     _lib.stream_ptr(vals.device))
+    rc = _lib.load().scree_tree_mask(vals.data_ptr(), offs.data_ptr(), is64, B, vals.shape[0], words,
+                                     mask.data_ptr(), _lib.stream_ptr(vals.device))
     _lib.check(rc, "tree_mask")
     return mask
 
@@ -225,41 +236,41 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     gets 0 and LSE -inf.  heads is a multiple of the cache's kv_heads; head_dim 32, 64 or 128;
     page_size a multiple of 16; at most 4096 sequences.  Returns an Array on q's offsets (and
     the LSE (T, heads) fp32 when ``return_lse``)."""
-    qt = q.values
+    qt, pools = q.values, cache._pools
     _require_cuda(qt, "paged_attention")
-    slots = _ints(slots, q.batch_size, "slots", cache)
-    assert qt.dtype in (torch.float16, torch.bfloat16), "fp16 or bf16 only"
-    L, P, Hkv, page, D = cache.k.shape
-    assert qt.dtype == cache.k.dtype and qt.device == cache.k.device, "q must have the cache's dtype and device"
+    S, M, P, page, Hkv, D = pools.sizes
+    dev, dtype = qt.device, qt.dtype
+    assert dtype in (torch.float16, torch.bfloat16), "fp16 or bf16 only"
+    assert dtype == pools.dtype and dev == pools.device, "q must have the cache's dtype and device"
     assert qt.ndim == 3 and qt.shape[2] == D and qt.shape[1] % Hkv == 0, \
         "q must be (tokens, heads, head_dim) with heads a multiple of the cache's kv_heads"
     T, H, _ = qt.shape
-    words = 0
+    offs, is64, B = _offsets(q, dev)
+    slots = _ints(slots, B, "slots", dev)
+    mask_ptr, words = None, 0
     if mask is not None:
-        if not (isinstance(mask, torch.Tensor) and mask.dtype == torch.int64 and mask.device == qt.device):
+        if not (isinstance(mask, torch.Tensor) and mask.dtype == torch.int64 and mask.device == dev):
             raise TypeError("mask must be an int64 tensor on q's device")
         if mask.ndim != 2 or mask.shape[0] != T or mask.shape[1] < 1:
             raise ValueError("mask must be (tokens, words)")
         mask = mask.contiguous()
-        words = mask.shape[1]
-    if qt.stride(2) != 1 or qt.stride(0) % 8 or qt.stride(1) % 8 or qt.data_ptr() % 16:
+        mask_ptr, words = mask.data_ptr(), mask.shape[1]
+    sr, sh, sd = qt.stride()
+    if sd != 1 or sr % 8 or sh % 8 or qt.data_ptr() % 16:
         qt = qt.clone(memory_format=torch.contiguous_format)  # contiguous() would keep a misaligned base
-    out = torch.empty((T, H, D), dtype=qt.dtype, device=qt.device)
-    lse = torch.empty((T, H), dtype=torch.float32, device=qt.device) if return_lse else None
+        sr, sh, _ = qt.stride()
+    out = torch.empty((T, H, D), dtype=dtype, device=dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T:
         lib = _lib.load()
-        offs = _offsets(q)
-        S, M = cache.table.shape
-        B = q.batch_size
-        ws = torch.empty(lib.scree_attn_fwd_paged_workspace_size(B, T, H, Hkv, D), dtype=torch.uint8, device=qt.device)
+        size = lib.scree_attn_fwd_paged_workspace_size(B, T, H, Hkv, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         rc = lib.scree_attn_fwd_paged(
-            qt.data_ptr(), qt.stride(0), qt.stride(1), ctypes.byref(cache._pools), int(layer), cache.table.data_ptr(),
-            cache.lengths.data_ptr(), S, M, P, page, slots.data_ptr(), offs.data_ptr(),
-            1 if offs.dtype == torch.int64 else 0, B, T, H, D, _lib.dtype_code(qt.dtype), 1.0 / math.sqrt(D),
-            mask.data_ptr() if mask is not None else None, words, out.data_ptr(), out.stride(0), out.stride(1),
-            lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), _lib.stream_ptr(qt.device))
+            qt.data_ptr(), sr, sh, pools.ref, layer, cache.table.data_ptr(), cache.lengths.data_ptr(), S, M, P, page,
+            slots.data_ptr(), offs.data_ptr(), is64, B, T, H, D, _lib.BF16 if dtype == torch.bfloat16 else _lib.F16,
+            1.0 / math.sqrt(D), mask_ptr, words, out.data_ptr(), H * D, D, lse.data_ptr() if return_lse else None,
+            ws.data_ptr(), size, _lib.stream_ptr(dev))
         if rc:
             _lib.check(rc, "paged_attention")
     res = q._with_values(out)
     return (res, lse) if return_lse else res
-
