@@ -403,7 +403,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedParams p, int R) {
   constexpr int E = D / 32;  // columns of a lane
   __shared__ float sm_o[kJoinWarps][D];
-  __shared__ float sm_l[kJoinWarps];
+  __shared__ float2 sm_ml[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
   const int64_t c = (int64_t)blockIdx.x + 1;
@@ -423,43 +423,71 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   const int sub = warp % share;
   const int step = (np - 1) * (kJoinWarps / share);
   for (int row = (int)(c - w0 - 1) * (kJoinWarps / share) + warp / share; row < rows; row += step) {
-    float mx = -INFINITY;
-    for (int i = lane; i < np; i += 32) mx = fmaxf(mx, p.part_ml[slot_of(i) * R + row].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float acc[E], sum = 0.f;
+    // This warp's pieces sub, sub + share, ...: 32 at a time their (m, l) in the
+    // lanes, their O rows eight loads at a time.
+    float mx = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 8
-    for (int i = sub; i < np; i += share) {
-      const int64_t at = slot_of(i) * R + row;
-      const float2 ml = p.part_ml[at];
-      const float* src = p.part_o + at * D + lane * E;
-      float x[E];
-      if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-      else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
-      else x[0] = *src;
-      const float f = ex2_approx(ml.x - ref);
-      sum = fmaf(f, ml.y, sum);
+    for (int i0 = sub; i0 < np; i0 += 32 * share) {
+      const int mine = i0 + lane * share;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (mine < np) ml = p.part_ml[slot_of(mine) * R + row];
+      const int here = min(32, (np - i0 + share - 1) / share);
+      float x[8][E];
+      auto load = [&](int t0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+        for (int t = 0; t < 8; ++t) {
+          const int i = min(i0 + (t0 + t) * share, np - 1);
+          const float* src = p.part_o + (slot_of(i) * R + row) * D + lane * E;
+          if constexpr (E == 4) *reinterpret_cast<float4*>(x[t]) = *reinterpret_cast<const float4*>(src);
+          else if constexpr (E == 2) *reinterpret_cast<float2*>(x[t]) = *reinterpret_cast<const float2*>(src);
+          else x[t][0] = *src;
+        }
+      };
+      load(0);
+      float m2 = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+      m2 = fmaxf(m2, mx);
+      const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_approx(mx - ref), wt = ex2_approx(ml.x - ref);
+      mx = m2;
+      sum = sum * scale + wt * ml.y;  // (a lane's own pieces)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= scale;
+      for (int t0 = 0; t0 < here; t0 += 8) {
+        if (t0 > 0) load(t0);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float f = __shfl_sync(0xffffffffu, wt, (t0 + t) & 31);
+          if (t0 + t < here) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[t][e], acc[e]);
+          }
+        }
+      }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (share > 1) {
       __syncthreads();  // the row before has been read
 #pragma unroll
       for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = acc[e];
-      if (lane == 0) sm_l[warp] = sum;
+      if (lane == 0) sm_ml[warp] = make_float2(mx, sum);
       __syncthreads();
       if (warp > 0) continue;
+      mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, sm_ml[w].x);
+      const float ref = mx == -INFINITY ? 0.f : mx;
       sum = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) {
-        sum += sm_l[w];
+        const float f = ex2_approx(sm_ml[w].x - ref);
+        sum = fmaf(f, sm_ml[w].y, sum);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += sm_o[w][lane * E + e];
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, sm_o[w][lane * E + e], acc[e]);
       }
     }
     const int a = d.rt * R + row, hq = d.h * p.G + a % p.G;

@@ -617,28 +617,46 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
   if (r >= tpt * p.G || i >= n) return;
   const int64_t first = 2 * w0 + (worker_start(w0, U, N) == d.s0 ? 0 : 1);
   auto part_of = [&](int j) { return (j == 0 ? first : 2 * (w0 + j)) * 2 + x; };
-  float mx = -INFINITY;
-#pragma unroll 4
-  for (int j = 0; j < np; ++j) mx = fmaxf(mx, p.part_ml[part_of(j) * BM + r].x);
-  const float ref = mx == -INFINITY ? 0.f : mx;
   constexpr int E = D / 4 / kJoinWarps;  // float4 of a warp
+  constexpr int J = 4;                   // pieces loaded side by side
+  float mx = -INFINITY, sum = 0.f;
   float4 acc[E];
-  float sum = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
   const float4* po = reinterpret_cast<const float4*>(p.part_o);
-#pragma unroll 2
-  for (int j = 0; j < np; ++j) {
-    const float2 ml = p.part_ml[part_of(j) * BM + r];
-    const float f = ex2_approx(ml.x - ref);
-    sum = fmaf(f, ml.y, sum);
+  for (int j0 = 0; j0 < np; j0 += J) {
+    float2 ml[J];
+    float4 v[J][E];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int64_t part = part_of(min(j0 + j, np - 1));
+      ml[j] = j0 + j < np ? p.part_ml[part * BM + r] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[j][e] = po[(part * (D / 4) + warp * E + e) * BM + r];
+    }
+    const float m2 = fmaxf(mx, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_approx(mx - ref);
+    mx = m2;
+    sum *= scale;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float4 v = po[(part_of(j) * (D / 4) + warp * E + e) * BM + r];
-      acc[e].x = fmaf(f, v.x, acc[e].x);
-      acc[e].y = fmaf(f, v.y, acc[e].y);
-      acc[e].z = fmaf(f, v.z, acc[e].z);
-      acc[e].w = fmaf(f, v.w, acc[e].w);
+      acc[e].x *= scale;
+      acc[e].y *= scale;
+      acc[e].z *= scale;
+      acc[e].w *= scale;
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (j0 + j >= np) continue;
+      const float f = ex2_approx(ml[j].x - ref);
+      sum = fmaf(f, ml[j].y, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        acc[e].x = fmaf(f, v[j][e].x, acc[e].x);
+        acc[e].y = fmaf(f, v[j][e].y, acc[e].y);
+        acc[e].z = fmaf(f, v[j][e].z, acc[e].z);
+        acc[e].w = fmaf(f, v[j][e].w, acc[e].w);
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;

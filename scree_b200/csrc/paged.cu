@@ -106,14 +106,16 @@ struct SlotSet {  // slots named by the call, for the check that they differ
 
 // Warp w of the plan owns the pages [lo, hi).  Pass 1 copies refs and counts the
 // pages that match; pass 2 lists matching pages by rank.
-__device__ __forceinline__ void warp_pages(int P, int& lo, int& hi) {
-  const int per = (int)((((int64_t)P + 31) / 32 + 31) / 32 * 32);
-  lo = min((int64_t)P, (int64_t)(threadIdx.x >> 5) * per);
+__device__ __forceinline__ void warp_pages(int P, int& lo, int& hi, int warp, int warps) {
+  const int per = (int)((((int64_t)P + warps - 1) / warps + 31) / 32 * 32);
+  lo = min((int64_t)P, (int64_t)warp * per);
   hi = min((int64_t)P, (int64_t)lo + per);
 }
-__device__ int copy_and_count(const Book& b, bool used) {
+__device__ __forceinline__ void warp_pages(int P, int& lo, int& hi) { warp_pages(P, lo, hi, threadIdx.x >> 5, 32); }
+// (By warp `warp` of `warps`.)
+__device__ int copy_and_count(const Book& b, bool used, int warp, int warps) {
   int lo, hi;
-  warp_pages(b.P, lo, hi);
+  warp_pages(b.P, lo, hi, warp, warps);
   const int lane = threadIdx.x & 31;
   int n = 0;
   constexpr int U = 8;  // loads in flight per lane
@@ -136,6 +138,9 @@ __device__ int copy_and_count(const Book& b, bool used) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n;
+}
+__device__ __forceinline__ int copy_and_count(const Book& b, bool used) {
+  return copy_and_count(b, used, threadIdx.x >> 5, 32);
 }
 // The lowest `want` free pages into list; false if there are fewer.
 __device__ bool list_free(const Book& b, int want, int32_t* list) {
@@ -323,38 +328,50 @@ __device__ __forceinline__ void apply_moves(const Book& b, const Pools& pl, cons
                    (hi - lo) * W, lane);
     }
   } else if constexpr (OP == kAccept) {
-    // Row d of the path moves to row d of the draft.  A thread owns one W-byte
-    // column of the rows and moves it through the whole path: rows only move
-    // down (path[d] >= d, ascending), so reading a batch of rows before writing
-    // it reads nothing that an earlier batch wrote.
+    // Row d of the path moves to row d of the draft.  A task is an entry's rows in
+    // one pool of one layer, a run of 32 W-byte columns of them; a lane owns a
+    // column and moves it through the whole path: rows only move down (path[d] >=
+    // d, ascending), so reading a batch of rows before writing it reads nothing
+    // that an earlier batch wrote.
     using V = typename Vec<W>::T;
-    const int vpr = (int)(pl.row_bytes / W), cols = pl.H * vpr;
-    const int64_t tasks = (int64_t)n * pl.L * 2 * cols;
+    const unsigned vpr = (unsigned)(pl.row_bytes / W), cols = pl.H * vpr, runs = (cols + 31) / 32;
+    const unsigned pools = (unsigned)pl.L * 2 * runs;
     constexpr int U = 8;
-    for (int64_t t = warp * 32 + lane; t < tasks; t += warps * 32) {
-      const int col = (int)(t % cols);
-      const int64_t r = t / cols;
-      const int pool = (int)(r & 1), layer = (int)((r >> 1) % pl.L), i = (int)((r >> 1) / pl.L);
+    for (int64_t t = warp; t < (int64_t)n * pools; t += warps) {
+      const int i = (int)(t / pools);
+      const unsigned r = (unsigned)(t - (int64_t)i * pools), pool = r / runs, col = (r - pool * runs) * 32 + lane;
       const int kept = b.start(n)[i];
       const int s = slots[i];
       const int begin = b.lengths[s] - aux[i];
       const int32_t* row = b.table + (int64_t)s * b.M;
-      char* base = (pool ? pl.v : pl.k) + layer * pl.layer_bytes +
+      char* base = (pool & 1 ? pl.v : pl.k) + (pool >> 1) * pl.layer_bytes +
                    (int64_t)(col / vpr) * b.page * pl.row_bytes + (int64_t)(col % vpr) * W;
-      auto at = [&](int pos) {
-        return reinterpret_cast<V*>(base + row[pos / b.page] * pl.page_bytes + (int64_t)(pos % b.page) * pl.row_bytes);
+      // Byte offset of a row of the draft in its layer.
+      auto place = [&](int d) {
+        const unsigned pos = (unsigned)(begin + d), pg = pos / (unsigned)b.page;
+        return row[pg] * pl.page_bytes + (int64_t)(pos - pg * b.page) * pl.row_bytes;
       };
-      for (int d0 = 0; d0 < kept; d0 += U) {
-        V x[U];
-        int from[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          from[u] = d0 + u < kept ? path[(int64_t)i * depth + d0 + u] : d0 + u;
-          if (from[u] != d0 + u) x[u] = *at(begin + from[u]);
+      for (int d0 = 0; d0 < kept; d0 += 32) {
+        // 32 steps of the path at a time in the lanes.
+        int64_t src = 0, dst = 0;
+        if (d0 + lane < kept) {
+          src = place(path[(int64_t)i * depth + d0 + lane]);
+          dst = place(d0 + lane);
         }
+        const int here = min(32, kept - d0);
+        for (int e0 = 0; e0 < here; e0 += U) {
+          V x[U];
+          int64_t from[U], to[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (from[u] != d0 + u) *at(begin + d0 + u) = x[u];
+          for (int u = 0; u < U; ++u) {
+            from[u] = __shfl_sync(0xffffffffu, src, (e0 + u) & 31);
+            to[u] = __shfl_sync(0xffffffffu, dst, (e0 + u) & 31);
+            if (e0 + u < here && from[u] != to[u] && col < cols) x[u] = *reinterpret_cast<const V*>(base + from[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (e0 + u < here && from[u] != to[u] && col < cols) *reinterpret_cast<V*>(base + to[u]) = x[u];
+        }
       }
     }
   }
@@ -502,8 +519,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b,
   }
   int bad = mark_slots(b, slots, n, &set) ? 0 : kSitePagedArgs;
   // One warp per entry: lanes read the path and the draft's pages side by side.
+  // The last eight warps copy refs meanwhile.
   const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+  constexpr int kCopiers = 8, kCheckers = kPlanThreads / 32 - kCopiers;
+  if (threadIdx.x >> 5 >= kCheckers) copy_and_count(b, false, (threadIdx.x >> 5) - kCheckers, kCopiers);
+  for (int i = threadIdx.x >> 5; i < n && threadIdx.x >> 5 < kCheckers; i += kCheckers) {
     const int s = slots[i];
     if ((unsigned)s >= (unsigned)b.S) continue;  // reported above
     const int64_t len = b.lengths[s], m = drafted[i];
@@ -536,7 +556,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b,
       b.start(n)[i] = kept;
     }
   }
-  copy_and_count(b, false);
   end_plan(b, bad, 0);
   if (HERE) apply_here<kAccept, true>(b, pl, slots, drafted, path, depth, n);
 }
@@ -603,8 +622,9 @@ __device__ __forceinline__ int64_t warp_find_seq(const void* offs, int is64, int
   return lo;
 }
 
-// One warp per packed row of K or V.  The rows of entry b are the last
-// offs[b+1] - offs[b] of its slot.
+// One warp per token: its K and V rows.  The rows of entry b are the last
+// offs[b+1] - offs[b] of its slot.  The first loads of the rows are under way
+// while the chain offsets -> slot -> length -> page id finds where they go.
 template <int W>
 __global__ void __launch_bounds__(kThreads)
     paged_write_kernel(const Pools pl, int layer, const char* k, int64_t k_rb, int64_t k_hb, const char* v,
@@ -612,11 +632,26 @@ __global__ void __launch_bounds__(kThreads)
                        const int32_t* slots, const int32_t* table, const int32_t* lengths, int S, int M, int P,
                        int page, int* status) {
   using V = typename Vec<W>::T;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   if (status != nullptr && *reinterpret_cast<volatile int*>(status) != 0) return;
   const int lane = threadIdx.x & 31;
-  const int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (task >= 2 * T) return;
-  const int64_t t = task >> 1;
+  const int64_t t = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (t >= T) return;
+  const unsigned vpr = (unsigned)(pl.row_bytes / W), all = vpr * (unsigned)pl.H;
+  constexpr int U = 4;
+  V x[2][U];
+  auto load = [&](unsigned i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned i = i0 + 32 * u;
+      if (i < all) {
+        x[0][u] = *reinterpret_cast<const V*>(k + t * k_rb + (i / vpr) * k_hb + (int64_t)(i % vpr) * W);
+        x[1][u] = *reinterpret_cast<const V*>(v + t * v_rb + (i / vpr) * v_hb + (int64_t)(i % vpr) * W);
+      }
+    }
+  };
+  load(lane);
   const int64_t b = warp_find_seq(offs, is64, B, t, lane);
   const int64_t lo = load_offset(offs, is64, b), hi = load_offset(offs, is64, b + 1);
   const int s = slots[b];
@@ -629,29 +664,24 @@ __global__ void __launch_bounds__(kThreads)
     if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
     return;
   }
-  const int p = table[(int64_t)s * M + pos / page];
+  const unsigned at = (unsigned)pos / (unsigned)page;
+  const int p = table[(int64_t)s * M + at];
   if ((unsigned)p >= (unsigned)P) {
     if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedTable);
     return;
   }
-  const bool is_v = task & 1;
-  const char* src = is_v ? v + t * v_rb : k + t * k_rb;
-  const int64_t hb = is_v ? v_hb : k_hb;
-  char* dst = (is_v ? pl.v : pl.k) + layer * pl.layer_bytes + p * pl.page_bytes + (pos % page) * pl.row_bytes;
+  const int64_t to = layer * pl.layer_bytes + p * pl.page_bytes + (int64_t)((unsigned)pos - at * page) * pl.row_bytes;
   const int64_t dst_hb = (int64_t)page * pl.row_bytes;
-  const unsigned vpr = (unsigned)(pl.row_bytes / W), all = vpr * (unsigned)pl.H;
-  constexpr int U = 4;
   for (unsigned i0 = lane; i0 < all; i0 += 32 * U) {
-    V x[U];
+    if (i0 != (unsigned)lane) load(i0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const unsigned i = i0 + 32 * u;
-      if (i < all) x[u] = *reinterpret_cast<const V*>(src + (i / vpr) * hb + (int64_t)(i % vpr) * W);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned i = i0 + 32 * u;
-      if (i < all) *reinterpret_cast<V*>(dst + (i / vpr) * dst_hb + (int64_t)(i % vpr) * W) = x[u];
+      if (i < all) {
+        const int64_t d = to + (i / vpr) * dst_hb + (int64_t)(i % vpr) * W;
+        *reinterpret_cast<V*>(pl.k + d) = x[0][u];
+        *reinterpret_cast<V*>(pl.v + d) = x[1][u];
+      }
     }
   }
 }
@@ -819,13 +849,13 @@ extern "C" int scree_paged_accept(const scree_paged_book* book, const scree_page
   const Book b = make_book(book, workspace);
   cudaStream_t s = (cudaStream_t)stream;
   const int w = pick_width(pl.row_bytes, {(uintptr_t)pl.k, (uintptr_t)pl.v});
-  const int64_t threads = depth == 0 ? 0 : n * pl.L * 2 * pl.H * (pl.row_bytes / w);
-  const bool here = apply_by_plan(b, (threads + 31) / 32, w);
+  const int64_t units = depth == 0 ? 0 : n * pl.L * 2 * ((pl.H * (pl.row_bytes / w) + 31) / 32);
+  const bool here = apply_by_plan(b, units, w);
   SCREE_CUDA_TRY(launch_dependent(here ? plan_accept_kernel<true> : plan_accept_kernel<false>, dim3(1),
                                   dim3(kPlanThreads), 0, s, 1, b, pl, slots, drafted, path, (int)depth, (int)n));
   count_launch();
   if (here) return SCREE_OK;
-  return launch_apply<kAccept>(b, pl, slots, drafted, path, (int)depth, (int)n, (threads + 31) / 32, s);
+  return launch_apply<kAccept>(b, pl, slots, drafted, path, (int)depth, (int)n, units, s);
 }
 
 extern "C" int scree_paged_fork(const scree_paged_book* book, const scree_paged_pools* pools,
@@ -901,13 +931,13 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
   const int w = pick_width(pl.row_bytes, {(uintptr_t)pl.k, (uintptr_t)pl.v, (uintptr_t)k, (uintptr_t)v,
                                           (uintptr_t)k_row_bytes, (uintptr_t)k_head_bytes,
                                           (uintptr_t)v_row_bytes, (uintptr_t)v_head_bytes});
-  const unsigned grid = (unsigned)((2 * T + kThreads / 32 - 1) / (kThreads / 32));
+  const unsigned grid = (unsigned)((T + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t s = (cudaStream_t)stream;
 #define SCREE_WRITE(WW)                                                                                   \
-  paged_write_kernel<WW><<<grid, kThreads, 0, s>>>(                                                       \
-      pl, (int)layer, (const char*)k, k_row_bytes, k_head_bytes, (const char*)v, v_row_bytes,             \
-      v_head_bytes, offsets, offs_is_i64, B, T, slots, table, lengths, (int)S, (int)M, (int)P, (int)page, \
-      device_status_ptr())
+  SCREE_CUDA_TRY(launch_dependent(                                                                        \
+      paged_write_kernel<WW>, dim3(grid), dim3(kThreads), 0, s, 1, pl, (int)layer, (const char*)k,        \
+      k_row_bytes, k_head_bytes, (const char*)v, v_row_bytes, v_head_bytes, offsets, offs_is_i64, B, T,   \
+      slots, table, lengths, (int)S, (int)M, (int)P, (int)page, device_status_ptr()))
   switch (w) {
     case 16: SCREE_WRITE(16); break;
     case 8: SCREE_WRITE(8); break;
@@ -916,7 +946,7 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
     default: SCREE_WRITE(1); break;
   }
 #undef SCREE_WRITE
-  SCREE_LAUNCH_CHECK();
+  count_launch();
   return SCREE_OK;
 }
 
