@@ -3,7 +3,8 @@
 //
 // The rows that share a K/V head (new token t, query head g of the group: row
 // t G + g) are cut into tiles of 128 rows of whole tokens; a segment is a
-// (sequence, K/V head, pair of tiles A and B), its units are tiles of 128 keys.
+// (sequence, K/V head, pair of tiles A and B), its units are tiles of 128 keys
+// (and kLead more).
 // As in attn_paged.cu all units laid end to end are cut into equal runs, one per
 // CTA (one CTA per SM), and pieces of split segments are joined by a second
 // kernel.  A and B share every K/V tile in shared memory, and the tensor core
@@ -86,12 +87,15 @@ __device__ __forceinline__ int64_t seg_tiles(const PagedParams& p, int64_t n, in
   const int64_t keys = p.mask != nullptr ? len : len - n + min(n, (rt + 1) * tok2);
   return (keys + BN - 1) / BN;
 }
+// A segment's units are kLead idle ones, which stand for what starting and storing
+// a piece costs (5 us, where a tile takes 2.3), and its tiles.
+constexpr int kLead = 4;
 // Units of one K/V head of a sequence.
 __device__ __forceinline__ int64_t head_units(const PagedParams& p, int64_t n, int64_t len, int tok2) {
   const int64_t rts = (n + tok2 - 1) / tok2;
-  if (p.mask != nullptr) return rts * ((len + BN - 1) / BN);
+  if (p.mask != nullptr) return rts * (kLead + (len + BN - 1) / BN);
   int64_t u = 0;
-  for (int64_t r = 0; r < rts; ++r) u += seg_tiles(p, n, len, r, tok2);
+  for (int64_t r = 0; r < rts; ++r) u += kLead + seg_tiles(p, n, len, r, tok2);
   return u;
 }
 
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (k >= kRing && !(ok = __all_sync(0xffffffffu, wait(&rec_empty[slot], k / kRing - 1)))) break;
       Rec e;
       e.t0 = -1;
-      if (u < u1) {
+      while (u < u1) {
         int64_t q0 = 0, n = 0, len = 0, hu = 0;
         while (true) {  // the sequence of unit u (those after the run's first, in turn)
           q0 = load_offset(p.offs, p.is64, b);
@@ -238,26 +242,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         int64_t s0 = pre_b + e.h * hu, rt = 0, tiles;
         if (p.mask != nullptr) {
           tiles = seg_tiles(p, n, len, 0, tok2);
-          rt = (u - s0) / tiles;
-          s0 += rt * tiles;
+          rt = (u - s0) / (kLead + tiles);
+          s0 += rt * (kLead + tiles);
         } else {
-          while (u >= s0 + (tiles = seg_tiles(p, n, len, rt, tok2))) {
-            s0 += tiles;
+          while (u >= s0 + kLead + (tiles = seg_tiles(p, n, len, rt, tok2))) {
+            s0 += kLead + tiles;
             ++rt;
           }
         }
-        const int64_t s1 = s0 + tiles, end = min(u1, s1);
+        s0 += kLead;  // the unit of tile 0
+        const int64_t s1 = s0 + tiles, from = max(u, s0), end = min(u1, s1);
+        const bool start = u == u0;
+        u = max(end, from);
+        if (start && lane == 0) p.desc[w] = PagedDesc{s0, s1, b, e.h, (int)rt, u0 > s0 ? 1 : 0};
+        if (end <= s0) continue;  // the run ends in the segment's lead
         e.i0 = (int)rt * tok2;
         e.row0 = (int)q0 + e.i0;
         e.ntok = (int)n - e.i0;
         e.c0 = (int)(len - n);
         e.len = (int)len;
-        e.t0 = (int)(u - s0);
+        e.t0 = (int)(from - s0);
         e.t1 = (int)(end - s0);
-        e.part = u == s0 && end == s1 ? -1 : (int)(2 * w + (u == u0 ? 0 : 1));
+        // A run has at most one piece that continues a segment and one that leaves one.
+        e.part = from == s0 && end == s1 ? -1 : (int)(2 * w + (from > s0 ? 0 : 1));
         e.special = 0;
-        if (u == u0 && lane == 0) p.desc[w] = PagedDesc{s0, s1, b, e.h, (int)rt, u > s0 ? 1 : 0};
-        u = end;
+        break;
       }
       if (lane == 0) {
         ring[slot] = e;
@@ -615,15 +624,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
   const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
   const int i = d.rt * 2 * tpt + x * tpt + tok;  // new token of the sequence
   if (r >= tpt * p.G || i >= n) return;
-  const int64_t first = 2 * w0 + (worker_start(w0, U, N) == d.s0 ? 0 : 1);
-  auto part_of = [&](int j) { return (j == 0 ? first : 2 * (w0 + j)) * 2 + x; };
+  auto part_of = [&](int j) { return (j == 0 ? 2 * w0 + 1 : 2 * (w0 + j)) * 2 + x; };
   constexpr int E = D / 4 / kJoinWarps;  // float4 of a warp
-  constexpr int J = 4;                   // pieces loaded side by side
+  constexpr int J = 2;                   // pieces loaded side by side
   float mx = -INFINITY, sum = 0.f;
   float4 acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
   const float4* po = reinterpret_cast<const float4*>(p.part_o);
+#pragma unroll 1
   for (int j0 = 0; j0 < np; j0 += J) {
     float2 ml[J];
     float4 v[J][E];
@@ -634,7 +643,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
 #pragma unroll
       for (int e = 0; e < E; ++e) v[j][e] = po[(part * (D / 4) + warp * E + e) * BM + r];
     }
-    const float m2 = fmaxf(mx, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    const float m2 = fmaxf(mx, fmaxf(ml[0].x, ml[1].x));
     const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_approx(mx - ref);
     mx = m2;
     sum *= scale;
