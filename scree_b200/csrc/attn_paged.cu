@@ -4,8 +4,8 @@
 //   S = Q K^T scale over the visible keys, P = softmax(S), O = P V, LSE = m + ln l
 //
 // The rows that share a K/V head (token i, query head h * G + g -> row i G + g)
-// form row tiles of R rows; a (sequence, K/V head, row tile) is a segment of
-// ceil(len / 16) groups of 16 keys.  All segments laid end to end are cut into
+// form row tiles of R rows; a (sequence, K/V head, row tile) is a segment, its
+// units groups of KEYS keys (and kLead more).  All segments laid end to end are cut into
 // equal runs of groups, one run per worker, so the cache is read evenly by the
 // whole GPU whatever the lengths are: a long sequence is spread over many
 // workers, short ones share a worker.  A worker is one warp with a ring of
@@ -15,8 +15,11 @@
 // (m, l, O) and a second kernel joins them.
 //
 // Bound: HBM, 4 D bytes per key and K/V head (R <= 32 rows of mma.sync work per
-// key hide under that).  A group is 16 keys because that is the contraction of
-// one mma and pages hold multiples of it, so a group never spans pages.
+// key hide under that).  A group is as many keys as make 8 KB of K and V: the
+// chain scores -> maximum -> exponentials -> product takes a warp about 1,000
+// cycles whatever the number of keys, and with 16 keys at D = 64 that, not HBM,
+// set the pace (2 x 131071 keys: 28 us against XXLONG).  It is loaded in boxes of 16
+// keys, which never span pages.
 #include <algorithm>
 #include "attn_paged.cuh"
 
@@ -25,15 +28,20 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kKeys = kPagedKeys;    // keys of a group
+constexpr int kBox = kPagedKeys;     // keys of a box
+// A segment's units are kLead idle ones, which stand for what starting a piece
+// costs a worker, and its groups.
+constexpr int kLead = 1;
 
 template <int D> struct Cfg {
+  static constexpr int GP = 128 / D;               // boxes of a group
+  static constexpr int KEYS = GP * kBox;
   static constexpr int ROWB = D >= 64 ? 128 : 64;  // bytes of a box row (= swizzle span)
   static constexpr int NB = D * 2 / ROWB;          // boxes across D
-  static constexpr int BOX = kKeys * ROWB;
-  static constexpr int PART = NB * BOX;            // K (or V) of a group
-  static constexpr int STAGE = 2 * PART;
-  static constexpr int STAGES = 3 * 128 / D;       // 24 KB in flight per warp, 192 KB per SM
+  static constexpr int BOX = kBox * ROWB;
+  static constexpr int PART = GP * NB * BOX;       // K (or V) of a group
+  static constexpr int STAGE = 2 * PART;           // 8 KB
+  static constexpr int STAGES = 3;                 // 24 KB in flight per warp, 192 KB per SM
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int smem(int64_t B) {
     return 1024 + RING + kWarps * STAGES * 8 + 64 + (int)(B + 1) * 8;
@@ -87,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Units before each sequence, by every CTA for itself (a launch of its own
   // would cost more than these few loads).
   if (!paged_prefix<kWarps>(p, pre, [&](int64_t n, int64_t len) {
-        return (n * p.G + R - 1) / R * ((len + kKeys - 1) / kKeys) * p.Hkv;
+        return (int64_t)((unsigned)(n * p.G + R - 1) / R) * (kLead + (unsigned)(len + C::KEYS - 1) / C::KEYS) * p.Hkv;
       }))
     return;
   const int64_t U = pre[p.B];  // > 0: T = 0 does not launch, and a new token is a key
@@ -96,7 +104,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Neighbouring runs go to different SMs, so few workers are spread out too.
   const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
   if (w >= N) return;
-  const int64_t u0 = worker_start(w, U, N), u1 = worker_start(w + 1, U, N);
+  const PagedCut cut(U, N);
+  const int64_t u0 = cut.start(w), u1 = cut.start(w + 1);
 
   struct Seg {
     int b, h, rt, slot, len;
@@ -108,12 +117,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     g.b = lo;
     g.slot = p.slots[lo];
     g.len = p.lengths[g.slot];
-    const int64_t groups = (g.len + kKeys - 1) / kKeys;
-    const int64_t at = (u - pre[lo]) / groups;             // segment within the sequence
-    const int64_t rts = (pre[lo + 1] - pre[lo]) / groups / p.Hkv;  // row tiles
-    g.h = (int)(at / rts);
-    g.rt = (int)(at % rts);
-    g.s0 = pre[lo] + at * groups;
+    const unsigned groups = (unsigned)(g.len + C::KEYS - 1) / C::KEYS, seg = kLead + groups;
+    const int64_t at = udiv(u - pre[lo], seg);  // segment within the sequence
+    const unsigned rts = (unsigned)udiv(pre[lo + 1] - pre[lo], seg) / (unsigned)p.Hkv;  // row tiles
+    g.h = (int)((unsigned)at / rts);
+    g.rt = (int)((unsigned)at - g.h * rts);
+    g.s0 = pre[lo] + at * seg + kLead;  // the unit of group 0
     g.s1 = g.s0 + groups;
     return g;
   };
@@ -122,36 +131,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t ring_s = smem_u32(ring);
   uint64_t* full = bars + warp * C::STAGES;
 
-  // Loads run ahead of the work, across segments.  The page ids of 32 groups
-  // at a time sit in the lanes.
+  // Loads run ahead of the work, across segments.  The page ids of 32 boxes at a
+  // time sit in the lanes (past the end those of the last box: its keys are masked
+  // and its V is taken out).
   int64_t ui = u0;
   Seg gi = find(u0);
   int64_t win = -1;  // first unit of the window of page ids
   int my_page = 0;
   int ist = 0;
   auto issue = [&]() {
-    if (ui >= u1) return;
-    if (ui >= gi.s1) {
+    if (ui >= gi.s1 && ui < u1) {
       gi = find(ui);
       win = -1;
     }
-    if (win < 0 || ui >= win + 32) {
+    ui = max(ui, gi.s0);  // past the segment's lead
+    if (ui >= u1) return;
+    const int last = (gi.len - 1) / kBox;
+    if (win < 0 || ui >= win + 32 / C::GP) {
       win = ui;
-      const int64_t g = ui - gi.s0 + lane;
-      my_page = 0;
-      if (g < gi.s1 - gi.s0) my_page = paged_page(p, gi.slot, g);
+      my_page = paged_page(p, gi.slot, min((int)(ui - gi.s0) * C::GP + lane, last));
     }
-    const int page = __shfl_sync(0xffffffffu, my_page, (int)(ui - win));
+    int page[C::GP];
+#pragma unroll
+    for (int q = 0; q < C::GP; ++q)
+      page[q] = __shfl_sync(0xffffffffu, my_page, (int)(ui - win) * C::GP + q);
     if (lane == 0) {
-      const int in_page = (int)((ui - gi.s0) * kKeys % p.page);
-      const int row = (int)(p.layer_row + ((int64_t)page * p.Hkv + gi.h) * p.page + in_page);
       uint8_t* st = ring + ist * C::STAGE;
       mbar_expect_tx(&full[ist], C::STAGE);
 #pragma unroll
-      for (int c = 0; c < C::NB; ++c) tma_load_2d(st + c * C::BOX, &tm_k, &full[ist], c * (C::ROWB / 2), row);
+      for (int q = 0; q < C::GP; ++q) {
+        const unsigned box = (unsigned)min((int)(ui - gi.s0) * C::GP + q, last);
+        const int row = (int)(p.layer_row + ((int64_t)page[q] * p.Hkv + gi.h) * p.page + box * kBox % (unsigned)p.page);
 #pragma unroll
-      for (int c = 0; c < C::NB; ++c)
-        tma_load_2d(st + C::PART + c * C::BOX, &tm_v, &full[ist], c * (C::ROWB / 2), row);
+        for (int c = 0; c < C::NB; ++c) {
+          uint8_t* at = st + (q * C::NB + c) * C::BOX;
+          tma_load_2d(at, &tm_k, &full[ist], c * (C::ROWB / 2), row);
+          tma_load_2d(at + C::PART, &tm_v, &full[ist], c * (C::ROWB / 2), row);
+        }
+      }
     }
     ist = ist + 1 == C::STAGES ? 0 : ist + 1;
     ++ui;
@@ -159,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
   for (int i = 0; i < C::STAGES; ++i) issue();
 
-  // Byte offset of 16-byte chunk c of key k in a part (TMA's swizzle).
+  // Byte offset of 16-byte chunk c of key k of a box (TMA's swizzle).
   auto chunk = [](int k, int c) -> uint32_t {
     constexpr int CPR = C::ROWB / 16;
     const int sw = C::ROWB == 128 ? (k & 7) : ((k >> 1) & 3);
@@ -175,6 +192,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   for (int64_t u = u0; ok && u < u1;) {
     const Seg g = find(u);
+    if (u == u0 && lane == 0) p.desc[w] = PagedDesc{g.s0, g.s1, g.b, g.h, g.rt, u0 > g.s0 ? 1 : 0};
+    u = max(u, g.s0);
+    if (u >= u1) break;  // the run ends in a segment's lead
     const int64_t begin = u, end = min(u1, g.s1);
     const int64_t q0 = load_offset(p.offs, p.is64, g.b);
     const int n = (int)(load_offset(p.offs, p.is64, g.b + 1) - q0);
@@ -216,35 +236,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const uint32_t ks = ring_s + cst * C::STAGE, vs = ks + C::PART;
-      float s[MT][2][4];
+      constexpr int NT = 2 * C::GP;  // 8-key tiles of the scores
+      float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[mt][t][e] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        uint32_t kf[4];
-        ldsm_x4(ks + chunk(k_key, kk * 2 + k_c), kf);
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16816<T>(s[mt][0], qf[mt][kk], kf[0], kf[1]);
-          mma16816<T>(s[mt][1], qf[mt][kk], kf[2], kf[3]);
+        for (int q = 0; q < C::GP; ++q) {
+          uint32_t kf[4];
+          ldsm_x4(ks + q * C::NB * C::BOX + chunk(k_key, kk * 2 + k_c), kf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(s[mt][2 * q], qf[mt][kk], kf[0], kf[1]);
+            mma16816<T>(s[mt][2 * q + 1], qf[mt][kk], kf[2], kf[3]);
+          }
         }
-      }
-      const int k0 = (int)(u - g.s0) * kKeys;
-      const bool edge = k0 + kKeys > c0;  // holds new tokens, or runs past the end
-      uint32_t vis[MT][2];
+      const int k0 = (int)(u - g.s0) * C::KEYS;
+      const bool edge = k0 + C::KEYS > c0;  // holds new tokens, or runs past the end
+      unsigned long long vis[MT][2];
       if (edge) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int row = row_of(mt, r), i = row < rows ? (g.rt * R + row) / p.G : 0;
-            vis[mt][r] = (uint32_t)paged_visible<16>(p, q0 + i, i, k0, c0, g.len);
+            vis[mt][r] = paged_visible<C::KEYS>(p, q0 + i, i, k0, c0, g.len);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
               for (int e = 0; e < 2; ++e)
                 if (!(vis[mt][r] >> (t * 8 + qc + e) & 1)) s[mt][t][r * 2 + e] = -INFINITY;
@@ -257,7 +280,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float mx = fmaxf(fmaxf(s[mt][0][r * 2], s[mt][0][r * 2 + 1]), fmaxf(s[mt][1][r * 2], s[mt][1][r * 2 + 1]));
+          float mx = fmaxf(s[mt][0][r * 2], s[mt][0][r * 2 + 1]);
+#pragma unroll
+          for (int t = 1; t < NT; ++t) mx = fmax3(mx, s[mt][t][r * 2], s[mt][t][r * 2 + 1]);
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float mc = mx * p.sl2;
@@ -279,31 +304,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[mt][e >> 1];
         }
       }
-      uint32_t pf[MT][4];
+      uint32_t pf[MT][C::GP][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float mm = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < NT; ++t) {
             const float e0 = ex2_approx(fmaf(s[mt][t][r * 2], p.sl2, -mm));
             const float e1 = ex2_approx(fmaf(s[mt][t][r * 2 + 1], p.sl2, -mm));
             l[mt][r] += e0 + e1;
-            pf[mt][t * 2 + r] = pack2<T>(e0, e1);
+            pf[mt][t >> 1][(t & 1) * 2 + r] = pack2<T>(e0, e1);
           }
         }
       if (!edge) {
 #pragma unroll
-        for (int j = 0; j < KK; ++j) {
-          uint32_t vf[4];
-          ldsm_x4_t(vs + chunk(v_key, j * 2 + v_c), vf);
+        for (int q = 0; q < C::GP; ++q)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<T>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
-            mma16816<T>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+          for (int j = 0; j < KK; ++j) {
+            uint32_t vf[4];
+            ldsm_x4_t(vs + q * C::NB * C::BOX + chunk(v_key, j * 2 + v_c), vf);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<T>(o[mt][2 * j], pf[mt][q], vf[0], vf[1]);
+              mma16816<T>(o[mt][2 * j + 1], pf[mt][q], vf[2], vf[3]);
+            }
           }
-        }
       } else {
         // A key that a row does not see must not reach it even if its V is an
         // infinity or NaN (0 * NaN): such elements, and the rows past the end of
@@ -311,33 +338,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         // then added for the rows that do see them.
         const int left = g.len - k0;
         auto live = [&](int k) { return (k < left ? 0xFFFFu : 0u) | (k + 1 < left ? 0xFFFF0000u : 0u); };
-        const uint32_t live_lo = live(qc), live_hi = live(qc + 8);
         bool special = false;
 #pragma unroll
-        for (int j = 0; j < KK; ++j) {
-          uint32_t vf[4];
-          ldsm_x4_t(vs + chunk(v_key, j * 2 + v_c), vf);
+        for (int q = 0; q < C::GP; ++q) {
+          const uint32_t live_lo = live(q * kBox + qc), live_hi = live(q * kBox + qc + 8);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            vf[e] &= (e & 1) ? live_hi : live_lo;
-            const uint32_t nf = nonfinite_halves<T>(vf[e]);
-            special |= nf != 0;
-            vf[e] &= ~nf;
-          }
+          for (int j = 0; j < KK; ++j) {
+            uint32_t vf[4];
+            ldsm_x4_t(vs + q * C::NB * C::BOX + chunk(v_key, j * 2 + v_c), vf);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<T>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
-            mma16816<T>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+            for (int e = 0; e < 4; ++e) {
+              vf[e] &= (e & 1) ? live_hi : live_lo;
+              const uint32_t nf = nonfinite_halves<T>(vf[e]);
+              special |= nf != 0;
+              vf[e] &= ~nf;
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16816<T>(o[mt][2 * j], pf[mt][q], vf[0], vf[1]);
+              mma16816<T>(o[mt][2 * j + 1], pf[mt][q], vf[2], vf[3]);
+            }
           }
         }
         if (__any_sync(0xffffffffu, special)) {
 #pragma unroll 1
-          for (int k = 0; k < min(left, kKeys); ++k) {
+          for (int k = 0; k < min(left, C::KEYS); ++k) {
 #pragma unroll
             for (int j = 0; j < 2 * KK; ++j)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const uint8_t* at = ring + cst * C::STAGE + C::PART + chunk(k, j) + (qc + e) * 2;
+                const uint8_t* at =
+                    ring + cst * C::STAGE + C::PART + k / kBox * C::NB * C::BOX + chunk(k % kBox, j) + (qc + e) * 2;
                 const uint16_t h = *reinterpret_cast<const uint16_t*>(at);
                 if (nonfinite_halves<T>(h) & 0xFFFFu) {
                   const float x = Cvt<T>::to_f(*reinterpret_cast<const T*>(&h));
@@ -359,7 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) break;
     // ---------------------------------------------------------------- piece done
     const bool whole = begin == g.s0 && end == g.s1;
-    const int64_t slot = 2 * w + (begin == u0 ? 0 : 1);
+    // A run has at most one piece that continues a segment and one that leaves one.
+    const int64_t slot = 2 * w + (begin > g.s0 ? 0 : 1);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -388,7 +420,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((lane & 3) == 0) p.part_ml[slot * R + row] = make_float2(m[mt][r], sum);
         }
       }
-    if (begin == u0 && lane == 0) p.desc[w] = PagedDesc{g.s0, g.s1, g.b, g.h, g.rt, begin > g.s0 ? 1 : 0};
   }
 }
 
@@ -409,16 +440,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   const int64_t c = (int64_t)blockIdx.x + 1;
   const PagedHead hd = *p.head;
   const PagedDesc d = p.desc[c];  // garbage past the last worker, not used then
-  const int64_t U = hd.U, N = hd.N;
+  const int64_t N = hd.N;
   if (c >= N || !d.on) return;
-  const int64_t w0 = worker_of(d.s0, U, N);
-  const int np = (int)(worker_of(d.s1 - 1, U, N) - w0) + 1;
+  const PagedCut cut(hd.U, N);
+  const int64_t w0 = cut.of(d.s0);
+  const int np = (int)(cut.of(d.s1 - 1) - w0) + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t q0 = load_offset(p.offs, p.is64, d.b);
   const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
   const int rows = min(R, n * p.G - d.rt * R);
-  const int64_t first = 2 * w0 + (worker_start(w0, U, N) == d.s0 ? 0 : 1);
-  auto slot_of = [&](int i) { return i == 0 ? first : 2 * (w0 + i); };
+  auto slot_of = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
   const int share = np >= kManyPieces ? kJoinWarps : 1;  // warps of one row
   const int sub = warp % share;
   const int step = (np - 1) * (kJoinWarps / share);
@@ -594,10 +625,10 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   }
   SCREE_CHECK_ARG(pools->row_bytes == 2 * D, "attn_fwd_paged: pool rows of %lld bytes for head_dim %d",
                   (long long)pools->row_bytes, D);
-  SCREE_CHECK_ARG(S >= 1 && M >= 1 && P >= 1 && P < (1ll << 30) && page >= kKeys && page % kKeys == 0 &&
+  SCREE_CHECK_ARG(S >= 1 && M >= 1 && P >= 1 && P < (1ll << 30) && page >= kBox && page % kBox == 0 &&
                       M * page < (1ll << 31),
                   "attn_fwd_paged: bad cache sizes S=%lld M=%lld P=%lld page=%lld (a multiple of %d)",
-                  (long long)S, (long long)M, (long long)P, (long long)page, kKeys);
+                  (long long)S, (long long)M, (long long)P, (long long)page, kBox);
   SCREE_CHECK_ARG(layer >= 0 && layer < pools->L, "attn_fwd_paged: layer %lld of %lld", (long long)layer,
                   (long long)pools->L);
   const int64_t pool_rows = pools->L * P * H_kv * page;
@@ -648,8 +679,8 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   if (R == 0) return attn_paged_tc(p, pools->k, pools->v, pool_rows, D, bf16, workspace, s);
   CUtensorMap tk, tv;
   int rc;
-  if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, kKeys, bf16))) return rc;
-  if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, kKeys, bf16))) return rc;
+  if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, kBox, bf16))) return rc;
+  if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, kBox, bf16))) return rc;
   char* w = (char*)workspace;
   const int64_t N = max_workers();
   p.head = (PagedHead*)w;

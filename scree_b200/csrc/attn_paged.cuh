@@ -41,11 +41,25 @@ struct PagedParams {
   float* part_o;
 };
 
-// Units [start(w), start(w + 1)) are worker w's; the worker that holds unit u.
-__device__ __forceinline__ int64_t worker_start(int64_t w, int64_t U, int64_t N) { return w * U / N; }
-__device__ __forceinline__ int64_t worker_of(int64_t u, int64_t U, int64_t N) {
-  return ((u + 1) * N - 1) / U;
+// Division of non-negative numbers, in 32 bits where they fit (a 64-bit division
+// takes several hundred cycles, and a worker's start needs half a dozen).
+__device__ __forceinline__ int64_t udiv(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+  return a / b;
 }
+// Units [start(w), start(w + 1)) are worker w's: U / N each, one more for the first
+// U % N; the worker that holds unit u.
+struct PagedCut {
+  int64_t q, r;
+  __device__ __forceinline__ PagedCut(int64_t U, int64_t N) {
+    q = udiv(U, N);
+    r = U - q * N;
+  }
+  __device__ __forceinline__ int64_t start(int64_t w) const { return w * q + min(w, r); }
+  __device__ __forceinline__ int64_t of(int64_t u) const {
+    return u < r * (q + 1) ? udiv(u, q + 1) : r + udiv(u - r * (q + 1), q);
+  }
+};
 
 // Fills pre[b] = units of the sequences before b (units(n, len) of each), by the
 // whole block of 32 * WARPS threads; false for every thread if the call is to be
@@ -119,8 +133,8 @@ __device__ __forceinline__ bool paged_wait(const PagedParams& p, uint64_t* bar, 
 }
 
 // Page that holds key group g (16 keys) of a slot; a bad id is recorded and read as page 0.
-__device__ __forceinline__ int paged_page(const PagedParams& p, int slot, int64_t g) {
-  const int page = p.table[(int64_t)slot * p.M + g * kPagedKeys / p.page];
+__device__ __forceinline__ int paged_page(const PagedParams& p, int slot, int g) {
+  const int page = p.table[(int64_t)slot * p.M + (unsigned)g * kPagedKeys / (unsigned)p.page];
   if ((unsigned)page < (unsigned)p.P) return page;
   record_device_error(p.status, SCREE_DEVERR_BAD_INPUT, kSitePagedAttnPage);
   return 0;

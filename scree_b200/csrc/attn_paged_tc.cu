@@ -85,15 +85,15 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
 // Key tiles of the rt-th row tile pair: up to its last row's last visible key.
 __device__ __forceinline__ int64_t seg_tiles(const PagedParams& p, int64_t n, int64_t len, int64_t rt, int tok2) {
   const int64_t keys = p.mask != nullptr ? len : len - n + min(n, (rt + 1) * tok2);
-  return (keys + BN - 1) / BN;
+  return (unsigned)(keys + BN - 1) / BN;
 }
 // A segment's units are kLead idle ones, which stand for what starting and storing
 // a piece costs (5 us, where a tile takes 2.3), and its tiles.
 constexpr int kLead = 4;
 // Units of one K/V head of a sequence.
 __device__ __forceinline__ int64_t head_units(const PagedParams& p, int64_t n, int64_t len, int tok2) {
-  const int64_t rts = (n + tok2 - 1) / tok2;
-  if (p.mask != nullptr) return rts * (kLead + (len + BN - 1) / BN);
+  const int64_t rts = (unsigned)(n + tok2 - 1) / (unsigned)tok2;
+  if (p.mask != nullptr) return rts * (kLead + (unsigned)(len + BN - 1) / BN);
   int64_t u = 0;
   for (int64_t r = 0; r < rts; ++r) u += kLead + seg_tiles(p, n, len, r, tok2);
   return u;
@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t U = pre[p.B], N = min((int64_t)gridDim.x, U), w = blockIdx.x;
   if (w == 0 && threadIdx.x == 0) *p.head = PagedHead{U, N};
   if (w >= N) return;
-  const int64_t u0 = worker_start(w, U, N), u1 = worker_start(w + 1, U, N);
+  const PagedCut cut(U, N);
+  const int64_t u0 = cut.start(w), u1 = cut.start(w + 1);
   const int b_first = paged_find(pre, p.B, u0);
   const int64_t pre_first = pre[b_first];
   __syncthreads();  // the prefix has been read: its memory becomes the Q buffer
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (c < C::NCHUNK) {
       const int last = (e.len - 1) / kPagedKeys;
       const int g = min(t * kLanesPerTile + b * per, last / per * per);
-      const int row = (int)(p.layer_row + ((int64_t)page * p.Hkv + e.h) * p.page + (int64_t)g * kPagedKeys % p.page);
+      const int row = (int)(p.layer_row + ((int64_t)page * p.Hkv + e.h) * p.page + (unsigned)g * kPagedKeys % (unsigned)p.page);
       tma_load_2d(dst + c * BN * C::SWB + b * box * C::SWB, map, bar, c * C::CHUNK, row);
     }
   };
@@ -238,11 +239,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           pre_b += hu * p.Hkv;
           ++b;
         }
-        e.h = (int)((u - pre_b) / hu);
+        e.h = (int)udiv(u - pre_b, hu);
         int64_t s0 = pre_b + e.h * hu, rt = 0, tiles;
         if (p.mask != nullptr) {
           tiles = seg_tiles(p, n, len, 0, tok2);
-          rt = (u - s0) / (kLead + tiles);
+          rt = udiv(u - s0, kLead + tiles);
           s0 += rt * (kLead + tiles);
         } else {
           while (u >= s0 + kLead + (tiles = seg_tiles(p, n, len, rt, tok2))) {
@@ -611,11 +612,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
   const int64_t c = (int64_t)blockIdx.x + 1;
   const PagedHead hd = *p.head;
   const PagedDesc d = p.desc[c];
-  const int64_t U = hd.U, N = hd.N;
+  const int64_t N = hd.N;
   if (c >= N || !d.on) return;
-  const int64_t w0 = worker_of(d.s0, U, N);
+  const PagedCut cut(hd.U, N);
+  const int64_t w0 = cut.of(d.s0);
   if (w0 != c - 1) return;
-  const int np = (int)(worker_of(d.s1 - 1, U, N) - w0) + 1;
+  const int np = (int)(cut.of(d.s1 - 1) - w0) + 1;
   const int tpt = BM / p.G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int x = blockIdx.y >> 2, r = (blockIdx.y & 3) * 32 + lane;
