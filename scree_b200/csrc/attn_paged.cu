@@ -100,10 +100,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   const int64_t U = pre[p.B];  // > 0: T = 0 does not launch, and a new token is a key
   const int64_t N = min((int64_t)gridDim.x * kWarps, U);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.head = PagedHead{U, N};
   // Neighbouring runs go to different SMs, so few workers are spread out too.
   const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
-  if (w >= N) return;
+  if (w >= N) {
+    if (lane == 0) p.desc[w].on = 0;
+    return;
+  }
   const PagedCut cut(U, N);
   const int64_t u0 = cut.start(w), u1 = cut.start(w + 1);
 
@@ -192,12 +194,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   for (int64_t u = u0; ok && u < u1;) {
     const Seg g = find(u);
-    if (u == u0 && lane == 0) p.desc[w] = PagedDesc{g.s0, g.s1, g.b, g.h, g.rt, u0 > g.s0 ? 1 : 0};
+    const bool run_start = u == u0;
     u = max(u, g.s0);
-    if (u >= u1) break;  // the run ends in a segment's lead
     const int64_t begin = u, end = min(u1, g.s1);
     const int64_t q0 = load_offset(p.offs, p.is64, g.b);
     const int n = (int)(load_offset(p.offs, p.is64, g.b + 1) - q0);
+    if (run_start && lane == 0) {
+      const int w0 = (int)cut.of(g.s0);
+      p.desc[w] = PagedDesc{u0 > g.s0 ? 1 : 0, w0, (int)cut.of(g.s1 - 1) - w0 + 1, (int)q0, g.h, g.rt * R, n};
+    }
+    if (u >= u1) break;  // the run ends in a segment's lead
     const int c0 = g.len - n;
     const int rows = min(R, n * p.G - g.rt * R);
     // Rows of this lane: tile mt, half r -> row mt * 16 + r * 8 + qr of the tile.
@@ -432,30 +438,23 @@ constexpr int kJoinWarps = 8;
 constexpr int64_t kManyPieces = 16;
 template <int D, typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedParams p, int R) {
-  constexpr int E = D / 32;  // columns of a lane
+  constexpr int E = D / 32;         // columns of a lane
+  constexpr int kLoads = E == 4 ? 8 : 16;  // O rows under way at a time
   __shared__ float sm_o[kJoinWarps][D];
   __shared__ float2 sm_ml[kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const int64_t c = (int64_t)blockIdx.x + 1;
-  const PagedHead hd = *p.head;
-  const PagedDesc d = p.desc[c];  // garbage past the last worker, not used then
-  const int64_t N = hd.N;
-  if (c >= N || !d.on) return;
-  const PagedCut cut(hd.U, N);
-  const int64_t w0 = cut.of(d.s0);
-  const int np = (int)(cut.of(d.s1 - 1) - w0) + 1;
+  const PagedDesc d = p.desc[blockIdx.x + 1];
+  if (!d.on) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t q0 = load_offset(p.offs, p.is64, d.b);
-  const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
-  const int rows = min(R, n * p.G - d.rt * R);
-  auto slot_of = [&](int i) { return i == 0 ? 2 * w0 + 1 : 2 * (w0 + i); };
+  const int np = d.np, rows = min(R, d.n * p.G - d.i0), nth = (int)blockIdx.x - d.w0;
+  auto slot_of = [&](int i) { return (int64_t)(i == 0 ? 2 * d.w0 + 1 : 2 * (d.w0 + i)); };
   const int share = np >= kManyPieces ? kJoinWarps : 1;  // warps of one row
   const int sub = warp % share;
   const int step = (np - 1) * (kJoinWarps / share);
-  for (int row = (int)(c - w0 - 1) * (kJoinWarps / share) + warp / share; row < rows; row += step) {
+  for (int row = nth * (kJoinWarps / share) + warp / share; row < rows; row += step) {
     // This warp's pieces sub, sub + share, ...: 32 at a time their (m, l) in the
-    // lanes, their O rows eight loads at a time.
+    // lanes, their O rows kLoads at a time.
     float mx = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -464,10 +463,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
       float2 ml = make_float2(-INFINITY, 0.f);
       if (mine < np) ml = p.part_ml[slot_of(mine) * R + row];
       const int here = min(32, (np - i0 + share - 1) / share);
-      float x[8][E];
+      float x[kLoads][E];
       auto load = [&](int t0) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int t = 0; t < kLoads; ++t) {
           const int i = min(i0 + (t0 + t) * share, np - 1);
           const float* src = p.part_o + (slot_of(i) * R + row) * D + lane * E;
           if constexpr (E == 4) *reinterpret_cast<float4*>(x[t]) = *reinterpret_cast<const float4*>(src);
@@ -485,10 +484,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
       sum = sum * scale + wt * ml.y;  // (a lane's own pieces)
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] *= scale;
-      for (int t0 = 0; t0 < here; t0 += 8) {
+      for (int t0 = 0; t0 < here; t0 += kLoads) {
         if (t0 > 0) load(t0);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int t = 0; t < kLoads; ++t) {
           const float f = __shfl_sync(0xffffffffu, wt, (t0 + t) & 31);
           if (t0 + t < here) {
 #pragma unroll
@@ -521,8 +520,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
         for (int e = 0; e < E; ++e) acc[e] = fmaf(f, sm_o[w][lane * E + e], acc[e]);
       }
     }
-    const int a = d.rt * R + row, hq = d.h * p.G + a % p.G;
-    const int64_t tok = q0 + a / p.G;
+    const int a = d.i0 + row, hq = d.h * p.G + a % p.G;
+    const int64_t tok = d.row0 + a / p.G;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T y[E];
 #pragma unroll
@@ -545,7 +544,7 @@ int64_t max_workers() { return (int64_t)num_sms() * kWarps; }
 size_t ws_bytes(int R, int D) {
   if (R == 0) return attn_paged_tc_workspace(D);
   const int64_t N = max_workers();
-  return 64 + (size_t)N * sizeof(PagedDesc) + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
+  return (size_t)N * sizeof(PagedDesc) / 16 * 16 + 16 + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
 }
 
 template <int D, typename T, int MT>
@@ -683,10 +682,10 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   if ((rc = make_pool_map(&tv, pools->v, pool_rows, D, kBox, bf16))) return rc;
   char* w = (char*)workspace;
   const int64_t N = max_workers();
-  p.head = (PagedHead*)w;
-  p.desc = (PagedDesc*)(w + 64);
-  p.part_ml = (float2*)(w + 64 + N * sizeof(PagedDesc));
-  p.part_o = (float*)(w + 64 + N * sizeof(PagedDesc) + 2 * N * R * 8);
+  p.desc = (PagedDesc*)w;
+  w += N * sizeof(PagedDesc) / 16 * 16 + 16;
+  p.part_ml = (float2*)w;
+  p.part_o = (float*)(w + 2 * N * R * 8);
 #define SCREE_PAGED_CASE(DD)                                                                       \
   if (D == DD) {                                                                                   \
     if (bf16)                                                                                      \

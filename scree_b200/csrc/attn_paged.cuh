@@ -9,12 +9,13 @@ constexpr int kPagedKeys = 16;      // pages hold a multiple of this many keys
 constexpr int kPagedMaxSeqs = 4096; // sequences of a call (their prefix sits in shared memory)
 constexpr int kSitePagedAttn = 70, kSitePagedAttnPage = 71, kSitePagedAttnWait = 72;
 
-struct PagedHead {  // units of work and workers of a launch
-  int64_t U, N;
-};
-struct PagedDesc {  // the segment that a worker's first piece continues
-  int64_t s0, s1;
-  int32_t b, h, rt, on;
+// What the join needs of worker c: the segment that its first piece continues
+// (on = 0: none; written for every worker of the grid).
+struct PagedDesc {
+  int32_t on;
+  int32_t w0, np;    // the segment's first worker, its pieces
+  int32_t row0;      // packed row (token) of the tile's first query
+  int32_t h, i0, n;  // K/V head; index of the tile's first row (or token), new tokens of the sequence
 };
 
 struct PagedParams {
@@ -35,7 +36,6 @@ struct PagedParams {
   int64_t o_rs, o_hs;
   float* lse;
   int* status;
-  PagedHead* head;
   PagedDesc* desc;
   float2* part_ml;
   float* part_o;

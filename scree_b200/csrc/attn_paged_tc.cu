@@ -118,8 +118,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!paged_prefix<kWarps>(p, pre, [&](int64_t n, int64_t len) { return head_units(p, n, len, tok2) * p.Hkv; }))
     return;
   const int64_t U = pre[p.B], N = min((int64_t)gridDim.x, U), w = blockIdx.x;
-  if (w == 0 && threadIdx.x == 0) *p.head = PagedHead{U, N};
-  if (w >= N) return;
+  if (w >= N) {
+    if (threadIdx.x == 0) p.desc[w].on = 0;
+    return;
+  }
   const PagedCut cut(U, N);
   const int64_t u0 = cut.start(w), u1 = cut.start(w + 1);
   const int b_first = paged_find(pre, p.B, u0);
@@ -255,7 +257,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t s1 = s0 + tiles, from = max(u, s0), end = min(u1, s1);
         const bool start = u == u0;
         u = max(end, from);
-        if (start && lane == 0) p.desc[w] = PagedDesc{s0, s1, b, e.h, (int)rt, u0 > s0 ? 1 : 0};
+        if (start && lane == 0) {
+          const int w0 = (int)cut.of(s0);
+          p.desc[w] = PagedDesc{u0 > s0 ? 1 : 0, w0, (int)cut.of(s1 - 1) - w0 + 1, (int)q0, e.h, (int)rt * tok2, (int)n};
+        }
         if (end <= s0) continue;  // the run ends in the segment's lead
         e.i0 = (int)rt * tok2;
         e.row0 = (int)q0 + e.i0;
@@ -609,24 +614,15 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(const PagedParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const int64_t c = (int64_t)blockIdx.x + 1;
-  const PagedHead hd = *p.head;
-  const PagedDesc d = p.desc[c];
-  const int64_t N = hd.N;
-  if (c >= N || !d.on) return;
-  const PagedCut cut(hd.U, N);
-  const int64_t w0 = cut.of(d.s0);
-  if (w0 != c - 1) return;
-  const int np = (int)(cut.of(d.s1 - 1) - w0) + 1;
-  const int tpt = BM / p.G;
+  const PagedDesc d = p.desc[blockIdx.x + 1];
+  if (!d.on || d.w0 != (int)blockIdx.x) return;
+  const int np = d.np, tpt = BM / p.G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int x = blockIdx.y >> 2, r = (blockIdx.y & 3) * 32 + lane;
   const int tok = r / p.G, hq = r - tok * p.G;
-  const int64_t q0 = load_offset(p.offs, p.is64, d.b);
-  const int n = (int)(load_offset(p.offs, p.is64, d.b + 1) - q0);
-  const int i = d.rt * 2 * tpt + x * tpt + tok;  // new token of the sequence
-  if (r >= tpt * p.G || i >= n) return;
-  auto part_of = [&](int j) { return (j == 0 ? 2 * w0 + 1 : 2 * (w0 + j)) * 2 + x; };
+  const int i = d.i0 + x * tpt + tok;  // new token of the sequence
+  if (r >= tpt * p.G || i >= d.n) return;
+  auto part_of = [&](int j) { return (int64_t)(j == 0 ? 2 * d.w0 + 1 : 2 * (d.w0 + j)) * 2 + x; };
   constexpr int E = D / 4 / kJoinWarps;  // float4 of a warp
   constexpr int J = 2;                   // pieces loaded side by side
   float mx = -INFINITY, sum = 0.f;
@@ -672,13 +668,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int head = d.h * p.G + hq;
-  T* orow = reinterpret_cast<T*>(p.o + (q0 + i) * p.o_rs + (int64_t)head * p.o_hs) + warp * E * 4;
+  T* orow = reinterpret_cast<T*>(p.o + ((int64_t)d.row0 + i) * p.o_rs + (int64_t)head * p.o_hs) + warp * E * 4;
 #pragma unroll
   for (int e = 0; e < E; ++e)
     *reinterpret_cast<uint2*>(orow + e * 4) = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv),
                                                          pack2<T>(acc[e].z * inv, acc[e].w * inv));
   if (warp == 0 && p.lse != nullptr)
-    p.lse[(q0 + i) * p.H + head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
+    p.lse[((int64_t)d.row0 + i) * p.H + head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994531f;
 }
 
 // Tensor map over q viewed as {D, H, T}: a box is the G heads of a K/V head of
@@ -732,7 +728,7 @@ int launch_tc(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& t
 
 size_t attn_paged_tc_workspace(int D) {
   const size_t N = (size_t)num_sms();
-  return 64 + N * sizeof(PagedDesc) + 2 * N * 2 * BM * (8 + 4 * (size_t)D);
+  return N * sizeof(PagedDesc) / 16 * 16 + 16 + 2 * N * 2 * BM * (8 + 4 * (size_t)D);
 }
 
 int attn_paged_tc(const PagedParams& in, const void* k, const void* v, int64_t pool_rows, int D, bool bf16,
@@ -740,10 +736,10 @@ int attn_paged_tc(const PagedParams& in, const void* k, const void* v, int64_t p
   PagedParams p = in;
   const size_t N = (size_t)num_sms();
   char* w = (char*)workspace;
-  p.head = (PagedHead*)w;
-  p.desc = (PagedDesc*)(w + 64);
-  p.part_ml = (float2*)(w + 64 + N * sizeof(PagedDesc));
-  p.part_o = (float*)(w + 64 + N * sizeof(PagedDesc) + 2 * N * 2 * BM * 8);
+  p.desc = (PagedDesc*)w;
+  w += N * sizeof(PagedDesc) / 16 * 16 + 16;
+  p.part_ml = (float2*)w;
+  p.part_o = (float*)(w + 2 * N * 2 * BM * 8);
   // Boxes as tall as pages allow: rows of a box are consecutive in a page.
   int box = kPagedKeys;
   while (box < BN && p.page % (2 * box) == 0) box *= 2;
