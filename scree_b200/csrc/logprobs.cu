@@ -150,12 +150,6 @@ __device__ __forceinline__ void stat_move(Stat& s, float to) {
   s.s1 *= w;
   s.m = to;
 }
-__device__ __forceinline__ Stat stat_join(Stat a, Stat b) {
-  const float m = max_nan(a.m, b.m);
-  stat_move(a, m);
-  stat_move(b, m);
-  return Stat{m, a.s1 + b.s1, a.s2 + b.s2};
-}
 __device__ __forceinline__ Stat stat_warp(Stat s) {
   float m = s.m;
 #pragma unroll
@@ -189,6 +183,7 @@ struct FwdArgs {
   int64_t row_stride, N;
   int V;
   int chunks, segs;  // chunks of a row, segments that they are dealt to (= CTAs of a cluster)
+  int seg_bits;      // segs = 1 << seg_bits
   const void* targets;
   int t64;
   int top;
@@ -267,9 +262,10 @@ struct TopList {
   unsigned long long cand[kAbove + kTies];
   uint32_t pair_v[kPairs];  // order_bits of the pair's maximum
   int pair_id[kPairs];      // chunk of the window * kThreads + thread
+  int chosen[kPairs];       // the pairs that reach the top-th largest maximum
   uint32_t bound[kThreads / 32];
-  uint32_t tau;
-  int pairs, above, ties;
+  uint32_t t2;
+  int pairs, picked, above, ties;
   int cur;  // which of best[] holds the list
 };
 
@@ -286,7 +282,8 @@ __device__ __forceinline__ int work_sum(TopList& t, int v) {
 }
 
 // Merges the window of `nch` chunks from chunk c0 on into the list.  wm: the
-// window's maxima [chunk][thread]; tm: this thread's maximum over the window.
+// window's maxima [chunk][thread]; tm: this thread's maximum over the window.  One
+// barrier a step: the rest of the row's stream waits for it.
 template <typename T>
 __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int mis, int V, const T* wm,
                                           int c0, int nch, float tm) {
@@ -295,86 +292,85 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
   auto first = [&](int q, int th, int i) { return ((c0 + q) * CV + i * kThreads + th) * VE - mis; };
   // Whether the pair has elements, and its maximum.
   auto pair_max = [&](int q) {
-    return first(q, tid, 0) < V ? order_bits(Cvt<T>::to_f(wm[q * kThreads + tid])) : 0u;
+    return q < nch && first(q, tid, 0) < V ? order_bits(Cvt<T>::to_f(wm[q * kThreads + tid])) : 0u;
   };
   // A bound from below: of the w warps that hold elements each has r = ceil(top / w)
   // thread maxima at or above its r-th, so `top` threads reach the smallest of these.
+  const int warps = min(kThreads / 32, max(1, ((V + mis + VE - 1) / VE - c0 * CV + 31) / 32));
+  const uint32_t mine = first(0, tid, 0) < V ? order_bits(tm) : 0u;
   {
-    const int warps = min(kThreads / 32, max(1, ((V + mis + VE - 1) / VE - c0 * CV + 31) / 32));
-    uint32_t v = first(0, tid, 0) < V ? order_bits(tm) : 0u, r = 0;
+    uint32_t v = mine, r = 0;
     for (int q = (top + warps - 1) / warps; q > 0; --q) {
       r = __reduce_max_sync(0xffffffffu, v);
       if (lane == __ffs(__ballot_sync(0xffffffffu, v == r)) - 1) v = 0;
     }
     if (lane == 0) t.bound[warp] = r;
-    work_sync();
-    if (tid == 0) {
-      uint32_t tau = t.bound[0];
-      for (int w = 1; w < warps; ++w) tau = min(tau, t.bound[w]);
-      // An element equal to the list's last has a higher index: it must be above.
-      const uint32_t kth = (uint32_t)(t.best[t.cur][top - 1] >> 32);
-      t.tau = kth == 0xFFFFFFFFu ? kth : max(tau, kth + 1);
-    }
-    work_sync();
   }
+  work_sync();
   const int cur = t.cur;
-  const uint32_t tau = t.tau;
-  for (int q = 0; q < nch; ++q) {
-    const uint32_t o = pair_max(q);
-    if (o != 0 && o >= tau) {
-      const int at = atomicAdd(&t.pairs, 1);
-      if (at < kPairs) {
-        t.pair_v[at] = o;
-        t.pair_id[at] = q * kThreads + tid;
+  uint32_t tau = 0xFFFFFFFFu;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w)
+    if (w < warps) tau = min(tau, t.bound[w]);
+  {
+    // An element equal to the list's last has a higher index: it must be above.
+    const uint32_t kth = (uint32_t)(t.best[cur][top - 1] >> 32);
+    tau = kth == 0xFFFFFFFFu ? kth : max(tau, kth + 1);
+  }
+  if (mine >= tau) {
+#pragma unroll
+    for (int q = 0; q < kWin<T>; ++q) {
+      const uint32_t o = pair_max(q);
+      if (o != 0 && o >= tau) {
+        const int at = atomicAdd(&t.pairs, 1);
+        if (at < kPairs) {
+          t.pair_v[at] = o;
+          t.pair_id[at] = q * kThreads + tid;
+        }
       }
     }
   }
   if (tid < kMaxTop) t.best[cur ^ 1][tid] = 0;
+  if (tid == 0) t.t2 = tau == 0 ? 0 : tau - 1;
   work_sync();
   // t2: the top-th largest pair maximum (just below tau if there are fewer pairs).
-  int n = t.pairs;
+  // Chosen are the pairs that fewer than `top` others exceed, which reach it.
+  const int n = t.pairs;
   const bool flood = n > kPairs;
-  uint32_t t2 = tau == 0 ? 0 : tau - 1;
   if (flood) {
-    t2 = 0;
+    uint32_t t2 = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t at_least = t2 | (1u << bit);
       int c = 0;
       for (int q = 0; q < nch; ++q) c += pair_max(q) >= at_least;
       if (work_sum(t, c) >= top) t2 = at_least;
     }
-    if (tid == 0) t.pairs = 0;
-    work_sync();
-    for (int q = 0; q < nch; ++q) {
-      const uint32_t o = pair_max(q);
-      if (o > t2) {  // fewer than `top` pairs
-        const int at = atomicAdd(&t.pairs, 1);
-        t.pair_v[at] = o;
-        t.pair_id[at] = q * kThreads + tid;
-      }
-    }
-    work_sync();
-    n = t.pairs;
-  } else if (n >= top) {
+    if (tid == 0) t.t2 = t2;
+    for (int q = 0; q < nch; ++q)
+      if (pair_max(q) > t2)  // fewer than `top` pairs
+        t.chosen[atomicAdd(&t.picked, 1)] = q * kThreads + tid;
+  } else {
     for (int j = tid; j < n; j += kThreads) {
       const uint32_t v = t.pair_v[j];
       int above = 0, reach = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = 0; i < n; ++i) {
         above += t.pair_v[i] > v;
         reach += t.pair_v[i] >= v;
       }
-      if (above < top && reach >= top) t.tau = v;
+      if (above < top) {
+        t.chosen[atomicAdd(&t.picked, 1)] = t.pair_id[j];
+        if (reach >= top) t.t2 = v;
+      }
     }
-    work_sync();
-    t2 = t.tau;
   }
-  // Elements of the pairs that reach t2: those above it all, those equal to it
-  // unless they come in a flood.
-  for (int j = tid; j < n * E; j += kThreads) {
-    const int p = j / E;
-    if (t.pair_v[p] < t2) continue;
-    const int id = t.pair_id[p];
+  work_sync();
+  // Their elements: those above t2 all, those equal to it unless they come in a flood.
+  const uint32_t t2 = t.t2;
+  const int elements = t.picked * E;
+#pragma unroll 2
+  for (int j = tid; j < elements; j += kThreads) {
+    const int id = t.chosen[j / E];
     const int e = first(id / kThreads, id % kThreads, j % E / VE) + j % VE;
     if (e < 0 || e >= V) continue;
     const float x = Cvt<T>::to_f(row[e]);
@@ -396,13 +392,13 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
       for (int i = 0; i < kU && ties < top; ++i) {
         const int e0 = first(q, tid, i);
         float f[VE];
-        int mine = 0;
+        int here = 0;
         if (pair_max(q) >= t2) {
           unpack_vec<T>(load_vec<T>(row, e0, V), f);
 #pragma unroll
-          for (int u = 0; u < VE; ++u) mine += e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2;
+          for (int u = 0; u < VE; ++u) here += e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2;
         }
-        int before = mine;
+        int before = here;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int y = __shfl_up_sync(0xffffffffu, before, o);
@@ -410,13 +406,13 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
         }
         if (lane == 31) t.bound[warp] = (uint32_t)before;
         work_sync();
-        int at = ties + before - mine, all = 0;
+        int at = ties + before - here, all = 0;
 #pragma unroll
         for (int w = 0; w < kThreads / 32; ++w) {
           if (w < warp) at += (int)t.bound[w];
           all += (int)t.bound[w];
         }
-        if (mine > 0) {
+        if (here > 0) {
 #pragma unroll
           for (int u = 0; u < VE; ++u)
             if (e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2) {
@@ -430,26 +426,27 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
   }
   // Keys differ, so a key's rank is the number of larger ones, whatever order
   // they were noted in.
-  for (int i = tid; i < above + ties + kMaxTop; i += kThreads) {
+  for (int i = tid; i < above + ties + top; i += kThreads) {
     const unsigned long long key = i < above          ? t.cand[i]
                                    : i < above + ties ? t.cand[kAbove + i - above]
                                                       : t.best[cur][i - above - ties];
     if (key == 0) continue;
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < kMaxTop; ++j) rank += t.best[cur][j] > key;
 #pragma unroll 4
+    for (int j = 0; j < top; ++j) rank += t.best[cur][j] > key;
+#pragma unroll 8
     for (int j = 0; j < above; ++j) rank += t.cand[j] > key;
 #pragma unroll 4
     for (int j = 0; j < ties; ++j) rank += t.cand[kAbove + j] > key;
     if (rank < top) t.best[cur ^ 1][rank] = key;
   }
   work_sync();
+  // (Others read these behind the next barrier.)
   if (tid == 0) {
     t.cur = cur ^ 1;
-    t.pairs = t.above = t.ties = 0;
+    t.pairs = t.picked = t.above = t.ties = 0;
   }
-  work_sync();
+  __syncwarp();
 }
 
 // What a row's other segments hand to its first CTA.
@@ -496,15 +493,15 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
   // through the ring, the two at its ends are read element by element.
   auto row_of = [&](int64_t n) { return reinterpret_cast<const T*>(a.x) + n * a.row_stride; };
   auto mis_of = [](const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); };
-  auto seg_begin = [&](int64_t seg) { return (int)((int64_t)a.chunks * seg / a.segs); };
+  auto seg_begin = [&](int seg) { return (int)(((int64_t)a.chunks * seg) >> a.seg_bits); };
 
   if (warp == kThreads / 32) {
     // ---------------------------------------------------------------- copies
     int k = 0;  // chunks issued
     bool ok = true;
     for (int64_t item = blockIdx.x; lane == 0 && ok && item < items; item += gridDim.x) {
-      const T* row = row_of(item / a.segs);
-      const int seg = (int)(item % a.segs), mis = mis_of(row);
+      const T* row = row_of(item >> a.seg_bits);
+      const int seg = (int)item & (a.segs - 1), mis = mis_of(row);
       const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
       for (int c = seg_begin(seg); c < seg_begin(seg + 1); ++c, ++k) {
         const int st = k % kStages;
@@ -534,8 +531,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
   int k = 0;  // chunks taken
   int parity = 0;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t n = item / a.segs;
-    const int seg = (int)(item % a.segs);
+    const int64_t n = item >> a.seg_bits;
+    const int seg = (int)item & (a.segs - 1);
     const int c0 = seg_begin(seg), c1 = seg_begin(seg + 1);
     const T* row = row_of(n);
     const int mis = mis_of(row);
@@ -545,7 +542,7 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
     // touch it behind the first chunk's barrier.
     if (a.top > 0 && warp == 0) {
       tl.best[0][lane] = 0;
-      if (lane == 0) tl.pairs = tl.above = tl.ties = tl.cur = 0;
+      if (lane == 0) tl.pairs = tl.picked = tl.above = tl.ties = tl.cur = 0;
     }
     float tm = -INFINITY;  // this thread's maximum over the window
     int wn = 0;            // chunks of the window so far
@@ -834,6 +831,8 @@ extern "C" int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, 
   a.V = (int)V;
   a.chunks = (int)row_chunks(V, dtype);
   a.segs = row_segs(N, V, dtype);
+  a.seg_bits = 0;
+  while (1 << a.seg_bits < a.segs) ++a.seg_bits;
   a.targets = targets;
   a.t64 = targets_is_i64;
   a.top = top;
