@@ -318,8 +318,14 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
     tau = kth == 0xFFFFFFFFu ? kth : max(tau, kth + 1);
   }
   if (mine >= tau) {
+    // Candidates first by a float comparison, in few instructions (this code runs
+    // once per row, so its size costs instruction fetches); NaN passes it.
+    const float tau_f = order_value(tau);
+    uint32_t pass = 0;
 #pragma unroll
-    for (int q = 0; q < kWin<T>; ++q) {
+    for (int q = 0; q < kWin<T>; ++q) pass |= Cvt<T>::to_f(wm[q * kThreads + tid]) < tau_f ? 0u : 1u << q;
+    for (pass &= (1u << nch) - 1; pass != 0; pass &= pass - 1) {
+      const int q = __ffs(pass) - 1;
       const uint32_t o = pair_max(q);
       if (o != 0 && o >= tau) {
         const int at = atomicAdd(&t.pairs, 1);
@@ -368,7 +374,7 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
   // Their elements: those above t2 all, those equal to it unless they come in a flood.
   const uint32_t t2 = t.t2;
   const int elements = t.picked * E;
-#pragma unroll 2
+#pragma unroll 1
   for (int j = tid; j < elements; j += kThreads) {
     const int id = t.chosen[j / E];
     const int e = first(id / kThreads, id % kThreads, j % E / VE) + j % VE;
@@ -426,19 +432,20 @@ __device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int
   }
   // Keys differ, so a key's rank is the number of larger ones, whatever order
   // they were noted in.
-  for (int i = tid; i < above + ties + top; i += kThreads) {
-    const unsigned long long key = i < above          ? t.cand[i]
-                                   : i < above + ties ? t.cand[kAbove + i - above]
-                                                      : t.best[cur][i - above - ties];
-    if (key == 0) continue;
+  // Eight lanes share a key's comparisons.
+  for (int i0 = 0; i0 < above + ties + top; i0 += kThreads / 8) {
+    const int i = i0 + (tid >> 3);
+    const unsigned long long key = i < above                ? t.cand[i]
+                                   : i < above + ties       ? t.cand[kAbove + i - above]
+                                   : i < above + ties + top ? t.best[cur][i - above - ties]
+                                                            : 0;
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < top; ++j) rank += t.best[cur][j] > key;
-#pragma unroll 8
-    for (int j = 0; j < above; ++j) rank += t.cand[j] > key;
-#pragma unroll 4
-    for (int j = 0; j < ties; ++j) rank += t.cand[kAbove + j] > key;
-    if (rank < top) t.best[cur ^ 1][rank] = key;
+    for (int j = tid & 7; j < top; j += 8) rank += t.best[cur][j] > key;
+    for (int j = tid & 7; j < above; j += 8) rank += t.cand[j] > key;
+    for (int j = tid & 7; j < ties; j += 8) rank += t.cand[kAbove + j] > key;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (key != 0 && rank < top && (tid & 7) == 0) t.best[cur ^ 1][rank] = key;
   }
   work_sync();
   // (Others read these behind the next barrier.)
