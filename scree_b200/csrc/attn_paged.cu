@@ -18,8 +18,8 @@
 // key hide under that).  A group is as many keys as make 8 KB of K and V: the
 // chain scores -> maximum -> exponentials -> product takes a warp about 1,000
 // cycles whatever the number of keys, and with 16 keys at D = 64 that, not HBM,
-// set the pace (2 x 131071 keys: 28 us against XXLONG).  It is loaded in boxes of 16
-// keys, which never span pages.
+// set the pace (2 x 131071 keys: main kernel 25 us against 21).  It is loaded in
+// boxes of 16 keys, which never span pages.
 #include <algorithm>
 #include "attn_paged.cuh"
 

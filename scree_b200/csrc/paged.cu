@@ -24,7 +24,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kThreads = 256;
 constexpr int kMaxSlots = 65536;
-constexpr int kHereEntries = 8192, kHereWarps = 128;  // see apply_by_plan
+constexpr int kHereEntries = 2048, kHereWarps = 32;  // see apply_by_plan
 constexpr int kSitePagedArgs = 60;    // a slot, count, length or path out of range
 constexpr int kSitePagedFull = 61;    // not enough free pages
 constexpr int kSitePagedShared = 62;  // a draft on pages that other slots hold
@@ -786,8 +786,11 @@ int launch_apply_w(const Book& b, const Pools& pl, const int32_t* slots, const i
   count_launch();
   return SCREE_OK;
 }
-// A call is applied by its plan's CTA if that takes it no longer than a second
-// launch: measured, XXMEASURE.
+// A call is applied by its plan's CTA if that takes it about as long as a second
+// launch, which costs the host 3 us more.  Reserve, by the plan's CTA / by a
+// launch of its own: 4.4 / 4.4 us at 256 table entries, 5.9 / 5.8 at 2,048, 7.0 /
+// 6.6 at 4,096, 15.1 / 9.4 at 16,384.  Fork and accept with one moving task per
+// warp (32): 8.4 / 7.2 and 7.5 / 5.8 us; with four: 16.2 / 7.5 and 17.9 / 6.0.
 bool apply_by_plan(const Book& b, int64_t units, int w) {
   return (int64_t)b.S * b.M <= kHereEntries && units <= kHereWarps && w == 16;
 }
