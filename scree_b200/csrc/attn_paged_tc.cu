@@ -8,7 +8,10 @@
 // As in attn_paged.cu all units laid end to end are cut into equal runs, one per
 // CTA (one CTA per SM), and pieces of split segments are joined by a second
 // kernel.  A and B share every K/V tile in shared memory, and the tensor core
-// works on one while the softmax of the other runs.
+// works on one while the softmax of the other runs.  Where a segment has but one
+// tile of rows, A takes its even key tiles and B the odd ones, and A's warps join
+// the two when they store the piece (one alone left half of the softmax warps idle:
+// 64 x 2048 keys, 64 rows, 176 us against XXSPLIT).
 //
 //   warp 8   finds the CTA's pieces, publishes their records through a ring,
 //            loads Q and the K ring (TMA; a tile is 128 / box rows boxes, since
@@ -140,12 +143,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* pv_done = p_full + 2;            // [2]
   uint64_t* q_empty = pv_done + 2;
   uint64_t* o_empty = q_empty + 1;           // [2]
-  uint64_t* rec_full = o_empty + 2;          // [kRing]
+  uint64_t* ml_full = o_empty + 2;           // B's (m, l) of a split piece are there
+  uint64_t* ml_free = ml_full + 1;           // and have been read
+  uint64_t* rec_full = ml_free + 1;          // [kRing]
   uint64_t* rec_empty = rec_full + kRing;    // [kRing]
   Rec* ring = reinterpret_cast<Rec*>(rec_empty + kRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring + kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((1 + 2 * C::KSTAGES + 2 * C::VSTAGES + 8 + 3 + 2 * kRing) * 8 + kRing * sizeof(Rec) + 8 <= 512,
+  static_assert((1 + 2 * C::KSTAGES + 2 * C::VSTAGES + 8 + 5 + 2 * kRing) * 8 + kRing * sizeof(Rec) + 8 <= 512,
                 "barrier area");
   const uint32_t sQ = smem_u32(smem), sK = smem_u32(smem + C::OFF_K), sV = smem_u32(smem + C::OFF_V);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,6 +158,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
+    mbar_init(ml_full, 128);
+    mbar_init(ml_free, 128);
     for (int i = 0; i < C::KSTAGES; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -195,6 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     e = ring[k % kRing];
     return true;
   };
+  // A piece of one tile of rows and at least two of keys is split by keys between A and B.
+  auto is_split = [&](const Rec& e) { return e.ntok <= tpt && e.t1 - e.t0 >= 2; };
   // Tile t's keys by one warp: lane l < 8 knows the page of key group 8 t + l (the
   // last valid group beyond the end: its keys are masked, its V cleared).
   auto tile_pages = [&](const Rec& e, int t) {
@@ -220,8 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) {
     // ------------------------------------------------------------ pieces, Q, K
     regs_dec<kRegsOther>();
-    int kc = 0, k = 0;
-    bool ok = true;
+    int kc = 0, k = 0, splits = 0;
+    bool ok = true, was_split = false;
     int b = b_first;
     int64_t pre_b = pre_first;  // units before sequence b
     for (int64_t u = u0; ok; ++k) {
@@ -281,6 +290,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (e.t0 < 0) break;
       if (k > 0 && !(ok = __all_sync(0xffffffffu, wait(q_empty, k - 1)))) break;
+      // Q_B's place holds (m, l) at the end of a split piece.
+      if (was_split && !(ok = __all_sync(0xffffffffu, wait(ml_free, splits - 1)))) break;
+      was_split = is_split(e);
+      splits += was_split;
       const bool two = e.ntok > tpt;
       if (lane == 0) {
         mbar_expect_tx(q_full, (two ? 2 : 1) * tpt * p.G * D * 2);
@@ -328,8 +341,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = kk * 16;
         return (uint32_t)(((e / C::CHUNK) * rows * C::SWB + (e % C::CHUNK) * 2) >> 4);
       };
-      auto issue_s = [&](int x, int kpos) {
-        const uint64_t dq = make_sdesc(sQ + x * C::Q_BYTES, 16, 8 * C::SWB, C::SWZ);
+      auto issue_s = [&](int x, int qx, int kpos) {
+        const uint64_t dq = make_sdesc(sQ + qx * C::Q_BYTES, 16, 8 * C::SWB, C::SWZ);
         const uint64_t dk = make_sdesc(sK + (kpos % C::KSTAGES) * C::KV_BYTES, 16, 8 * C::SWB, C::SWZ);
         const uint32_t dt = tmem + C::COL_S + x * BN;
 #pragma unroll
@@ -356,9 +369,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (e.t0 < 0) break;
         const int nt = e.t1 - e.t0, nx = e.ntok > tpt ? 2 : 1;
         if (!(ok = wait(q_full, k))) break;
+        // O_X += P_X V of ring position vpos, round r of the piece.
+        auto pv = [&](int x, int r, int vpos) {
+          // O_X is overwritten once the piece before has been read out of it.
+          if (r == 0 && xc[x] > 0 && !wait(&o_empty[x], xc[x] - 1)) return false;
+          if (!wait(&p_half[x], sc[x] + r)) return false;
+          tc_fence_after();
+          issue_pv(x, r == 0, vpos, 0, BN / 32);
+          if (!wait(&p_full[x], sc[x] + r)) return false;
+          tc_fence_after();
+          issue_pv(x, r == 0, vpos, BN / 32, BN / 16);
+          umma_commit(&pv_done[x]);
+          return true;
+        };
+        if (is_split(e)) {
+          // S_A of tile 0 and S_B of tile 1, then each tile's product and S of the tile after next.
+          auto s_of = [&](int j) {
+            const int kn = kc + j;
+            if (!wait(&k_full[kn % C::KSTAGES], kn / C::KSTAGES)) return false;
+            tc_fence_after();
+            issue_s(j & 1, 0, kn);
+            umma_commit(&k_empty[kn % C::KSTAGES]);
+            if (j + 1 == nt) umma_commit(q_empty);  // the last S product
+            return true;
+          };
+          ok = s_of(0) && s_of(1);
+          for (int j = 0; ok && j < nt; ++j) {
+            const int vpos = vc + j;
+            if (!(ok = wait(&v_full[vpos % C::VSTAGES], vpos / C::VSTAGES))) break;
+            if (!(ok = pv(j & 1, j >> 1, vpos))) break;
+            umma_commit(&v_empty[vpos % C::VSTAGES]);
+            if (j + 2 < nt) ok = s_of(j + 2);
+          }
+          kc += nt;
+          vc += nt;
+          for (int x = 0; x < 2; ++x) {
+            sc[x] += (nt + 1 - x) / 2;
+            ++xc[x];
+          }
+          continue;
+        }
         if (!(ok = wait(&k_full[kc % C::KSTAGES], kc / C::KSTAGES))) break;
         tc_fence_after();
-        for (int x = 0; x < nx; ++x) issue_s(x, kc);
+        for (int x = 0; x < nx; ++x) issue_s(x, x, kc);
         umma_commit(&k_empty[kc % C::KSTAGES]);
         if (nt == 1) umma_commit(q_empty);
         for (int j = 0; ok && j < nt; ++j) {
@@ -367,16 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait(&v_full[vpos % C::VSTAGES], vpos / C::VSTAGES))) break;
           if (more && !(ok = wait(&k_full[kn % C::KSTAGES], kn / C::KSTAGES))) break;
           for (int x = 0; ok && x < nx; ++x) {
-            // O_X is overwritten once the piece before has been read out of it.
-            if (j == 0 && xc[x] > 0 && !(ok = wait(&o_empty[x], xc[x] - 1))) break;
-            if (!(ok = wait(&p_half[x], sc[x] + j))) break;
-            tc_fence_after();
-            issue_pv(x, j == 0, vpos, 0, BN / 32);
-            if (!(ok = wait(&p_full[x], sc[x] + j))) break;
-            tc_fence_after();
-            issue_pv(x, j == 0, vpos, BN / 32, BN / 16);
-            umma_commit(&pv_done[x]);
-            if (more) issue_s(x, kn);
+            if (!(ok = pv(x, j, vpos))) break;
+            if (more) issue_s(x, x, kn);
           }
           if (!ok) break;
           if (j + 2 == nt) umma_commit(q_empty);  // the last S products have been issued
@@ -402,24 +447,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t col_s = lane_base + C::COL_S + x * BN, col_o = lane_base + C::COL_O + x * D;
     const float sl2 = p.sl2;
     const int tok = r / p.G, hq = r - tok * p.G;  // token of the tile, head of the group
-    int sc = 0, vc = 0;
+    float2* ml_b = reinterpret_cast<float2*>(smem + C::Q_BYTES);  // (m, l) of B's rows of a split piece
+    int sc = 0, sc_b = 0, vc = 0, splits = 0;  // rounds of this tile so far, of B's; key tiles; split pieces
     bool ok = true;
     for (int k = 0; ok; ++k) {
       Rec e;
       ok = __all_sync(0xffffffffu, take(k, e));
       if (!ok || e.t0 < 0) break;
-      const bool tile_on = x == 0 || e.ntok > tpt;
-      const bool row_ok = r < tpt * p.G && x * tpt + tok < e.ntok;
-      const int nt = tile_on ? e.t1 - e.t0 : 0;
+      const bool split = is_split(e);
+      const int tiles = e.t1 - e.t0;
+      const int nt_b = split ? tiles / 2 : e.ntok > tpt ? tiles : 0;  // rounds of B
+      const int nt = x == 1 ? nt_b : tiles - (split ? nt_b : 0);
+      const int first_tok = split ? 0 : x * tpt;  // of this tile of rows
+      const bool row_ok = r < tpt * p.G && first_tok + tok < e.ntok;
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < nt; ++j) {
-        const int k0 = (e.t0 + j) * BN;
+        const int tile = split ? 2 * j + x : j;
+        const int k0 = (e.t0 + tile) * BN;
         const bool edge = k0 + BN > e.c0;
         if (edge) {
           // V row r of the tile: cleared past the end; of a drafted token, without
           // its infinities and NaN.  Both tiles' warps do this, each before it lets
           // its product start; whoever clears an element has set the mark first.
-          const int vpos = vc + j, st = vpos % C::VSTAGES;
+          const int vpos = vc + tile, st = vpos % C::VSTAGES;
           ok = wait(&v_full[st], vpos / C::VSTAGES);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
@@ -459,8 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         tmem_regs_ready<BN>(s);
         if (edge) {
-          const int i = e.i0 + x * tpt + (row_ok ? tok : 0);
-          const int64_t qrow = (int64_t)e.row0 + x * tpt + (row_ok ? tok : 0);
+          const int i = e.i0 + first_tok + (row_ok ? tok : 0);
+          const int64_t qrow = (int64_t)e.row0 + first_tok + (row_ok ? tok : 0);
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             const unsigned long long v = row_ok ? paged_visible<64>(p, qrow, i, k0 + hf * 64, e.c0, e.len) : 0ull;
@@ -534,14 +584,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&p_full[x]);
       }
       // ------------------------------------------------------------ the piece is done
-      if (ok && tile_on) {
+      if (ok && nt > 0) {
         ok = wait(&pv_done[x], sc + nt - 1);
         ok = __all_sync(0xffffffffu, ok);
       }
-      if (ok && tile_on) {
+      float fa = 1.f, fb = 0.f;  // weights of O_A and O_B in a split piece
+      if (ok && split) {
+        // B's warps leave (m, l) and go on; A's join the two and store the piece.
+        // (B cannot come here again before A has read: its next O waits for that.)
+        if (x == 1) {
+          ml_b[r] = make_float2(m_used, l);
+          mbar_arrive(ml_full);
+        } else {
+          ok = __all_sync(0xffffffffu, wait(ml_full, splits) && wait(&pv_done[1], sc_b + nt_b - 1));
+          const float2 o = ml_b[r];
+          fence_proxy_async_smem();
+          mbar_arrive(ml_free);
+          const float m = fmaxf(m_used, o.x), ref = m == -INFINITY ? 0.f : m;
+          fa = ex2_approx(m_used - ref);
+          fb = ex2_approx(o.x - ref);
+          l = fa * l + fb * o.y;
+          m_used = m;
+        }
+      }
+      if (ok && nt > 0 && !(split && x == 1)) {
         tc_fence_after();
         const bool special = *reinterpret_cast<volatile int32_t*>(&ring[k % kRing].special) != 0;
-        const int64_t qrow = (int64_t)e.row0 + x * tpt + tok;
+        const int64_t qrow = (int64_t)e.row0 + first_tok + tok;
         const int head = e.h * p.G + hq;
         const bool whole = e.part < 0;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -551,10 +620,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           tmem_ld32_sync(col_o + c * 32, o);
+          if (split) {
+            float ob[32];
+            tmem_ld32_sync(col_o + D + c * 32, ob);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) o[q] = fa * o[q] + fb * ob[q];
+          }
           if (special && row_ok) {
             // The infinities and NaN that were taken out of V, for the keys that this row sees.
             for (int kk = max(e.c0, e.t0 * BN); kk < min(e.len, e.t1 * BN); ++kk) {
-              if (!(paged_visible<16>(p, qrow, e.i0 + x * tpt + tok, kk, e.c0, e.len) & 1)) continue;
+              if (!(paged_visible<16>(p, qrow, e.i0 + first_tok + tok, kk, e.c0, e.len) & 1)) continue;
               const int page = paged_page(p, e.slot, kk / kPagedKeys);
               const uint32_t* v = reinterpret_cast<const uint32_t*>(
                   reinterpret_cast<const T*>(p.v) +
@@ -587,13 +662,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         mbar_arrive(&o_empty[x]);  // O_X has been read
+        if (split) mbar_arrive(&o_empty[1]);
         if (row_ok && !whole) p.part_ml[((int64_t)e.part * 2 + x) * BM + r] = make_float2(m_used, l);
         if (row_ok && whole && p.lse != nullptr)
           p.lse[qrow * p.H + head] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
       }
       mbar_arrive(&rec_empty[k % kRing]);
       sc += nt;
-      vc += e.t1 - e.t0;
+      sc_b += nt_b;
+      vc += tiles;
+      splits += split;
     }
   }
 
