@@ -14,7 +14,7 @@
 // whole is written out by it; pieces of a split segment go to the workspace as
 // (m, l, O) and a second kernel joins them.
 //
-// Bound: HBM, 4 D bytes per key and K/V head (R <= 32 rows of mma.sync work per
+// Bound: HBM, 4 D bytes per key and K/V head (R = 16 rows of mma.sync work per
 // key hide under that).  A group is as many keys as make 8 KB of K and V: the
 // chain scores -> maximum -> exponentials -> product takes a warp about 1,000
 // cycles whatever the number of keys, and with 16 keys at D = 64 that, not HBM,
@@ -29,6 +29,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBox = kPagedKeys;     // keys of a box
+constexpr int R = 16;                // rows of a tile: one mma
 // A segment's units are kLead idle ones, which stand for what starting a piece
 // costs a worker, and its groups.
 constexpr int kLead = 1;
@@ -73,12 +74,11 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
   cvt_from_f<T, 2>(f, o);
   return (uint32_t)*reinterpret_cast<uint16_t*>(&o[0]) | ((uint32_t)*reinterpret_cast<uint16_t*>(&o[1]) << 16);
 }
-template <int D, typename T, int MT>
+template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const PagedParams p) {
   using C = Cfg<D>;
-  constexpr int R = 16 * MT;
   constexpr int KK = D / 16;  // k-steps of Q K^T = pairs of 8-column tiles of O
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -206,34 +206,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (u >= u1) break;  // the run ends in a segment's lead
     const int c0 = g.len - n;
     const int rows = min(R, n * p.G - g.rt * R);
-    // Rows of this lane: tile mt, half r -> row mt * 16 + r * 8 + qr of the tile.
-    auto row_of = [&](int mt, int r) { return mt * 16 + r * 8 + qr; };
-    uint32_t qf[MT][KK][4];
+    // Rows of this lane: half r -> row r * 8 + qr of the tile.
+    auto row_of = [&](int r) { return r * 8 + qr; };
+    uint32_t qf[KK][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int r = 0; r < 2; ++r) {
+      const int row = row_of(r);
+      const int a = g.rt * R + row;
+      const bool in = row < rows;
+      const char* src = p.q + (q0 + (in ? a / p.G : 0)) * p.q_rs + (int64_t)(g.h * p.G + (in ? a % p.G : 0)) * p.q_hs;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = row_of(mt, r);
-        const int a = g.rt * R + row;
-        const bool in = row < rows;
-        const char* src = p.q + (q0 + (in ? a / p.G : 0)) * p.q_rs + (int64_t)(g.h * p.G + (in ? a % p.G : 0)) * p.q_hs;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          qf[mt][kk][r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + qc) * 2) : 0u;
-          qf[mt][kk][2 + r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + 8 + qc) * 2) : 0u;
-        }
+      for (int kk = 0; kk < KK; ++kk) {
+        qf[kk][r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + qc) * 2) : 0u;
+        qf[kk][2 + r] = in ? *reinterpret_cast<const uint32_t*>(src + (kk * 16 + 8 + qc) * 2) : 0u;
       }
-    float o[MT][2 * KK][4];
-    float m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * KK; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
     }
+    float o[2 * KK][4];
+    float m[2], l[2];
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2 * KK; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
 #pragma unroll 1
     for (; u < end; ++u) {
       ok = paged_wait(p, &full[cst], phase, abort_flag);
@@ -243,87 +238,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t ks = ring_s + cst * C::STAGE, vs = ks + C::PART;
       constexpr int NT = 2 * C::GP;  // 8-key tiles of the scores
-      float s[MT][NT][4];
+      float s[NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][t][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int q = 0; q < C::GP; ++q) {
           uint32_t kf[4];
           ldsm_x4(ks + q * C::NB * C::BOX + chunk(k_key, kk * 2 + k_c), kf);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<T>(s[mt][2 * q], qf[mt][kk], kf[0], kf[1]);
-            mma16816<T>(s[mt][2 * q + 1], qf[mt][kk], kf[2], kf[3]);
-          }
+          mma16816<T>(s[2 * q], qf[kk], kf[0], kf[1]);
+          mma16816<T>(s[2 * q + 1], qf[kk], kf[2], kf[3]);
         }
       const int k0 = (int)(u - g.s0) * C::KEYS;
       const bool edge = k0 + C::KEYS > c0;  // holds new tokens, or runs past the end
-      unsigned long long vis[MT][2];
+      unsigned long long vis[2];
       if (edge) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int r = 0; r < 2; ++r) {
+          const int row = row_of(r), i = row < rows ? (g.rt * R + row) / p.G : 0;
+          vis[r] = paged_visible<C::KEYS>(p, q0 + i, i, k0, c0, g.len);
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int row = row_of(mt, r), i = row < rows ? (g.rt * R + row) / p.G : 0;
-            vis[mt][r] = paged_visible<C::KEYS>(p, q0 + i, i, k0, c0, g.len);
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (!(vis[mt][r] >> (t * 8 + qc + e) & 1)) s[mt][t][r * 2 + e] = -INFINITY;
-          }
+            for (int e = 0; e < 2; ++e)
+              if (!(vis[r] >> (t * 8 + qc + e) & 1)) s[t][r * 2 + e] = -INFINITY;
+        }
       }
       // Running maximum; rescaled only when it grew by more than 2^8 (P stays <= 256).
-      float alpha[MT][2];
+      float alpha[2];
       bool need = false;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(s[0][r * 2], s[0][r * 2 + 1]);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float mx = fmaxf(s[mt][0][r * 2], s[mt][0][r * 2 + 1]);
-#pragma unroll
-          for (int t = 1; t < NT; ++t) mx = fmax3(mx, s[mt][t][r * 2], s[mt][t][r * 2 + 1]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mc = mx * p.sl2;
-          alpha[mt][r] = 1.f;
-          if (mc > m[mt][r] + 8.f) {
-            alpha[mt][r] = ex2_approx(m[mt][r] - mc);
-            m[mt][r] = mc;
-            need = true;
-          }
-        }
-      if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          l[mt][0] *= alpha[mt][0];
-          l[mt][1] *= alpha[mt][1];
-#pragma unroll
-          for (int j = 0; j < 2 * KK; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][j][e] *= alpha[mt][e >> 1];
+        for (int t = 1; t < NT; ++t) mx = fmax3(mx, s[t][r * 2], s[t][r * 2 + 1]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mc = mx * p.sl2;
+        alpha[r] = 1.f;
+        if (mc > m[r] + 8.f) {
+          alpha[r] = ex2_approx(m[r] - mc);
+          m[r] = mc;
+          need = true;
         }
       }
-      uint32_t pf[MT][C::GP][4];
+      if (__any_sync(0xffffffffu, need)) {
+        l[0] *= alpha[0];
+        l[1] *= alpha[1];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+        for (int j = 0; j < 2 * KK; ++j)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mm = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
+          for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e >> 1];
+      }
+      uint32_t pf[C::GP][4];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float e0 = ex2_approx(fmaf(s[mt][t][r * 2], p.sl2, -mm));
-            const float e1 = ex2_approx(fmaf(s[mt][t][r * 2 + 1], p.sl2, -mm));
-            l[mt][r] += e0 + e1;
-            pf[mt][t >> 1][(t & 1) * 2 + r] = pack2<T>(e0, e1);
-          }
+      for (int r = 0; r < 2; ++r) {
+        const float mm = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float e0 = ex2_approx(fmaf(s[t][r * 2], p.sl2, -mm));
+          const float e1 = ex2_approx(fmaf(s[t][r * 2 + 1], p.sl2, -mm));
+          l[r] += e0 + e1;
+          pf[t >> 1][(t & 1) * 2 + r] = pack2<T>(e0, e1);
         }
+      }
       if (!edge) {
 #pragma unroll
         for (int q = 0; q < C::GP; ++q)
@@ -331,11 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < KK; ++j) {
             uint32_t vf[4];
             ldsm_x4_t(vs + q * C::NB * C::BOX + chunk(v_key, j * 2 + v_c), vf);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<T>(o[mt][2 * j], pf[mt][q], vf[0], vf[1]);
-              mma16816<T>(o[mt][2 * j + 1], pf[mt][q], vf[2], vf[3]);
-            }
+            mma16816<T>(o[2 * j], pf[q], vf[0], vf[1]);
+            mma16816<T>(o[2 * j + 1], pf[q], vf[2], vf[3]);
           }
       } else {
         // A key that a row does not see must not reach it even if its V is an
@@ -359,11 +337,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               special |= nf != 0;
               vf[e] &= ~nf;
             }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<T>(o[mt][2 * j], pf[mt][q], vf[0], vf[1]);
-              mma16816<T>(o[mt][2 * j + 1], pf[mt][q], vf[2], vf[3]);
-            }
+            mma16816<T>(o[2 * j], pf[q], vf[0], vf[1]);
+            mma16816<T>(o[2 * j + 1], pf[q], vf[2], vf[3]);
           }
         }
         if (__any_sync(0xffffffffu, special)) {
@@ -379,10 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (nonfinite_halves<T>(h) & 0xFFFFu) {
                   const float x = Cvt<T>::to_f(*reinterpret_cast<const T*>(&h));
 #pragma unroll
-                  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                      if (vis[mt][r] >> k & 1) o[mt][j][r * 2 + e] += x;  // P > 0
+                  for (int r = 0; r < 2; ++r)
+                    if (vis[r] >> k & 1) o[j][r * 2 + e] += x;  // P > 0
                 }
               }
           }
@@ -399,33 +372,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A run has at most one piece that continues a segment and one that leaves one.
     const int64_t slot = 2 * w + (begin > g.s0 ? 0 : 1);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int r = 0; r < 2; ++r) {
+      float sum = l[r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int row = row_of(r);
+      if (row >= rows) continue;
+      if (whole) {
+        const int a = g.rt * R + row, hq = g.h * p.G + a % p.G;
+        const int64_t tok = q0 + a / p.G;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        char* dst = p.o + tok * p.o_rs + hq * p.o_hs;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float sum = l[mt][r];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const int row = row_of(mt, r);
-        if (row >= rows) continue;
-        if (whole) {
-          const int a = g.rt * R + row, hq = g.h * p.G + a % p.G;
-          const int64_t tok = q0 + a / p.G;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          char* dst = p.o + tok * p.o_rs + hq * p.o_hs;
+        for (int j = 0; j < 2 * KK; ++j)
+          *reinterpret_cast<uint32_t*>(dst + (j * 8 + qc) * 2) =
+              pack2<T>(o[j][r * 2] * inv, o[j][r * 2 + 1] * inv);
+        if (p.lse != nullptr && (lane & 3) == 0)
+          p.lse[tok * p.H + hq] = sum == 0.f ? -INFINITY : (m[r] + log2f(sum)) * 0.69314718055994531f;
+      } else {
+        float* dst = p.part_o + (slot * R + row) * D;
 #pragma unroll
-          for (int j = 0; j < 2 * KK; ++j)
-            *reinterpret_cast<uint32_t*>(dst + (j * 8 + qc) * 2) =
-                pack2<T>(o[mt][j][r * 2] * inv, o[mt][j][r * 2 + 1] * inv);
-          if (p.lse != nullptr && (lane & 3) == 0)
-            p.lse[tok * p.H + hq] = sum == 0.f ? -INFINITY : (m[mt][r] + log2f(sum)) * 0.69314718055994531f;
-        } else {
-          float* dst = p.part_o + (slot * R + row) * D;
-#pragma unroll
-          for (int j = 0; j < 2 * KK; ++j)
-            *reinterpret_cast<float2*>(dst + j * 8 + qc) = make_float2(o[mt][j][r * 2], o[mt][j][r * 2 + 1]);
-          if ((lane & 3) == 0) p.part_ml[slot * R + row] = make_float2(m[mt][r], sum);
-        }
+        for (int j = 0; j < 2 * KK; ++j)
+          *reinterpret_cast<float2*>(dst + j * 8 + qc) = make_float2(o[j][r * 2], o[j][r * 2 + 1]);
+        if ((lane & 3) == 0) p.part_ml[slot * R + row] = make_float2(m[r], sum);
       }
+    }
   }
 }
 
@@ -437,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kJoinWarps = 8;
 constexpr int64_t kManyPieces = 16;
 template <int D, typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedParams p, int R) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedParams p) {
   constexpr int E = D / 32;         // columns of a lane
   constexpr int kLoads = E == 4 ? 8 : 16;  // O rows under way at a time
   __shared__ float sm_o[kJoinWarps][D];
@@ -535,21 +506,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   }
 }
 
-// Rows of a tile; 0: the tensor-core kernel's 2 x 128.  See scree_attn_fwd_paged.
-int tile_rows(int64_t B, int64_t T, int64_t H, int64_t H_kv) {
-  const int64_t rows = T * (H / H_kv);
-  return rows <= 16 * B ? 16 : rows <= 32 * B || H / H_kv > 128 ? 32 : 0;
+// Which kernel: this one pads a tile's rows to 16 and reads the cache once per tile;
+// the tensor-core one pads them to 128 and runs at its softmax's pace.  Measured (us,
+// this / that; D 128, 4 query heads a K/V head), for 16 sequences of 4096 keys at 8,
+// 16, 24 and 40 rows: 61 / 69, 63 / 71, 102 / 73, 100 / 74; for 64 of 2048 keys: 100 /
+// 143, 106 / 144, 189 / 145, 277 / 147.  (Two tiles of 16 rows in one pass of this
+// kernel, its registers spilling: 85 and 143 at 24 rows.)  The rows of a sequence are
+// known on the device only; their mean decides.  A tensor-core tile holds whole
+// tokens, so at most 128 heads a group.
+bool few_rows(int64_t B, int64_t T, int64_t H, int64_t H_kv) {
+  return T * (H / H_kv) <= R * B || H / H_kv > 128;
 }
 int64_t max_workers() { return (int64_t)num_sms() * kWarps; }
-size_t ws_bytes(int R, int D) {
-  if (R == 0) return attn_paged_tc_workspace(D);
+size_t ws_bytes(bool few, int D) {
+  if (!few) return attn_paged_tc_workspace(D);
   const int64_t N = max_workers();
   return (size_t)N * sizeof(PagedDesc) / 16 * 16 + 16 + (size_t)(2 * N) * R * (8 + 4 * (size_t)D);
 }
 
-template <int D, typename T, int MT>
+template <int D, typename T>
 int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, cudaStream_t s) {
-  auto kern = attn_paged_kernel<D, T, MT>;
+  auto kern = attn_paged_kernel<D, T>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -561,8 +538,7 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams
   SCREE_CUDA_TRY(launch_dependent(kern, dim3((unsigned)num_sms()), dim3(kThreads), Cfg<D>::smem(p.B), s, 1, tk, tv, p));
   count_launch();
   SCREE_CUDA_TRY(launch_dependent(attn_paged_join_kernel<D, T>, dim3((unsigned)max_workers() - 1),
-                                  dim3(kJoinWarps * 32), 0, s, 1,
-                                  p, 16 * MT));
+                                  dim3(kJoinWarps * 32), 0, s, 1, p));
   count_launch();
   return SCREE_OK;
 }
@@ -597,7 +573,7 @@ using namespace scree;
 
 extern "C" size_t scree_attn_fwd_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t H_kv, int D) {
   if (B < 1 || T < 0 || H < 1 || H_kv < 1 || H % H_kv != 0) return 0;
-  return ws_bytes(tile_rows(B, T, H, H_kv), D);
+  return ws_bytes(few_rows(B, T, H, H_kv), D);
 }
 
 extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, const scree_paged_pools* pools,
@@ -643,8 +619,8 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
                   "attn_fwd_paged: output must be 16-byte aligned with strides multiple of 8");
   SCREE_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "attn_fwd_paged: workspace must be 16-byte aligned");
   SCREE_BIND_DEVICE(stream, q);
-  const int R = tile_rows(B, T, H, H_kv);
-  SCREE_CHECK_ARG(workspace_bytes >= ws_bytes(R, D), "attn_fwd_paged: workspace too small");
+  const bool few = few_rows(B, T, H, H_kv);
+  SCREE_CHECK_ARG(workspace_bytes >= ws_bytes(few, D), "attn_fwd_paged: workspace too small");
   const bool bf16 = dtype == SCREE_BF16;
   PagedParams p;
   p.q = (const char*)q;
@@ -675,7 +651,7 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   p.lse = lse;
   p.status = device_status_ptr();
   cudaStream_t s = (cudaStream_t)stream;
-  if (R == 0) return attn_paged_tc(p, pools->k, pools->v, pool_rows, D, bf16, workspace, s);
+  if (!few) return attn_paged_tc(p, pools->k, pools->v, pool_rows, D, bf16, workspace, s);
   CUtensorMap tk, tv;
   int rc;
   if ((rc = make_pool_map(&tk, pools->k, pool_rows, D, kBox, bf16))) return rc;
@@ -686,13 +662,9 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   w += N * sizeof(PagedDesc) / 16 * 16 + 16;
   p.part_ml = (float2*)w;
   p.part_o = (float*)(w + 2 * N * R * 8);
-#define SCREE_PAGED_CASE(DD)                                                                       \
-  if (D == DD) {                                                                                   \
-    if (bf16)                                                                                      \
-      return R == 16 ? launch_paged<DD, __nv_bfloat16, 1>(tk, tv, p, s)                            \
-                     : launch_paged<DD, __nv_bfloat16, 2>(tk, tv, p, s);                           \
-    return R == 16 ? launch_paged<DD, __half, 1>(tk, tv, p, s) : launch_paged<DD, __half, 2>(tk, tv, p, s); \
-  }
+#define SCREE_PAGED_CASE(DD)                                                                         \
+  if (D == DD)                                                                                       \
+    return bf16 ? launch_paged<DD, __nv_bfloat16>(tk, tv, p, s) : launch_paged<DD, __half>(tk, tv, p, s);
   SCREE_PAGED_CASE(128)
   SCREE_PAGED_CASE(64)
   SCREE_PAGED_CASE(32)

@@ -11,7 +11,7 @@
 // works on one while the softmax of the other runs.  Where a segment has but one
 // tile of rows, A takes its even key tiles and B the odd ones, and A's warps join
 // the two when they store the piece (one alone left half of the softmax warps idle:
-// 64 x 2048 keys, 64 rows, 176 us against XXSPLIT).
+// 64 x 2048 keys, 64 rows, 176 us against 148).
 //
 //   warp 8   finds the CTA's pieces, publishes their records through a ring,
 //            loads Q and the K ring (TMA; a tile is 128 / box rows boxes, since
