@@ -85,6 +85,23 @@ def test_forward(cuda, dtype, N, V, k):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("N,V,k,dtype", [(3000, 5003, 5, torch.bfloat16), (1790, 40003, 32, torch.float32),
+                                         (1, 1200001, 20, torch.bfloat16), (2, 600001, 9, torch.float32)])
+def test_many_rows_and_long_rows(cuda, N, V, k, dtype):
+    """Rows that follow one another in a CTA; rows of more chunks than a window holds."""
+    from scree_b200.kernels.native import token_logprobs
+
+    x, t = _logits(N, V, dtype, cuda, seed=1)
+    x[N // 2] = torch.arange(V, device=cuda).to(torch.float32).mul(1.0 / V).to(dtype)  # rising
+    x[-1, V // 3:] = x[-1, 0]  # equal from there on
+    r = token_logprobs(x, t, top_k=k)
+    for a in range(0, N, 500):
+        rows = slice(a, a + 500)
+        part = type(r)(*(y[rows] for y in r))
+        _check(x[rows], t[rows], k, part, x[rows].double())
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shift", [0, 1, 3])
 def test_strided_rows_and_any_alignment(cuda, dtype, shift):
@@ -184,8 +201,6 @@ def _grad_ref(x, t, k, gl, gh, gt):
 def test_gradient(cuda, dtype, N, V, k, given):
     from scree_b200.kernels.native import token_logprobs_autograd
 
-    if given == "top" and k == 0:
-        pytest.skip("no alternatives")
     x, t = _logits(N, V, dtype, cuda, seed=V + 1)
     if N > 2:
         t[1] = -1
@@ -196,7 +211,7 @@ def test_gradient(cuda, dtype, N, V, k, given):
     y = x.detach().requires_grad_(True)
     r = token_logprobs_autograd(y, t, top_k=k)
     pairs = [(r.logp, gl, "logp"), (r.entropy, gh, "entropy"), (r.top_logp, gt, "top")]
-    outs = [(o, w) for o, w, n in pairs if (given == "all" and o.numel()) or given == n]
+    outs = [(o, w) for o, w, n in pairs if (given in ("all", n)) and (o.numel() or n != "top" or given == n)]
     torch.autograd.backward([o for o, _ in outs], [w for _, w in outs])
     want, tol = _grad_ref(x.double(), t, k, gl.double(), gh.double(), gt.double())
     err = (y.grad.double() - want).abs()

@@ -459,13 +459,16 @@ SHAPES = {
     "chunk": [(0, 37), (100, 21), (7, 64)],
     "wide": [(50, 130), (300, 65), (0, 1)],
     "many": [(i * 7 % 90, 1 + i % 3) for i in range(70)],
+    "one_tile_of_rows": [(500, 20), (129, 31), (0, 20), (1000, 17)],
+    "uneven": [(400, 90), (3, 1), (250, 40), (0, 1), (777, 33)],
 }
 
 
 @pytest.mark.parametrize("shape", list(SHAPES))
 @pytest.mark.parametrize("D,H,Hkv,page,dtype", [
     (128, 8, 2, 16, torch.bfloat16), (64, 3, 3, 64, torch.float16), (32, 14, 2, 48, torch.bfloat16),
-    (128, 3, 1, 128, torch.float16), (64, 20, 1, 16, torch.bfloat16)])
+    (128, 3, 1, 128, torch.float16), (64, 20, 1, 16, torch.bfloat16), (128, 4, 4, 32, torch.bfloat16),
+    (32, 130, 1, 16, torch.float16)])
 @pytest.mark.parametrize("tree", [False, True])
 def test_attention(cuda, shape, D, H, Hkv, page, dtype, tree):
     import scree_b200 as scree
@@ -502,14 +505,15 @@ def test_attention_long_context_split_over_the_gpu(cuda):
     assert _status() == 0
 
 
-@pytest.mark.parametrize("D,H,Hkv", [(128, 4, 2), (64, 40, 1)])
-def test_rows_that_see_nothing_and_masked_specials(cuda, D, H, Hkv):
+@pytest.mark.parametrize("D,H,Hkv", [(128, 4, 2), (64, 40, 1), (128, 2, 2), (32, 6, 3)])
+@pytest.mark.parametrize("before", [21, 380])
+def test_rows_that_see_nothing_and_masked_specials(cuda, D, H, Hkv, before):
     """Masks that leave rows empty; infinities and NaN in K and V of drafted tokens reach
     exactly the rows that see them."""
     import scree_b200 as scree
     from scree_b200 import paged
 
-    news, ctx = [5, 20, 3], [0, 21, 0]
+    news, ctx = [5, 20, 3], [0, before, 0]
     lens = [a + b for a, b in zip(ctx, news)]
     cache, slots, hs = _make(cuda, lens, 16, Hkv, D, torch.float16, seed=11)
     rng = np.random.default_rng(0)
@@ -603,6 +607,80 @@ def test_offsets_past_32_bits(cuda):
         out, lse = paged.paged_attention(scree.Array(q, _i32([0, 1], cuda)), cache, 0, _i32([s], cuda), return_lse=True)
         _compare(out.values, lse, _reference(q, cache, 0, [s], [n], [1], _causal([1])))
     assert _status() == 0
+
+
+def test_prompt_in_chunks_equals_the_prompt_at_once(cuda):
+    """Causal attention of a long prompt, cached in chunks, against varlen self-attention."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+    from scree_b200.kernels.native import varlen_attention_triton
+
+    n, H, Hkv, D = 1500, 4, 2, 64
+    q, k, v = (torch.randn((n, h, D), generator=torch.Generator().manual_seed(h + i)).to(torch.bfloat16).to(cuda)
+               for i, h in enumerate((H, Hkv, Hkv)))
+    cache = paged.paged_cache(1, 100, 16, Hkv, D, 2, 100, device=cuda)
+    slots, got, at = _i32([1], cuda), [], 0
+    for size in (700, 1, 300, 499):
+        cache = paged.paged_reserve(cache, slots, _i32([size], cuda))
+        a = lambda t: scree.Array(t[at:at + size], _i32([0, size], cuda))  # noqa: B023, E731
+        paged.paged_write(cache, 0, slots, a(k), a(v))
+        got.append(paged.paged_attention(a(q), cache, 0, slots).values)
+        at += size
+    want = varlen_attention_triton(q, k, v, _i32([0, n], cuda), causal=True)
+    # each within half an ulp of its own P and O roundings of the same definition
+    torch.testing.assert_close(torch.cat(got).float(), want.float(), atol=2e-2, rtol=2.0**-7)
+    assert _status() == 0
+
+
+def test_graph_capture_of_a_decoding_step(cuda):
+    import scree_b200 as scree
+    from scree_b200 import paged
+    from scree_b200.kernels.native import token_logprobs
+
+    cache, slots, hs = _make(cuda, [300, 41], 16, 2, 64, torch.bfloat16, seed=5)
+    q = scree.Array(torch.randn((2, 4, 64), device=cuda).to(torch.bfloat16), _i32([0, 1, 2], cuda))
+    kv = scree.Array(torch.randn((2, 2, 64), device=cuda).to(torch.bfloat16), _i32([0, 1, 2], cuda))
+    one = _i32([1, 1], cuda)
+    head = torch.randn((4 * 64, 3000), device=cuda).to(torch.bfloat16)
+    given = torch.tensor([5, 2999], device=cuda)
+
+    def run():
+        c = paged.paged_reserve(cache, slots, one)
+        paged.paged_write(c, 0, slots, kv, kv)
+        out = paged.paged_attention(q, c, 0, slots).values
+        s = token_logprobs(out.view(2, -1) @ head, given, top_k=3)
+        return c.table, c.lengths, c.refs, out, s.logp, s.entropy, s.top_logp, s.top_ids
+
+    want = [t.clone() for t in run()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert _status() == 0
+
+
+def test_speculative_decoding_example(cuda):
+    """The example's drafted trees give the tokens of plain greedy decoding, up to the few
+    places where two logits lie within rounding of one another, in fewer steps."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parent.parent / "examples" / "speculative_decoding.py"
+    spec = importlib.util.spec_from_file_location("speculative_decoding", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    plain, fast, steps, cache = mod.main(cuda, new_tokens=16)
+    # A near tie may send one sequence another way from there on; the others must agree.
+    assert sum(p == f for p, f in zip(plain, fast)) >= len(plain) - 1
+    assert steps < 16
+    assert cache.lengths.tolist()[0] == cache.lengths.tolist()[1] == cache.lengths.tolist()[2] > 0
+    used = int((cache.refs > 0).sum())
+    assert (cache.refs[:used] > 0).all() and (cache.refs[used:] == 0).all() and _status() == 0
 
 
 def test_attention_refusals(cuda):
