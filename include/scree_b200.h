@@ -376,7 +376,7 @@ int scree_tree_mask(const int32_t* parents, const void* offsets, int offs_is_i64
  * those n_b; of the n_b, query i sees token j where bit j of its mask row
  * (words x 64 bits) is set, or j <= i if mask is NULL.  A query that sees nothing gets
  * O = 0 and LSE = -inf.  K/V head = query head / (H / H_kv).  D 32, 64 or 128;
- * page a multiple of 16; at most 4096 sequences.  lse (T, H) fp32 or NULL.
+ * page a multiple of 16; at most 4096 sequences; scale > 0.  lse (T, H) fp32 or NULL.
  * The pools' base and row strides must suit TMA (16-byte aligned base).
  * workspace: 16-byte aligned. */
 size_t scree_attn_fwd_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t H_kv, int D);

@@ -369,7 +369,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       cst = cst + 1 == C::STAGES ? 0 : cst + 1;
       if (cst == 0) phase ^= 1;
     }
-    if (!ok) break;
+    if (!ok) {  // stages cst up to ist are in flight
+      do {
+        paged_drain(&full[cst], phase);
+        cst = cst + 1 == C::STAGES ? 0 : cst + 1;
+        if (cst == 0) phase ^= 1;
+      } while (cst != ist);
+      break;
+    }
     // ---------------------------------------------------------------- piece done
     const bool whole = begin == g.s0 && end == g.s1;
     // A run has at most one piece that continues a segment and one that leaves one.
@@ -612,6 +619,7 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   const int64_t pool_rows = pools->L * P * H_kv * page;
   SCREE_CHECK_ARG(pool_rows < (1ll << 31), "attn_fwd_paged: pools of %lld rows are too large", (long long)pool_rows);
   SCREE_CHECK_ARG(mask == nullptr || (words >= 1 && words < (1 << 20)), "attn_fwd_paged: bad mask width");
+  SCREE_CHECK_ARG(scale > 0.f, "attn_fwd_paged: scale %g must be positive", (double)scale);
   if (T == 0) return SCREE_OK;
   SCREE_CHECK_ARG(q && pools->k && pools->v && table && lengths && slots && offsets && o, "attn_fwd_paged: null pointer");
   SCREE_CHECK_ARG((uintptr_t)pools->k % 16 == 0 && (uintptr_t)pools->v % 16 == 0,

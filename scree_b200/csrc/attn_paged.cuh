@@ -132,6 +132,13 @@ __device__ __forceinline__ bool paged_wait(const PagedParams& p, uint64_t* bar, 
   return ok;
 }
 
+// Exit path: waits, as long at most, for a copy that may still be under way, so no
+// CTA ends with a copy to its shared memory in flight.
+__device__ __forceinline__ void paged_drain(uint64_t* bar, uint32_t parity) {
+  volatile int quiet = 0;
+  mbar_wait_impl(bar, parity & 1, &quiet, nullptr, kSitePagedAttnWait);
+}
+
 // Page that holds key group g (16 keys) of a slot; a bad id is recorded and read as page 0.
 __device__ __forceinline__ int paged_page(const PagedParams& p, int slot, int g) {
   const int page = p.table[(int64_t)slot * p.M + (unsigned)g * kPagedKeys / (unsigned)p.page];

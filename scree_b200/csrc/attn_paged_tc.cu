@@ -148,12 +148,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_empty = q_empty + 1;           // [2]
   uint64_t* ml_full = o_empty + 2;           // B's (m, l) of a split piece are there
   uint64_t* ml_free = ml_full + 1;           // and have been read
-  uint64_t* rec_full = ml_free + 1;          // [kRing]
+  uint64_t* mma_end = ml_free + 1;           // all MMAs are done
+  uint64_t* rec_full = mma_end + 1;          // [kRing]
   uint64_t* rec_empty = rec_full + kRing;    // [kRing]
   Rec* ring = reinterpret_cast<Rec*>(rec_empty + kRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring + kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((1 + 2 * C::KSTAGES + 2 * C::VSTAGES + 8 + 5 + 2 * kRing) * 8 + kRing * sizeof(Rec) + 8 <= 512,
+  static_assert((1 + 2 * C::KSTAGES + 2 * C::VSTAGES + 8 + 6 + 2 * kRing) * 8 + kRing * sizeof(Rec) + 8 <= 512,
                 "barrier area");
   const uint32_t sQ = smem_u32(smem), sK = smem_u32(smem + C::OFF_K), sV = smem_u32(smem + C::OFF_V);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(q_empty, 1);
     mbar_init(ml_full, 128);
     mbar_init(ml_free, 128);
+    mbar_init(mma_end, 1);
     for (int i = 0; i < C::KSTAGES; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -232,23 +234,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) {
     // ------------------------------------------------------------ pieces, Q, K
     regs_dec<kRegsOther>();
-    int kc = 0, k = 0, splits = 0;
+    int kc = 0, k = 0, qc = 0, splits = 0;
     bool ok = true, was_split = false;
-    int b = b_first;
-    int64_t pre_b = pre_first;  // units before sequence b
+    int b = b_first, of = -1;
+    int64_t pre_b = pre_first, hu = 0;  // units before sequence b; of one K/V head of sequence `of`
     for (int64_t u = u0; ok; ++k) {
       const int slot = k % kRing;
       if (k >= kRing && !(ok = __all_sync(0xffffffffu, wait(&rec_empty[slot], k / kRing - 1)))) break;
       Rec e;
       e.t0 = -1;
       while (u < u1) {
-        int64_t q0 = 0, n = 0, len = 0, hu = 0;
+        int64_t q0 = 0, n = 0, len = 0;
         while (true) {  // the sequence of unit u (those after the run's first, in turn)
           q0 = load_offset(p.offs, p.is64, b);
           n = load_offset(p.offs, p.is64, b + 1) - q0;
           e.slot = p.slots[b];
           len = p.lengths[e.slot];
-          hu = head_units(p, n, len, tok2);
+          if (of != b) hu = head_units(p, n, len, tok2);
+          of = b;
           if (u < pre_b + hu * p.Hkv || b + 1 >= p.B) break;
           pre_b += hu * p.Hkv;
           ++b;
@@ -307,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         e.row0 + x * tpt);
       }
       __syncwarp();
+      ++qc;
       int page = tile_pages(e, e.t0);
       for (int t = e.t0; t < e.t1; ++t, ++kc) {
         const int st = kc % C::KSTAGES;
@@ -316,6 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         page = next;
       }
     }
+    if (qc > 0) paged_drain(q_full, qc - 1);
+    for (int i = max(0, kc - C::KSTAGES); i < kc; ++i) paged_drain(&k_full[i % C::KSTAGES], i / C::KSTAGES);
   } else if (warp == 10) {
     // ------------------------------------------------------------ V
     regs_dec<kRegsOther>();
@@ -336,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         page = next;
       }
     }
+    for (int i = max(0, vc - C::VSTAGES); i < vc; ++i) paged_drain(&v_full[i % C::VSTAGES], i / C::VSTAGES);
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
     regs_dec<kRegsOther>();
@@ -438,6 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++xc[x];
         }
       }
+      umma_commit(mma_end);  // TMEM is freed behind the last product
+      paged_drain(mma_end, 0);
     }
   } else if (warp == 11) {
     regs_dec<kRegsOther>();  // idle: only completes its warpgroup's register release

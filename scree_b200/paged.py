@@ -256,7 +256,7 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
         mask = mask.contiguous()
         mask_ptr, words = mask.data_ptr(), mask.shape[1]
     sr, sh, sd = qt.stride()
-    if sd != 1 or sr % 8 or sh % 8 or qt.data_ptr() % 16:
+    if sd != 1 or sr % 8 or sh % 8 or sr * sh == 0 or qt.data_ptr() % 16:
         qt = qt.clone(memory_format=torch.contiguous_format)  # contiguous() would keep a misaligned base
         sr, sh, _ = qt.stride()
     out = torch.empty((T, H, D), dtype=dtype, device=dev)

@@ -735,3 +735,76 @@ def test_attention_refusals(cuda):
         paged.paged_attention(A(torch.zeros((3, 4, 96), dtype=torch.bfloat16, device=cuda)), odd, 0, slots)
     empty = call(q=A(q[:0], _i32([0, 0, 0], cuda)))
     assert empty.values.shape == (0, 4, 64) and _status() == 0
+
+
+def test_attention_of_many_rows_on_views(cuda):
+    """Queries as views: of a fused projection, heads first, one row for all tokens, a misaligned base."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+
+    lens, news = [300, 141], [45, 35]
+    cache, slots, _ = _make(cuda, lens, 16, 2, 64, torch.bfloat16, seed=8)
+    T, H, D = sum(news), 8, 64
+    gen = torch.Generator().manual_seed(9)
+    qkv = torch.randn((T, 3, H, D), generator=gen).to(torch.bfloat16).to(cuda)
+    offs = _i32([0, 45, 80], cuda)
+    call = lambda q: paged.paged_attention(scree.Array(q, offs), cache, 0, slots).values  # noqa: E731
+    q = qkv[:, 1].contiguous()
+    want = call(q)
+    _compare(want, paged.paged_attention(scree.Array(q, offs), cache, 0, slots, return_lse=True)[1],
+             _reference(q, cache, 0, slots.tolist(), lens, news, _causal(news)))
+    assert torch.equal(call(qkv[:, 1]), want)
+    assert torch.equal(call(q.transpose(0, 1).contiguous().transpose(0, 1)), want)
+    odd = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device=cuda)[1:].view(T, H, D).copy_(q)
+    assert torch.equal(call(odd), want)
+    assert torch.equal(call(q[:1].expand(T, H, D)), call(q[:1].repeat(T, 1, 1)))
+    assert torch.equal(call(q[:, :1].expand(T, H, D)), call(q[:, :1].repeat(1, H, 1)))
+    assert _status() == 0
+
+
+def test_offsets_past_32_bits_many_rows(cuda):
+    """As above for queries that take the tensor-core kernel, and an accept in the pools' last pages."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+
+    P, page, H, D = 2**21 + 64, 16, 1, 128
+    if torch.cuda.mem_get_info()[0] < 40 * 2**30:
+        pytest.skip("needs 40 GB")
+    k = torch.empty((1, P, H, page, D), dtype=torch.bfloat16, device=cuda)
+    v = torch.empty_like(k)
+    refs = torch.ones(P, dtype=torch.int32, device=cuda)
+    refs[-9:] = 0
+    cache = paged.PagedCache(k=k, v=v, table=torch.full((1, 8), -1, dtype=torch.int32, device=cuda),
+                             lengths=torch.zeros(1, dtype=torch.int32, device=cuda), refs=refs)
+    slots, n, m = _i32([0], cuda), 100, 40
+    cache = paged.paged_reserve(cache, slots, _i32([n], cuda))
+    assert cache.table[0, 0].item() == P - 9
+    gen = torch.Generator().manual_seed(4)
+    kv = torch.randn((n, 2, H, D), generator=gen).to(torch.bfloat16).to(cuda)
+    offs = _i32([0, n], cuda)
+    paged.paged_write(cache, 0, slots, scree.Array(kv[:, 0], offs), scree.Array(kv[:, 1], offs))
+    q = torch.randn((m, 2, D), generator=gen).to(torch.bfloat16).to(cuda)
+    out, lse = paged.paged_attention(scree.Array(q, _i32([0, m], cuda)), cache, 0, slots, return_lse=True)
+    _compare(out.values, lse, _reference(q, cache, 0, [0], [n], [m], _causal([m])))
+    path = [1, 5, 6, 30, 39]
+    cache = paged.paged_accept(cache, slots, _i32([m], cuda), torch.tensor([path], dtype=torch.int32, device=cuda))
+    rows = _rows(cache, cache.k, 0, 0, n - m + len(path))
+    assert np.array_equal(rows[n - m:, 0], to64(kv[[n - m + j for j in path], 0, 0]))
+    assert cache.lengths.item() == n - m + len(path) and _status() == 0
+
+
+def test_attention_refuses_a_scale_that_is_not_positive(cuda):
+    from scree_b200 import _lib
+
+    cache, slots, _ = _make(cuda, [40], 16, 2, 64, torch.bfloat16, seed=6)
+    q = torch.zeros((1, 4, 64), dtype=torch.bfloat16, device=cuda)
+    offs, out, lib = _i32([0, 1], cuda), torch.empty_like(q), _lib.load()
+    S, M, P, page, H, D = cache._pools.sizes
+    ws = torch.empty(lib.scree_attn_fwd_paged_workspace_size(1, 1, 4, 2, 64), dtype=torch.uint8, device=cuda)
+    for scale in (0.0, -1.0, float("nan")):
+        rc = lib.scree_attn_fwd_paged(
+            q.data_ptr(), 256, 64, cache._pools.ref, 0, cache.table.data_ptr(), cache.lengths.data_ptr(), S, M, P, page,
+            slots.data_ptr(), offs.data_ptr(), 0, 1, 1, 4, 64, _lib.BF16, scale, None, 0, out.data_ptr(), 256, 64, None,
+            ws.data_ptr(), ws.numel(), _lib.stream_ptr(q.device))
+        with pytest.raises(ValueError, match="scale"):
+            _lib.check(rc, "paged_attention")
