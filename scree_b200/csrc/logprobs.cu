@@ -39,14 +39,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;     // one alternative per lane when lists are merged
 constexpr int kU = 4;           // vectors of a thread per chunk
-constexpr int kPairs = 512;     // pairs noted at a merge before it counts as a flood
-constexpr int kAbove = 1024;    // elements above the k-th pair maximum: fewer than kMaxTop pairs x 32
-constexpr int kTies = 256;      // elements equal to it before they count as a flood
 constexpr int kCtasPerSm = 3;
 constexpr int kStages = 3;      // ring of chunks
 constexpr int kChunkBytes = kThreads * kU * 16;
-constexpr int kWinBytes = 32 * kThreads;
-constexpr int kRingSmem = kStages * kChunkBytes + kWinBytes + 128;
+constexpr int kWinRow = 32 + 4;  // a thread's maxima over a window (a word more: its rows start in different banks)
+constexpr int kWinBytes = kWinRow * kThreads;
+constexpr int kRingSmem = kStages * kChunkBytes + 2 * kWinBytes + 128;
+constexpr int kWarps = kThreads / 32;      // that work; one more copies, one finishes rows
 constexpr int kMaxSegs = 8;     // a portable cluster
 constexpr int kSiteRing = 51;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -182,6 +181,18 @@ template <typename K> __device__ __forceinline__ K lane_join(K a, K b, int lane)
   return lane_merge(a > r ? a : r, lane);
 }
 
+// 32 keys in descending order.
+template <typename K> __device__ __forceinline__ K lane_sort(K v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const K o = __shfl_xor_sync(0xffffffffu, v, j);
+      v = (((lane & j) == 0) == ((lane & k) == 0)) == (v > o) ? v : o;
+    }
+  return v;
+}
+
 struct FwdArgs {
   const void* x;
   int64_t row_stride, N;
@@ -198,25 +209,23 @@ struct FwdArgs {
   int* status;
 };
 
-// The row's outputs from its joined statistics; `key` is the lane's alternative.
+// The row's outputs from its joined statistics; `key` is the lane's alternative, t
+// the target and xt its logit (lane 0).
 template <typename T>
-__device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const Stat& s,
-                                           unsigned long long key, int lane) {
+__device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const Stat& s, unsigned long long key,
+                                           int64_t t, float xt, int lane) {
   // A row with nothing left (every logit -inf): logp = -inf, H = 0.
   const bool empty = s.m == -INFINITY;
   const float ls = log2f(s.s1) * kLn2;
   if (lane == 0) {
     if (a.norm != nullptr) a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
     a.entropy[n] = empty ? 0.f : (log2f(s.s1) - s.s2 / s.s1) * kLn2;
-    const int64_t t = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[n]
-                            : (int64_t)reinterpret_cast<const int32_t*>(a.targets)[n];
     float lp = 0.f;  // negative target: no token given
     if (t >= (int64_t)a.V) {
       record_device_error(a.status, SCREE_DEVERR_BAD_INPUT, kSiteTarget);
       lp = __uint_as_float(0x7FFFFFFFu);
     } else if (t >= 0) {
-      const float x = Cvt<T>::to_f(reinterpret_cast<const T*>(a.x)[n * a.row_stride + t]);
-      lp = empty ? -INFINITY : (x - s.m) - ls;
+      lp = empty ? -INFINITY : (xt - s.m) - ls;
     }
     a.logp[n] = lp;
   }
@@ -235,17 +244,12 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volati
   return ok;
 }
 
-// Barrier of the eight working warps.
-__device__ __forceinline__ void work_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-}
-
 // Vector at element e0 of a row (e0 a multiple of the vector size from a 16-byte
 // boundary); elements outside [0, V) read as -inf.
 template <typename T>
 __device__ __forceinline__ uint4 load_vec(const T* row, int e0, int V) {
   constexpr int VE = Lv<T>::N;
-  if (e0 >= 0 && e0 + VE <= V) return __ldcs(reinterpret_cast<const uint4*>(row + e0));
+  if (e0 >= 0 && e0 + VE <= V) return *reinterpret_cast<const uint4*>(row + e0);
   uint32_t w[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) w[u] = neg_inf_word<T>();
@@ -260,204 +264,180 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int e0, int V) {
 
 template <typename T> constexpr int kWin = 32 / (int)sizeof(T);  // chunks of a window
 
-// The list of the `top` best keys so far and the scratch of a merge.
-struct TopList {
-  unsigned long long best[2][kMaxTop];
-  unsigned long long cand[kAbove + kTies];
-  uint32_t pair_v[kPairs];  // order_bits of the pair's maximum
-  int pair_id[kPairs];      // chunk of the window * kThreads + thread
-  int chosen[kPairs];       // the pairs that reach the top-th largest maximum
-  uint32_t bound[kThreads / 32];
-  uint32_t t2;
-  int pairs, picked, above, ties;
-  int cur;  // which of best[] holds the list
+// A bound from below as a value of type T (NaN: every value reaches it), and which
+// of a word's elements reach it (NaN does): bit 0, and bit 16 of 16-bit types.
+template <typename T> struct Bound;
+template <> struct Bound<float> {
+  float v;
+  __device__ __forceinline__ explicit Bound(float f) : v(f) {}
+  __device__ __forceinline__ uint32_t reach(uint32_t w) const { return __uint_as_float(w) < v ? 0u : 1u; }
 };
-
-// Sum over the working threads (a barrier before and after).
-__device__ __forceinline__ int work_sum(TopList& t, int v) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) t.bound[threadIdx.x >> 5] = (uint32_t)v;
-  work_sync();
-  int s = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) s += (int)t.bound[w];
-  work_sync();
-  return s;
+template <> struct Bound<__nv_bfloat16> {
+  __nv_bfloat162 v;
+  __device__ __forceinline__ explicit Bound(float f) : v(__bfloat162bfloat162(__float2bfloat16_rd(f))) {}
+  __device__ __forceinline__ uint32_t reach(uint32_t w) const {
+    return ~__hlt2_mask(*reinterpret_cast<__nv_bfloat162*>(&w), v) & 0x00010001u;
+  }
+};
+template <> struct Bound<__half> {
+  __half2 v;
+  __device__ __forceinline__ explicit Bound(float f) : v(__half2half2(__float2half_rd(f))) {}
+  __device__ __forceinline__ uint32_t reach(uint32_t w) const {
+    return ~__hlt2_mask(*reinterpret_cast<__half2*>(&w), v) & 0x00010001u;
+  }
+};
+// Bit b of the words' reach(), word w shifted by w: which element of them it is.
+template <typename T> __device__ __forceinline__ int reach_element(int b) {
+  return sizeof(T) == 4 ? b : (b & 15) * 2 + (b >> 4);
 }
 
-// Merges the window of `nch` chunks from chunk c0 on into the list.  wm: the
-// window's maxima [chunk][thread]; tm: this thread's maximum over the window.  One
-// barrier a step: the rest of the row's stream waits for it.
+// Scratch of the merging warp.
+constexpr int kManyKeys = 12;  // elements of a pair that are sorted into the list at once
+constexpr int kCand = 96;      // elements that wait for their ranks
+struct MergeScratch {
+  unsigned long long cand[kCand + 32];  // (and the list, when they are ranked)
+  unsigned long long sorted[32];
+  int queue[64];                        // pairs to look at: their first elements
+  uint32_t queue_max[64];               // and order_bits of their maxima
+  uint16_t threads[kThreads];           // those whose maximum reaches the bound
+};
+
+// Merges the window of `nch` chunks from chunk c0 on into the list (32 keys in the
+// lanes, descending; the first `top` count).  wm: the window's maxima, kWinRow
+// bytes a thread; tm: the threads' maxima over the window.  By one warp, once a row:
+// what it costs is the fetching of its instructions and its chains of dependent
+// ones, so it is loops of few instructions, and lanes that each take a pair.
 template <typename T>
-__device__ __noinline__ void merge_window(TopList& t, int top, const T* row, int mis, int V, const T* wm,
-                                          int c0, int nch, float tm) {
-  constexpr int VE = Lv<T>::N, CV = kThreads * kU, E = kU * VE;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto first = [&](int q, int th, int i) { return ((c0 + q) * CV + i * kThreads + th) * VE - mis; };
-  // Whether the pair has elements, and its maximum.
-  auto pair_max = [&](int q) {
-    return q < nch && first(q, tid, 0) < V ? order_bits(Cvt<T>::to_f(wm[q * kThreads + tid])) : 0u;
-  };
-  // A bound from below: of the w warps that hold elements each has r = ceil(top / w)
-  // thread maxima at or above its r-th, so `top` threads reach the smallest of these.
-  const int warps = min(kThreads / 32, max(1, ((V + mis + VE - 1) / VE - c0 * CV + 31) / 32));
-  const uint32_t mine = first(0, tid, 0) < V ? order_bits(tm) : 0u;
-  {
-    uint32_t v = mine, r = 0;
-    for (int q = (top + warps - 1) / warps; q > 0; --q) {
-      r = __reduce_max_sync(0xffffffffu, v);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, v == r)) - 1) v = 0;
-    }
-    if (lane == 0) t.bound[warp] = r;
-  }
-  work_sync();
-  const int cur = t.cur;
-  uint32_t tau = 0xFFFFFFFFu;
+__device__ __forceinline__ unsigned long long merge_window(unsigned long long best, int top, const T* row, int mis,
+                                                           int V, const uint8_t* wm, const float* tm, int c0, int nch,
+                                                           MergeScratch& sc, int lane) {
+  constexpr int VE = Lv<T>::N, CV = kThreads * kU, E = kU * VE, G = kThreads / 32;
+  const uint32_t lt = (1u << lane) - 1;
+  const int base0 = c0 * CV * VE - mis;  // first element of the window's first thread
+  // A bound from below: the top-th largest of 64 maxima over four threads each (its
+  // upper 16 bits).
+  uint32_t m[G], tau = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w)
-    if (w < warps) tau = min(tau, t.bound[w]);
+  for (int g = 0; g < G; ++g)  // a thread without elements reaches no bound
+    m[g] = base0 + (g * 32 + lane) * VE < V ? order_bits(tm[g * 32 + lane]) : 0u;
   {
-    // An element equal to the list's last has a higher index: it must be above.
-    const uint32_t kth = (uint32_t)(t.best[cur][top - 1] >> 32);
-    tau = kth == 0xFFFFFFFFu ? kth : max(tau, kth + 1);
-  }
-  if (mine >= tau) {
-    // Candidates first by a float comparison, in few instructions (this code runs
-    // once per row, so its size costs instruction fetches); NaN passes it.
-    const float tau_f = order_value(tau);
-    uint32_t pass = 0;
-#pragma unroll
-    for (int q = 0; q < kWin<T>; ++q) pass |= Cvt<T>::to_f(wm[q * kThreads + tid]) < tau_f ? 0u : 1u << q;
-    for (pass &= (1u << nch) - 1; pass != 0; pass &= pass - 1) {
-      const int q = __ffs(pass) - 1;
-      const uint32_t o = pair_max(q);
-      if (o != 0 && o >= tau) {
-        const int at = atomicAdd(&t.pairs, 1);
-        if (at < kPairs) {
-          t.pair_v[at] = o;
-          t.pair_id[at] = q * kThreads + tid;
-        }
-      }
-    }
-  }
-  if (tid < kMaxTop) t.best[cur ^ 1][tid] = 0;
-  if (tid == 0) t.t2 = tau == 0 ? 0 : tau - 1;
-  work_sync();
-  // t2: the top-th largest pair maximum (just below tau if there are fewer pairs).
-  // Chosen are the pairs that fewer than `top` others exceed, which reach it.
-  const int n = t.pairs;
-  const bool flood = n > kPairs;
-  if (flood) {
-    uint32_t t2 = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t at_least = t2 | (1u << bit);
-      int c = 0;
-      for (int q = 0; q < nch; ++q) c += pair_max(q) >= at_least;
-      if (work_sum(t, c) >= top) t2 = at_least;
-    }
-    if (tid == 0) t.t2 = t2;
-    for (int q = 0; q < nch; ++q)
-      if (pair_max(q) > t2)  // fewer than `top` pairs
-        t.chosen[atomicAdd(&t.picked, 1)] = q * kThreads + tid;
-  } else {
-    for (int j = tid; j < n; j += kThreads) {
-      const uint32_t v = t.pair_v[j];
-      int above = 0, reach = 0;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        above += t.pair_v[i] > v;
-        reach += t.pair_v[i] >= v;
-      }
-      if (above < top) {
-        t.chosen[atomicAdd(&t.picked, 1)] = t.pair_id[j];
-        if (reach >= top) t.t2 = v;
-      }
-    }
-  }
-  work_sync();
-  // Their elements: those above t2 all, those equal to it unless they come in a flood.
-  const uint32_t t2 = t.t2;
-  const int elements = t.picked * E;
+    const uint32_t a = max(max(m[0], m[1]), max(m[2], m[3])), b = max(max(m[4], m[5]), max(m[6], m[7]));
 #pragma unroll 1
-  for (int j = tid; j < elements; j += kThreads) {
-    const int id = t.chosen[j / E];
-    const int e = first(id / kThreads, id % kThreads, j % E / VE) + j % VE;
-    if (e < 0 || e >= V) continue;
-    const float x = Cvt<T>::to_f(row[e]);
-    const uint32_t o = order_bits(x);
-    if (o > t2) {
-      t.cand[min(atomicAdd(&t.above, 1), kAbove - 1)] = order_key(x, (uint32_t)e);
-    } else if (o == t2 && !flood) {
-      const int at = atomicAdd(&t.ties, 1);
-      if (at < kTies) t.cand[kAbove + at] = order_key(x, (uint32_t)e);
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+      const uint32_t at_least = tau | bit;
+      const int n = __popc(__ballot_sync(0xffffffffu, a >= at_least)) + __popc(__ballot_sync(0xffffffffu, b >= at_least));
+      if (n >= top) tau = at_least;
     }
   }
-  work_sync();
-  const int above = t.above;
-  int ties = t.ties;
-  if (flood || ties > kTies) {
-    // Elements equal to t2 in the order of their indices, as many as can count.
-    ties = 0;
-    for (int q = 0; q < nch && ties < top; ++q)
-      for (int i = 0; i < kU && ties < top; ++i) {
-        const int e0 = first(q, tid, i);
-        float f[VE];
-        int here = 0;
-        if (pair_max(q) >= t2) {
-          unpack_vec<T>(load_vec<T>(row, e0, V), f);
+  unsigned long long kth = __shfl_sync(0xffffffffu, best, top - 1);
+  tau = max(tau, (uint32_t)(kth >> 32));
+  const Bound<T> bound(order_value(tau));
+  int flagged = 0;
 #pragma unroll
-          for (int u = 0; u < VE; ++u) here += e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2;
-        }
-        int before = here;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += y;
-        }
-        if (lane == 31) t.bound[warp] = (uint32_t)before;
-        work_sync();
-        int at = ties + before - here, all = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) {
-          if (w < warp) at += (int)t.bound[w];
-          all += (int)t.bound[w];
-        }
-        if (here > 0) {
-#pragma unroll
-          for (int u = 0; u < VE; ++u)
-            if (e0 + u >= 0 && e0 + u < V && order_bits(f[u]) == t2) {
-              if (at < top) t.cand[kAbove + at] = order_key(f[u], (uint32_t)(e0 + u));
-              ++at;
-            }
-        }
-        ties = min(top, ties + all);
-        work_sync();
-      }
-  }
-  // Keys differ, so a key's rank is the number of larger ones, whatever order
-  // they were noted in.
-  // Eight lanes share a key's comparisons.
-  for (int i0 = 0; i0 < above + ties + top; i0 += kThreads / 8) {
-    const int i = i0 + (tid >> 3);
-    const unsigned long long key = i < above                ? t.cand[i]
-                                   : i < above + ties       ? t.cand[kAbove + i - above]
-                                   : i < above + ties + top ? t.best[cur][i - above - ties]
-                                                            : 0;
-    int rank = 0;
-    for (int j = tid & 7; j < top; j += 8) rank += t.best[cur][j] > key;
-    for (int j = tid & 7; j < above; j += 8) rank += t.cand[j] > key;
-    for (int j = tid & 7; j < ties; j += 8) rank += t.cand[kAbove + j] > key;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    if (key != 0 && rank < top && (tid & 7) == 0) t.best[cur ^ 1][rank] = key;
-  }
-  work_sync();
-  // (Others read these behind the next barrier.)
-  if (tid == 0) {
-    t.cur = cur ^ 1;
-    t.pairs = t.picked = t.above = t.ties = 0;
+  for (int g = 0; g < G; ++g) {
+    const bool in = m[g] >= tau && m[g] != 0;
+    const uint32_t b = __ballot_sync(0xffffffffu, in);
+    if (in) sc.threads[flagged + __popc(b & lt)] = (uint16_t)(g * 32 + lane);
+    flagged += __popc(b);
   }
   __syncwarp();
+  int queued = 0, waiting = 0;
+  // The waiting elements enter the list.  Keys differ, so a key's place is the number
+  // of larger ones.
+  auto rank = [&]() {
+    const int had = __popc(__ballot_sync(0xffffffffu, best != 0));
+    if (lane < had) sc.cand[waiting + lane] = best;
+    sc.sorted[lane] = 0;
+    __syncwarp();
+    const int n = waiting + had;
+#pragma unroll 1
+    for (int i = lane; i - lane < n; i += 32) {
+      const unsigned long long key = i < n ? sc.cand[i] : 0;
+      int above = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) above += sc.cand[j] > key;
+      if (i < n && above < 32) sc.sorted[above] = key;
+    }
+    __syncwarp();
+    best = sc.sorted[lane];
+    kth = __shfl_sync(0xffffffffu, best, top - 1);
+    waiting = 0;
+  };
+  // The queued pairs' elements that reach the bound and are above the list's last; a
+  // lane reads a pair.
+  auto drain = [&]() {
+    __syncwarp();
+#pragma unroll 1
+    for (int at = 0; at < queued; at += 32) {
+      const bool in = at + lane < queued;
+      const int e0 = in ? sc.queue[at + lane] : 0;
+      const unsigned long long most = in ? (unsigned long long)sc.queue_max[at + lane] << 32 | (0xFFFFFFFFu - max(e0, 0)) : 0;
+      uint32_t pass = 0;
+      if (most > kth) {
+        uint4 v[kU];
+#pragma unroll
+        for (int i = 0; i < kU; ++i) v[i] = load_vec<T>(row, e0 + i * kThreads * VE, V);
+#pragma unroll
+        for (int i = 0; i < kU; ++i)
+          pass |= bound.reach(v[i].x) << (4 * i) | bound.reach(v[i].y) << (4 * i + 1) | bound.reach(v[i].z) << (4 * i + 2) |
+                  bound.reach(v[i].w) << (4 * i + 3);
+      }
+      // Pairs with many such elements by the whole warp.
+      for (uint32_t many = __ballot_sync(0xffffffffu, __popc(pass) >= kManyKeys); many != 0; many &= many - 1) {
+        const int src = __ffs(many) - 1;
+        if (__shfl_sync(0xffffffffu, most, src) <= kth) continue;
+        const int e = __shfl_sync(0xffffffffu, e0, src) + lane / VE * kThreads * VE + lane % VE;
+        unsigned long long key = lane < E && e >= 0 && e < V ? order_key(Cvt<T>::to_f(row[e]), (uint32_t)e) : 0;
+        if (key <= kth) key = 0;
+        best = lane_join(best, lane_sort(key, lane), lane);
+        kth = __shfl_sync(0xffffffffu, best, top - 1);
+      }
+      if (__popc(pass) >= kManyKeys) pass = 0;
+#pragma unroll 1
+      while (__any_sync(0xffffffffu, pass != 0)) {
+        const int x = reach_element<T>(__ffs(pass) - 1), e = e0 + x / VE * kThreads * VE + x % VE;
+        unsigned long long key = 0;
+        if (pass != 0 && e >= 0 && e < V) key = order_key(Cvt<T>::to_f(row[e]), (uint32_t)e);
+        pass &= pass - 1;
+        const uint32_t b = __ballot_sync(0xffffffffu, key > kth);
+        if (key > kth) sc.cand[waiting + __popc(b & lt)] = key;
+        waiting += __popc(b);
+        if (waiting > kCand - 32) rank();
+      }
+    }
+    __syncwarp();
+    queued = 0;
+  };
+  // A pair can matter if its maximum, at its lowest index, is above the list's last.
+  // Of 32 threads at a time: of equal values the first ones come early.
+#pragma unroll 1
+  for (int f0 = 0; f0 < flagged; f0 += 32) {
+    const int th = sc.threads[min(f0 + lane, flagged - 1)], e0 = base0 + th * VE;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(wm + th * kWinRow);
+    uint32_t pass = 0;
+#pragma unroll
+    for (int i = 0; i < kWinRow / 4 - 1; ++i) pass |= bound.reach(w[i]) << i;
+    const int have = f0 + lane < flagged ? min(nch, (V - e0 + CV * VE - 1) / (CV * VE)) : 0;  // chunks with elements
+    pass &= sizeof(T) == 4 ? (1u << have) - 1 : ((1u << ((have + 1) >> 1)) - 1) | ((1u << (have >> 1)) - 1) << 16;
+#pragma unroll 1
+    while (__any_sync(0xffffffffu, pass != 0)) {
+      bool in = pass != 0;
+      const int q = in ? reach_element<T>(__ffs(pass) - 1) : 0, e = e0 + q * CV * VE;
+      const uint32_t o = order_bits(Cvt<T>::to_f(reinterpret_cast<const T*>(w)[q]));
+      in = in && ((unsigned long long)o << 32 | (0xFFFFFFFFu - max(e, 0))) > kth;
+      pass &= pass - 1;
+      const uint32_t b = __ballot_sync(0xffffffffu, in);
+      if (in) {
+        sc.queue[queued + __popc(b & lt)] = e;
+        sc.queue_max[queued + __popc(b & lt)] = o;
+      }
+      queued += __popc(b);
+      if (queued > 32) drain();
+    }
+  }
+  if (queued > 0) drain();
+  if (waiting > 0) rank();
+  return best;
 }
 
 // What a row's other segments hand to its first CTA.
@@ -473,21 +453,28 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(const FwdArgs a) {
   constexpr int VE = Lv<T>::N, CV = kThreads * kU;  // elements of a vector, vectors of a chunk
   extern __shared__ __align__(16) uint8_t ring[];
-  T* wm = reinterpret_cast<T*>(ring + kStages * kChunkBytes);  // a window's maxima
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kChunkBytes + kWinBytes);
+  uint8_t* wm = ring + kStages * kChunkBytes;  // two windows' maxima
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kChunkBytes + 2 * kWinBytes);
   uint64_t* empty = full + kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
-  __shared__ Stat sm_stat[2][kThreads / 32];
-  __shared__ TopList tl;
+  uint64_t* win_full = empty + kStages;  // [2] a window has been read: its maxima, and the row's sums behind its last
+  uint64_t* win_empty = win_full + 2;    // [2] they have been taken
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(win_empty + 2);
+  __shared__ Stat sm_stat[2][kWarps];
+  __shared__ float tm[2][kThreads];  // the threads' maxima over a window
+  __shared__ MergeScratch scratch;
   __shared__ SegOut so;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kThreads / 32);
+      mbar_init(&empty[i], kWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&win_full[i], kWarps);
+      mbar_init(&win_empty[i], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -505,8 +492,13 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
   auto row_of = [&](int64_t n) { return reinterpret_cast<const T*>(a.x) + n * a.row_stride; };
   auto mis_of = [](const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); };
   auto seg_begin = [&](int seg) { return (int)(((int64_t)a.chunks * seg) >> a.seg_bits); };
+  // (A row's alignment may leave it one chunk less; a segment has one at least.)
+  auto seg_end = [&](int seg, int mis) {
+    const int own = (a.V + mis + VE * CV - 1) / (VE * CV);
+    return max(seg_begin(seg) + 1, min(seg_begin(seg + 1), own));
+  };
 
-  if (warp == kThreads / 32) {
+  if (warp == kWarps) {
     // ---------------------------------------------------------------- copies
     int k = 0;  // chunks issued
     bool ok = true;
@@ -514,7 +506,8 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
       const T* row = row_of(item >> a.seg_bits);
       const int seg = (int)item & (a.segs - 1), mis = mis_of(row);
       const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
-      for (int c = seg_begin(seg); c < seg_begin(seg + 1); ++c, ++k) {
+      const int c1 = seg_end(seg, mis);
+      for (int c = seg_begin(seg); c < c1; ++c, ++k) {
         const int st = k % kStages;
         if (k >= kStages &&
             !(ok = ring_wait(&empty[st], ((k / kStages) - 1) & 1, abort_flag, a.status)))
@@ -539,132 +532,161 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) logprobs_kernel(con
     return;
   }
 
-  int k = 0;  // chunks taken
-  int parity = 0;
+  if (warp == kWarps + 1) {
+    // ---------------------------------------------------------------- alternatives, results
+    // A wait that gives up has set the status word; the work runs on (its results
+    // do not count) so that all warps come to their ends.
+    auto target_of = [&](int64_t item) {
+      const int64_t n = item >> a.seg_bits;
+      return item >= items ? -1
+             : a.t64       ? reinterpret_cast<const int64_t*>(a.targets)[n]
+                           : (int64_t)reinterpret_cast<const int32_t*>(a.targets)[n];
+    };
+    auto logit_of = [&](int64_t item, int64_t t) {
+      return t >= 0 && t < a.V ? row_of(item >> a.seg_bits)[t] : T();
+    };
+    int w = 0;  // windows taken
+    int64_t t0 = target_of(blockIdx.x), t1 = target_of(blockIdx.x + (int64_t)gridDim.x);
+    T x0 = logit_of(blockIdx.x, t0);
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+      const int64_t n = item >> a.seg_bits;
+      const int seg = (int)item & (a.segs - 1);
+      const T* row = row_of(n);
+      const int mis = mis_of(row), c1 = seg_end(seg, mis);
+      // The targets and their logits are loaded rows ahead.
+      const int64_t t = t0;
+      const T xt = x0;
+      t0 = t1;
+      x0 = logit_of(item + gridDim.x, t0);
+      t1 = target_of(item + 2 * (int64_t)gridDim.x);
+      unsigned long long best = 0;
+      for (int c = seg_begin(seg);; ++w) {
+        const int buf = w & 1, nch = a.top > 0 ? min(kWin<T>, c1 - c) : c1 - c;
+        ring_wait(&win_full[buf], (w >> 1) & 1, abort_flag, a.status);
+        if (a.top > 0)
+          best = merge_window<T>(best, a.top, row, mis, a.V, wm + buf * kWinBytes, tm[buf], c, nch, scratch, lane);
+        c += nch;
+        Stat s = lane < kWarps ? sm_stat[buf][lane] : Stat{-INFINITY, 0.f, 0.f};  // (read in vain but behind the last)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&win_empty[buf]);
+        if (c < c1) continue;
+        ++w;
+        s = stat_warp(s);
+        if (a.segs > 1) {
+          if (seg > 0) {
+            const uint32_t at = smem_peer(smem_u32(&so.stat[seg]), 0);
+            if (lane == 0) {
+              st_cluster(at, s.m);
+              st_cluster(at + 4, s.s1);
+              st_cluster(at + 8, s.s2);
+            }
+            if (a.top > 0) st_cluster(smem_peer(smem_u32(&so.keys[seg][lane]), 0), best);
+          }
+          __syncwarp();
+          cluster_sync();
+          if (seg > 0) break;
+          const Stat o = lane > 0 && lane < a.segs ? so.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+          s = stat_warp(lane == 0 ? s : o);
+          if (a.top > 0)
+            for (int j = 1; j < a.segs; ++j) best = lane_join(best, so.keys[j][lane], lane);
+        }
+        finish_row<T>(a, n, s, best, t, Cvt<T>::to_f(xt), lane);
+        break;
+      }
+    }
+    return;
+  }
+
+  int k = 0, w = 0;  // chunks, windows taken
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t n = item >> a.seg_bits;
     const int seg = (int)item & (a.segs - 1);
-    const int c0 = seg_begin(seg), c1 = seg_begin(seg + 1);
     const T* row = row_of(n);
     const int mis = mis_of(row);
+    const int c0 = seg_begin(seg), c1 = seg_end(seg, mis);
     const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
     Stat st{-INFINITY, 0.f, 0.f};
-    // Warp 0, which has read the item before's list, starts this one's; the others
-    // touch it behind the first chunk's barrier.
-    if (a.top > 0 && warp == 0) {
-      tl.best[0][lane] = 0;
-      if (lane == 0) tl.pairs = tl.picked = tl.above = tl.ties = tl.cur = 0;
-    }
-    float tm = -INFINITY;  // this thread's maximum over the window
-    int wn = 0;            // chunks of the window so far
+    for (int c = c0; c < c1; ++w) {
+      const int buf = w & 1, end = a.top > 0 ? min(c1, c + kWin<T>) : c1;
+      if (w >= 2) ring_wait(&win_empty[buf], ((w >> 1) - 1) & 1, abort_flag, a.status);
+      T* out = reinterpret_cast<T*>(wm + buf * kWinBytes + threadIdx.x * kWinRow);
+      float top_max = -INFINITY;  // this thread's maximum over the window
 #pragma unroll 1
-    for (int c = c0; c < c1; ++c, ++k) {
-      // A wait that gives up has set the status word; the work runs on (its
-      // results do not count) so that all threads meet at the barriers.
-      const int slot = k % kStages;
-      ring_wait(&full[slot], (k / kStages) & 1, abort_flag, a.status);
-      const uint4* src = reinterpret_cast<const uint4*>(ring + slot * kChunkBytes);
-      auto vec = [&](int i) {
-        const int v = c * CV + i * kThreads + (int)threadIdx.x;
-        return v >= v_lo && v < v_hi ? src[i * kThreads + threadIdx.x] : load_vec<T>(row, v * VE - mis, a.V);
-      };
-      uint4 d[kU];
-      if (c * CV >= v_lo && (c + 1) * CV <= v_hi) {
+      for (; c < end; ++c, ++k) {
+        // A wait that gives up has set the status word; the work runs on (its
+        // results do not count) so that all threads meet at the barriers.
+        const int slot = k % kStages;
+        ring_wait(&full[slot], (k / kStages) & 1, abort_flag, a.status);
+        const uint4* src = reinterpret_cast<const uint4*>(ring + slot * kChunkBytes);
+        auto vec = [&](int i) {
+          const int v = c * CV + i * kThreads + (int)threadIdx.x;
+          return v >= v_lo && v < v_hi ? src[i * kThreads + threadIdx.x] : load_vec<T>(row, v * VE - mis, a.V);
+        };
+        uint4 d[kU];
+        if (c * CV >= v_lo && (c + 1) * CV <= v_hi) {
 #pragma unroll
-        for (int i = 0; i < kU; ++i) d[i] = src[i * kThreads + threadIdx.x];
-      } else {
+          for (int i = 0; i < kU; ++i) d[i] = src[i * kThreads + threadIdx.x];
+        } else {
 #pragma unroll
-        for (int i = 0; i < kU; ++i) d[i] = vec(i);
+          for (int i = 0; i < kU; ++i) d[i] = vec(i);
+        }
+        float cm = vec_max<T>(d[0]);
+#pragma unroll
+        for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
+        if (!(cm <= st.m)) stat_move(st, cm);
+        if (!(fabsf(st.m) >= Far<T>::kMax)) {
+          const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
+          uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
+#pragma unroll
+          for (int i = 0; i < kU; ++i) {
+            float f[VE];
+            unpack_vec<T>(Far<T>::raise(d[i]), f);
+#pragma unroll
+            for (int u = 0; u < VE; u += 2) {
+              const uint64_t t = f2_fma(f2_pack(f[u], f[u + 1]), l2, nm);
+              float t0, t1;
+              f2_unpack(t, t0, t1);
+              const uint64_t e = f2_pack(ex2_approx(t0), ex2_approx(t1));
+              s1[(u >> 1) & 1] = f2_add(s1[(u >> 1) & 1], e);
+              s2[(u >> 1) & 1] = f2_fma(e, t, s2[(u >> 1) & 1]);
+            }
+          }
+          float x, y;
+          f2_unpack(f2_add(s1[0], s1[1]), x, y);
+          st.s1 += x + y;
+          f2_unpack(f2_add(s2[0], s2[1]), x, y);
+          st.s2 += x + y;
+        } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
+          // A maximum near the type's lowest value (a masked row), where m log2e may
+          // overflow and -inf differs from the lowest value; or an infinity.
+#pragma unroll 1
+          for (int i = 0; i < kU; ++i) {
+            float f[VE];
+            unpack_vec<T>(vec(i), f);
+#pragma unroll
+            for (int u = 0; u < VE; ++u) {
+              const float t = (f[u] - st.m) * kLog2e, e = ex2_approx(t);
+              st.s1 += e;
+              st.s2 = fmaf(e, fmaxf(t, -1000.f), st.s2);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
+        if (a.top == 0) continue;
+        *out++ = Cvt<T>::from_f(cm);  // exact: an element's value
+        top_max = max_nan(top_max, cm);
       }
-      float cm = vec_max<T>(d[0]);
-#pragma unroll
-      for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
-      if (!(cm <= st.m)) stat_move(st, cm);
-      if (!(fabsf(st.m) >= Far<T>::kMax)) {
-        const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
-        uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < kU; ++i) {
-          float f[VE];
-          unpack_vec<T>(Far<T>::raise(d[i]), f);
-#pragma unroll
-          for (int u = 0; u < VE; u += 2) {
-            const uint64_t t = f2_fma(f2_pack(f[u], f[u + 1]), l2, nm);
-            float t0, t1;
-            f2_unpack(t, t0, t1);
-            const uint64_t e = f2_pack(ex2_approx(t0), ex2_approx(t1));
-            s1[(u >> 1) & 1] = f2_add(s1[(u >> 1) & 1], e);
-            s2[(u >> 1) & 1] = f2_fma(e, t, s2[(u >> 1) & 1]);
-          }
-        }
-        float x, y;
-        f2_unpack(f2_add(s1[0], s1[1]), x, y);
-        st.s1 += x + y;
-        f2_unpack(f2_add(s2[0], s2[1]), x, y);
-        st.s2 += x + y;
-      } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
-        // A maximum near the type's lowest value (a masked row), where m log2e may
-        // overflow and -inf differs from the lowest value; or an infinity.
-#pragma unroll 1
-        for (int i = 0; i < kU; ++i) {
-          float f[VE];
-          unpack_vec<T>(vec(i), f);
-#pragma unroll
-          for (int u = 0; u < VE; ++u) {
-            const float t = (f[u] - st.m) * kLog2e, e = ex2_approx(t);
-            st.s1 += e;
-            st.s2 = fmaf(e, fmaxf(t, -1000.f), st.s2);
-          }
-        }
+      if (a.top > 0) tm[buf][threadIdx.x] = top_max;
+      if (c == c1) {
+        st = stat_warp(st);
+        if (lane == 0) sm_stat[buf][warp] = st;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[slot]);
-      if (a.top == 0) continue;
-      wm[wn * kThreads + threadIdx.x] = Cvt<T>::from_f(cm);  // exact: an element's value
-      tm = max_nan(tm, cm);
-      if (++wn == kWin<T> || c + 1 == c1) {
-        merge_window<T>(tl, a.top, row, mis, a.V, wm, c + 1 - wn, wn, tm);
-        wn = 0;
-        tm = -INFINITY;
-      }
+      if (lane == 0) mbar_arrive(&win_full[buf]);
     }
-    st = stat_warp(st);
-    if (lane == 0) sm_stat[parity][warp] = st;
-    work_sync();
-    // Warp 0 finishes the item while the others begin the next (they write the
-    // other half of sm_stat, and this half only behind that item's barrier).
-    if (warp == 0) {
-      Stat s = lane < kThreads / 32 ? sm_stat[parity][lane] : Stat{-INFINITY, 0.f, 0.f};
-      s = stat_warp(s);
-      const unsigned long long key = lane < a.top ? tl.best[tl.cur][lane] : 0;
-      if (a.segs == 1) {
-        finish_row<T>(a, n, s, key, lane);
-      } else {
-        if (seg > 0) {
-          const uint32_t at = smem_peer(smem_u32(&so.stat[seg]), 0);
-          if (lane == 0) {
-            st_cluster(at, s.m);
-            st_cluster(at + 4, s.s1);
-            st_cluster(at + 8, s.s2);
-          }
-          if (a.top > 0) st_cluster(smem_peer(smem_u32(&so.keys[seg][lane]), 0), key);
-        }
-        cluster_sync();
-        if (seg == 0) {
-          const Stat o = lane > 0 && lane < a.segs ? so.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-          s = stat_warp(lane == 0 ? s : o);
-          unsigned long long best = key;
-          if (a.top > 0)
-            for (int j = 1; j < a.segs; ++j) best = lane_join(best, so.keys[j][lane], lane);
-          finish_row<T>(a, n, s, best, lane);
-        }
-      }
-      __syncwarp();
-    } else if (a.segs > 1) {
-      cluster_sync();
-    }
-    parity ^= 1;
   }
+  if (a.segs > 1) cluster_sync();
 }
 
 struct BwdArgs {
@@ -809,7 +831,7 @@ template <typename T> int launch_fwd(const FwdArgs& a, cudaStream_t s) {
     attr_set[dev & 63] = true;
   }
   const int64_t grid = a.segs > 1 ? a.N * a.segs : std::min<int64_t>(a.N, (int64_t)kCtasPerSm * num_sms());
-  SCREE_CUDA_TRY(launch_dependent(logprobs_kernel<T>, dim3((unsigned)grid), dim3(kThreads + 32), kRingSmem, s, a.segs, a));
+  SCREE_CUDA_TRY(launch_dependent(logprobs_kernel<T>, dim3((unsigned)grid), dim3(kThreads + 64), kRingSmem, s, a.segs, a));
   count_launch();
   return SCREE_OK;
 }
