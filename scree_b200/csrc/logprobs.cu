@@ -8,24 +8,27 @@
 //
 // Forward: each logit is read from HBM once, and that bounds it.  Persistent CTAs
 // stream rows in chunks of 16 KB: one warp copies them into a ring with bulk
-// copies, running on into the CTA's next row while the other eight finish one, so
-// 3 CTAs keep up to 144 KB per SM in flight.  6,144 x 128,000 in 16 bits: 276 us
-// (5.7 TB/s) without alternatives, 332 (4.7) with four, whose merges the eight
-// warps cannot hide; 4,099 x 65,539 with eight: 152 (3.5: a row is nine chunks
-// here, the last a short one, then a merge); 1 x 131,072 with twenty: 11.6.  Each
-// thread keeps its own maximum, s1 and s2; they are rescaled only when a chunk
-// raises the maximum.  Of few rows each is cut into segments for the CTAs of a
-// cluster, which hand their results to its first CTA through shared memory.
+// copies, running on into the CTA's next row while eight read one, so 3 CTAs keep
+// up to 144 KB per SM in flight.  The eight never meet at a barrier: each thread
+// keeps its own maximum, s1 and s2 (rescaled only when a chunk raises the maximum),
+// and a tenth warp joins them, two rows behind at most.  Of few rows each is cut
+// into segments for the CTAs of a cluster, which hand their results to its first
+// CTA through shared memory.  6,144 x 128,000 in 16 bits: 270 us (5.8 TB/s), with
+// four alternatives 276; 4,099 x 65,539 with eight: 106; 16,384 x 16,384: 115, with
+// four 195 (the tenth warp's pace: 5 us a row); 1 x 131,072 with twenty: 8.4.  (With
+// the eight warps joining and merging at barriers between rows: 276, 332, 152, 178,
+// 318 and 11.6.)
 //
 // Alternatives: a thread notes the maximum of its elements of each chunk (a pair:
-// thread, chunk).  After kWin chunks or at the row's end the k-th largest pair
-// maximum is found; only the k pairs that reach it can hold one of the k best
-// elements, so their elements (k x 32) are read again, from L2, and ranked with
-// the list so far.  That is once per row of up to 131,000 16-bit logits, and the
-// streaming loop pays one store per chunk.  (Pushing elements above a running
-// bound as they stream past cost 4,000 cycles each time a warp met one, twice the
-// time of a chunk.)  Floods of equal values are taken in the order of their
-// indices by a scan that stops when it has enough.
+// thread, chunk), so the streaming loop pays one store a chunk.  After kWin chunks or
+// at the row's end the tenth warp takes the top-th largest of 64 thread maxima as a
+// bound; the few pairs that reach it can hold one of the best elements, and those
+// are read again, from L2, and ranked with the list so far, while the eight go on.
+// That is once per row of up to 131,000 16-bit logits.  (Pushing elements above a
+// running bound as they stream past cost 4,000 cycles each time a warp met one,
+// twice the time of a chunk.)  Equal values are taken in the order of their
+// indices: keys hold both, and a pair whose lowest index is behind the list's last
+// is passed over, so floods of equal values end early.
 //
 // Numerics: sums in fp32, exponents in units of log2 (one FMA and one ex2 per
 // element; the product x log2e is not rounded before m is subtracted).
@@ -153,13 +156,14 @@ __device__ __forceinline__ void stat_move(Stat& s, float to) {
   s.s1 *= w;
   s.m = to;
 }
-__device__ __forceinline__ Stat stat_warp(Stat s) {
+// Joined over groups of W lanes.
+template <int W = 32> __device__ __forceinline__ Stat stat_warp(Stat s) {
   float m = s.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = W / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   stat_move(s, m);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = W / 2; o > 0; o >>= 1) {
     s.s1 += __shfl_xor_sync(0xffffffffu, s.s1, o);
     s.s2 += __shfl_xor_sync(0xffffffffu, s.s2, o);
   }
@@ -209,17 +213,17 @@ struct FwdArgs {
   int* status;
 };
 
-// The row's outputs from its joined statistics; `key` is the lane's alternative, t
+// The row's outputs from its joined statistics (s2: lane 0's); `key` is the lane's alternative, t
 // the target and xt its logit (lane 0).
 template <typename T>
 __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const Stat& s, unsigned long long key,
                                            int64_t t, float xt, int lane) {
   // A row with nothing left (every logit -inf): logp = -inf, H = 0.
   const bool empty = s.m == -INFINITY;
-  const float ls = log2f(s.s1) * kLn2;
+  const float l2 = log2f(s.s1), ls = l2 * kLn2;
   if (lane == 0) {
     if (a.norm != nullptr) a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
-    a.entropy[n] = empty ? 0.f : (log2f(s.s1) - s.s2 / s.s1) * kLn2;
+    a.entropy[n] = empty ? 0.f : (l2 - __fdividef(s.s2, s.s1)) * kLn2;
     float lp = 0.f;  // negative target: no token given
     if (t >= (int64_t)a.V) {
       record_device_error(a.status, SCREE_DEVERR_BAD_INPUT, kSiteTarget);
@@ -260,6 +264,20 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int e0, int V) {
       if (e0 + u >= 0 && e0 + u < V) el[u] = row[e0 + u];
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A vector at element e0 of a row, its elements outside [0, V) replaced by -inf.
+template <typename T> __device__ __forceinline__ uint4 keep_row(const uint4& v, int e0, int V) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t m;
+    if constexpr (sizeof(T) == 4) m = (unsigned)(e0 + j) < (unsigned)V ? 0xFFFFFFFFu : 0u;
+    else m = ((unsigned)(e0 + 2 * j) < (unsigned)V ? 0xFFFFu : 0u) | ((unsigned)(e0 + 2 * j + 1) < (unsigned)V ? 0xFFFF0000u : 0u);
+    r[j] = (w[j] & m) | (neg_inf_word<T>() & ~m);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 template <typename T> constexpr int kWin = 32 / (int)sizeof(T);  // chunks of a window
@@ -314,28 +332,24 @@ __device__ __forceinline__ unsigned long long merge_window(unsigned long long be
   constexpr int VE = Lv<T>::N, CV = kThreads * kU, E = kU * VE, G = kThreads / 32;
   const uint32_t lt = (1u << lane) - 1;
   const int base0 = c0 * CV * VE - mis;  // first element of the window's first thread
-  // A bound from below: the top-th largest of 64 maxima over four threads each (its
-  // upper 16 bits).
-  uint32_t m[G], tau = 0;
+  // A bound from below: the top-th largest of 64 maxima over four threads each.
+  float m[G];  // (-inf of threads without elements)
 #pragma unroll
-  for (int g = 0; g < G; ++g)  // a thread without elements reaches no bound
-    m[g] = base0 + (g * 32 + lane) * VE < V ? order_bits(tm[g * 32 + lane]) : 0u;
+  for (int g = 0; g < G; ++g) m[g] = tm[g * 32 + lane];
+  uint32_t tau;
   {
-    const uint32_t a = max(max(m[0], m[1]), max(m[2], m[3])), b = max(max(m[4], m[5]), max(m[6], m[7]));
-#pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
-      const uint32_t at_least = tau | bit;
-      const int n = __popc(__ballot_sync(0xffffffffu, a >= at_least)) + __popc(__ballot_sync(0xffffffffu, b >= at_least));
-      if (n >= top) tau = at_least;
-    }
+    const uint32_t a = order_bits(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])));
+    const uint32_t b = order_bits(max_nan(max_nan(m[4], m[5]), max_nan(m[6], m[7])));
+    tau = __shfl_sync(0xffffffffu, lane_join(lane_sort(a, lane), lane_sort(b, lane), lane), top - 1);
   }
   unsigned long long kth = __shfl_sync(0xffffffffu, best, top - 1);
   tau = max(tau, (uint32_t)(kth >> 32));
-  const Bound<T> bound(order_value(tau));
+  const float tau_f = order_value(tau);
+  const Bound<T> bound(tau_f);
   int flagged = 0;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    const bool in = m[g] >= tau && m[g] != 0;
+    const bool in = !(m[g] < tau_f);
     const uint32_t b = __ballot_sync(0xffffffffu, in);
     if (in) sc.threads[flagged + __popc(b & lt)] = (uint16_t)(g * 32 + lane);
     flagged += __popc(b);
@@ -417,7 +431,8 @@ __device__ __forceinline__ unsigned long long merge_window(unsigned long long be
     uint32_t pass = 0;
 #pragma unroll
     for (int i = 0; i < kWinRow / 4 - 1; ++i) pass |= bound.reach(w[i]) << i;
-    const int have = f0 + lane < flagged ? min(nch, (V - e0 + CV * VE - 1) / (CV * VE)) : 0;  // chunks with elements
+    // Chunks in which the thread has elements.
+    const int have = f0 + lane < flagged && e0 < V ? min(nch, (V - e0 + CV * VE - 1) / (CV * VE)) : 0;
     pass &= sizeof(T) == 4 ? (1u << have) - 1 : ((1u << ((have + 1) >> 1)) - 1) | ((1u << (have >> 1)) - 1) << 16;
 #pragma unroll 1
     while (__any_sync(0xffffffffu, pass != 0)) {
@@ -486,9 +501,10 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
   // Item = segment of a row; with several segments a CTA has one item, and the
   // segment is its rank in the cluster.
   const int64_t items = a.N * a.segs;
-  // Vectors start at 16-byte boundaries: a row begins `mis` elements into its
-  // first vector; vectors [1 if mis, (V + mis) / VE) lie inside the row and go
-  // through the ring, the two at its ends are read element by element.
+  // Vectors start at 16-byte boundaries: a row begins `mis` elements into its first
+  // one.  A row's vectors go through the ring with what its neighbours have in the
+  // first and the last; only where that would leave the tensor the copying warp
+  // fetches their elements one by one.
   auto row_of = [&](int64_t n) { return reinterpret_cast<const T*>(a.x) + n * a.row_stride; };
   auto mis_of = [](const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); };
   auto seg_begin = [&](int seg) { return (int)(((int64_t)a.chunks * seg) >> a.seg_bits); };
@@ -504,8 +520,9 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
     bool ok = true;
     for (int64_t item = blockIdx.x; lane == 0 && ok && item < items; item += gridDim.x) {
       const T* row = row_of(item >> a.seg_bits);
-      const int seg = (int)item & (a.segs - 1), mis = mis_of(row);
-      const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
+      const int seg = (int)item & (a.segs - 1), mis = mis_of(row), v_end = (a.V + mis + VE - 1) / VE;
+      const int v_lo = row - mis < row_of(0) ? 1 : 0;
+      const int v_hi = row - mis + (int64_t)v_end * VE > row_of(a.N - 1) + a.V ? (a.V + mis) / VE : v_end;
       const int c1 = seg_end(seg, mis);
       for (int c = seg_begin(seg); c < c1; ++c, ++k) {
         const int st = k % kStages;
@@ -513,6 +530,13 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
             !(ok = ring_wait(&empty[st], ((k / kStages) - 1) & 1, abort_flag, a.status)))
           break;
         const int lo = max(c * CV, v_lo), hi = min((c + 1) * CV, v_hi);
+        auto fetch = [&](int v) {
+          T* to = reinterpret_cast<T*>(ring + st * kChunkBytes) + (v - c * CV) * VE;
+          for (int e = max(v * VE - mis, 0); e < min((v + 1) * VE - mis, a.V); ++e) to[e - (v * VE - mis)] = row[e];
+          fence_proxy_async_smem();  // the place's next copy
+        };
+        if (c == 0 && v_lo > 0) fetch(0);
+        if (v_hi < v_end && v_hi >= max(c * CV, v_lo) && v_hi < (c + 1) * CV) fetch(v_hi);
         if (lo < hi) {
           mbar_expect_tx(&full[st], (uint32_t)(hi - lo) * 16);
           bulk_load_1d(ring + st * kChunkBytes + (lo - c * CV) * 16, row + (int64_t)lo * VE - mis,
@@ -571,7 +595,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
         if (lane == 0) mbar_arrive(&win_empty[buf]);
         if (c < c1) continue;
         ++w;
-        s = stat_warp(s);
+        s = stat_warp<kWarps>(s);
         if (a.segs > 1) {
           if (seg > 0) {
             const uint32_t at = smem_peer(smem_u32(&so.stat[seg]), 0);
@@ -586,10 +610,12 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
           cluster_sync();
           if (seg > 0) break;
           const Stat o = lane > 0 && lane < a.segs ? so.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-          s = stat_warp(lane == 0 ? s : o);
+          s = stat_warp<kMaxSegs>(lane == 0 ? s : o);
           if (a.top > 0)
             for (int j = 1; j < a.segs; ++j) best = lane_join(best, so.keys[j][lane], lane);
         }
+        s.m = __shfl_sync(0xffffffffu, s.m, 0);
+        s.s1 = __shfl_sync(0xffffffffu, s.s1, 0);
         finish_row<T>(a, n, s, best, t, Cvt<T>::to_f(xt), lane);
         break;
       }
@@ -597,6 +623,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
     return;
   }
 
+  const int tid = threadIdx.x;
   int k = 0, w = 0;  // chunks, windows taken
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t n = item >> a.seg_bits;
@@ -604,70 +631,74 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
     const T* row = row_of(n);
     const int mis = mis_of(row);
     const int c0 = seg_begin(seg), c1 = seg_end(seg, mis);
-    const int v_lo = mis > 0 ? 1 : 0, v_hi = (a.V + mis) / VE;
+    const int v_end = (a.V + mis + VE - 1) / VE;
     Stat st{-INFINITY, 0.f, 0.f};
     for (int c = c0; c < c1; ++w) {
       const int buf = w & 1, end = a.top > 0 ? min(c1, c + kWin<T>) : c1;
       if (w >= 2) ring_wait(&win_empty[buf], ((w >> 1) - 1) & 1, abort_flag, a.status);
-      T* out = reinterpret_cast<T*>(wm + buf * kWinBytes + threadIdx.x * kWinRow);
+      T* out = reinterpret_cast<T*>(wm + buf * kWinBytes + tid * kWinRow);
       float top_max = -INFINITY;  // this thread's maximum over the window
 #pragma unroll 1
       for (; c < end; ++c, ++k) {
-        // A wait that gives up has set the status word; the work runs on (its
-        // results do not count) so that all threads meet at the barriers.
         const int slot = k % kStages;
         ring_wait(&full[slot], (k / kStages) & 1, abort_flag, a.status);
-        const uint4* src = reinterpret_cast<const uint4*>(ring + slot * kChunkBytes);
-        auto vec = [&](int i) {
-          const int v = c * CV + i * kThreads + (int)threadIdx.x;
-          return v >= v_lo && v < v_hi ? src[i * kThreads + threadIdx.x] : load_vec<T>(row, v * VE - mis, a.V);
-        };
-        uint4 d[kU];
-        if (c * CV >= v_lo && (c + 1) * CV <= v_hi) {
+        const uint4* src = reinterpret_cast<const uint4*>(ring + slot * kChunkBytes) + tid;
+        float cm = -INFINITY;
+        if (c * CV + (tid & ~31) < v_end) {
+          auto vec = [&](int i) {
+            const int e = (c * CV + i * kThreads + tid) * VE - mis, e0 = e - lane * VE;  // of the thread, of the warp
+            if (e0 >= 0 && e0 + 32 * VE <= a.V) return src[i * kThreads];
+            if (e0 >= a.V)
+              return make_uint4(neg_inf_word<T>(), neg_inf_word<T>(), neg_inf_word<T>(), neg_inf_word<T>());
+            return keep_row<T>(src[i * kThreads], e, a.V);
+          };
+          uint4 d[kU];
+          if (c * CV * VE >= mis && (c + 1) * CV * VE <= a.V + mis) {
 #pragma unroll
-          for (int i = 0; i < kU; ++i) d[i] = src[i * kThreads + threadIdx.x];
-        } else {
+            for (int i = 0; i < kU; ++i) d[i] = src[i * kThreads];
+          } else {
 #pragma unroll
-          for (int i = 0; i < kU; ++i) d[i] = vec(i);
-        }
-        float cm = vec_max<T>(d[0]);
-#pragma unroll
-        for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
-        if (!(cm <= st.m)) stat_move(st, cm);
-        if (!(fabsf(st.m) >= Far<T>::kMax)) {
-          const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
-          uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
-#pragma unroll
-          for (int i = 0; i < kU; ++i) {
-            float f[VE];
-            unpack_vec<T>(Far<T>::raise(d[i]), f);
-#pragma unroll
-            for (int u = 0; u < VE; u += 2) {
-              const uint64_t t = f2_fma(f2_pack(f[u], f[u + 1]), l2, nm);
-              float t0, t1;
-              f2_unpack(t, t0, t1);
-              const uint64_t e = f2_pack(ex2_approx(t0), ex2_approx(t1));
-              s1[(u >> 1) & 1] = f2_add(s1[(u >> 1) & 1], e);
-              s2[(u >> 1) & 1] = f2_fma(e, t, s2[(u >> 1) & 1]);
-            }
+            for (int i = 0; i < kU; ++i) d[i] = vec(i);
           }
-          float x, y;
-          f2_unpack(f2_add(s1[0], s1[1]), x, y);
-          st.s1 += x + y;
-          f2_unpack(f2_add(s2[0], s2[1]), x, y);
-          st.s2 += x + y;
-        } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
-          // A maximum near the type's lowest value (a masked row), where m log2e may
-          // overflow and -inf differs from the lowest value; or an infinity.
-#pragma unroll 1
-          for (int i = 0; i < kU; ++i) {
-            float f[VE];
-            unpack_vec<T>(vec(i), f);
+          cm = vec_max<T>(d[0]);
 #pragma unroll
-            for (int u = 0; u < VE; ++u) {
-              const float t = (f[u] - st.m) * kLog2e, e = ex2_approx(t);
-              st.s1 += e;
-              st.s2 = fmaf(e, fmaxf(t, -1000.f), st.s2);
+          for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
+          if (!(cm <= st.m)) stat_move(st, cm);
+          if (!(fabsf(st.m) >= Far<T>::kMax)) {
+            const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
+            uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < kU; ++i) {
+              float f[VE];
+              unpack_vec<T>(Far<T>::raise(d[i]), f);
+#pragma unroll
+              for (int u = 0; u < VE; u += 2) {
+                const uint64_t t = f2_fma(f2_pack(f[u], f[u + 1]), l2, nm);
+                float t0, t1;
+                f2_unpack(t, t0, t1);
+                const uint64_t e = f2_pack(ex2_approx(t0), ex2_approx(t1));
+                s1[(u >> 1) & 1] = f2_add(s1[(u >> 1) & 1], e);
+                s2[(u >> 1) & 1] = f2_fma(e, t, s2[(u >> 1) & 1]);
+              }
+            }
+            float x, y;
+            f2_unpack(f2_add(s1[0], s1[1]), x, y);
+            st.s1 += x + y;
+            f2_unpack(f2_add(s2[0], s2[1]), x, y);
+            st.s2 += x + y;
+          } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
+            // A maximum near the type's lowest value (a masked row), where m log2e may
+            // overflow and -inf differs from the lowest value; or an infinity.
+#pragma unroll 1
+            for (int i = 0; i < kU; ++i) {
+              float f[VE];
+              unpack_vec<T>(vec(i), f);
+#pragma unroll
+              for (int u = 0; u < VE; ++u) {
+                const float t = (f[u] - st.m) * kLog2e, e = ex2_approx(t);
+                st.s1 += e;
+                st.s2 = fmaf(e, fmaxf(t, -1000.f), st.s2);
+              }
             }
           }
         }
@@ -677,7 +708,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
         *out++ = Cvt<T>::from_f(cm);  // exact: an element's value
         top_max = max_nan(top_max, cm);
       }
-      if (a.top > 0) tm[buf][threadIdx.x] = top_max;
+      if (a.top > 0) tm[buf][tid] = top_max;
       if (c == c1) {
         st = stat_warp(st);
         if (lane == 0) sm_stat[buf][warp] = st;

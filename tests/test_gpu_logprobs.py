@@ -295,3 +295,49 @@ def test_refusals(cuda):
     st = _lib.device_status()
     assert st >> 16 == _lib.DEVERR_BAD_INPUT and st & 0xFFFF == 50
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 3, 9, 2047, 8193, 16391])
+def test_neighbouring_rows_do_not_matter(cuda, dtype, V):
+    """Rows of odd lengths at every alignment, their neighbours NaN, the tensor between NaN."""
+    from scree_b200.kernels import native
+
+    for shift in range(0, 8, 3):
+        for N in (1, 2, 5):
+            x, t = _logits(N, V, dtype, cuda, seed=shift + N)
+            k = min(V, 7)
+            buf = torch.full((shift + 2 * N * V + 9,), float("nan"), dtype=dtype, device=cuda)
+            rows = buf[shift:shift + 2 * N * V].view(N, 2, V)[:, 0]  # row stride 2 V
+            rows.copy_(x)
+            alone = native.token_logprobs(x, t, top_k=k)
+            got = native.token_logprobs(rows, t, top_k=k)
+            _check(x, t, k, got, x.double())
+            assert torch.equal(got.top_ids, alone.top_ids)
+            whole = buf[shift:shift + 2 * N * V].view(2 * N, V)      # every other row is NaN
+            two = native.token_logprobs(whole, t.repeat_interleave(2), top_k=k)
+            assert two.logp[1::2].isnan().all()
+            _check(x, t, k, native.TokenLogprobs(*(r[::2] for r in two)), x.double())
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("kept", [0, 1, 5, 31, 40])
+def test_rows_masked_but_for_a_few_tokens(cuda, kept):
+    """Constrained decoding: all logits -inf but a few; the rest rank by index."""
+    from scree_b200.kernels import native
+
+    N, V, k = 6, 150001, 32
+    x = torch.full((N, V), -float("inf"), dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator().manual_seed(kept)
+    for n in range(N):
+        at = torch.randperm(V, generator=g)[:kept].to(cuda)
+        x[n, at] = torch.randn(kept, generator=g).to(torch.bfloat16).to(cuda)
+    t = x.float().argmax(1)
+    got = native.token_logprobs(x, t, top_k=k)
+    order = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(got.top_ids, order)
+    if kept:
+        _check(x, t, k, got, x.double())
+    else:
+        assert (got.logp == -float("inf")).all() and (got.entropy == 0).all()
+    assert _status() == 0
