@@ -282,13 +282,15 @@ template <typename T> __device__ __forceinline__ uint4 keep_row(const uint4& v, 
 
 template <typename T> constexpr int kWin = 32 / (int)sizeof(T);  // chunks of a window
 
-// A bound from below as a value of type T (NaN: every value reaches it), and which
-// of a word's elements reach it (NaN does): bit 0, and bit 16 of 16-bit types.
+// A bound as a value of type T, and which of a word's elements reach it, which are
+// beyond it (NaN always, and everything if it is NaN): bit 0, and bit 16 of 16-bit
+// types.
 template <typename T> struct Bound;
 template <> struct Bound<float> {
   float v;
   __device__ __forceinline__ explicit Bound(float f) : v(f) {}
   __device__ __forceinline__ uint32_t reach(uint32_t w) const { return __uint_as_float(w) < v ? 0u : 1u; }
+  __device__ __forceinline__ uint32_t beyond(uint32_t w) const { return __uint_as_float(w) <= v ? 0u : 1u; }
 };
 template <> struct Bound<__nv_bfloat16> {
   __nv_bfloat162 v;
@@ -296,12 +298,18 @@ template <> struct Bound<__nv_bfloat16> {
   __device__ __forceinline__ uint32_t reach(uint32_t w) const {
     return ~__hlt2_mask(*reinterpret_cast<__nv_bfloat162*>(&w), v) & 0x00010001u;
   }
+  __device__ __forceinline__ uint32_t beyond(uint32_t w) const {
+    return ~__hle2_mask(*reinterpret_cast<__nv_bfloat162*>(&w), v) & 0x00010001u;
+  }
 };
 template <> struct Bound<__half> {
   __half2 v;
   __device__ __forceinline__ explicit Bound(float f) : v(__half2half2(__float2half_rd(f))) {}
   __device__ __forceinline__ uint32_t reach(uint32_t w) const {
     return ~__hlt2_mask(*reinterpret_cast<__half2*>(&w), v) & 0x00010001u;
+  }
+  __device__ __forceinline__ uint32_t beyond(uint32_t w) const {
+    return ~__hle2_mask(*reinterpret_cast<__half2*>(&w), v) & 0x00010001u;
   }
 };
 // Bit b of the words' reach(), word w shifted by w: which element of them it is.
@@ -397,9 +405,12 @@ __device__ __forceinline__ unsigned long long merge_window(unsigned long long be
                   bound.reach(v[i].w) << (4 * i + 3);
       }
       // Pairs with many such elements by the whole warp.
-      for (uint32_t many = __ballot_sync(0xffffffffu, __popc(pass) >= kManyKeys); many != 0; many &= many - 1) {
+      uint32_t left = 0xFFFFFFFFu;  // lanes not looked at yet
+      while (true) {
+        const uint32_t many = __ballot_sync(0xffffffffu, __popc(pass) >= kManyKeys && most > kth) & left;
+        if (many == 0) break;
         const int src = __ffs(many) - 1;
-        if (__shfl_sync(0xffffffffu, most, src) <= kth) continue;
+        left = ~((2u << src) - 1);
         const int e = __shfl_sync(0xffffffffu, e0, src) + lane / VE * kThreads * VE + lane % VE;
         unsigned long long key = lane < E && e >= 0 && e < V ? order_key(Cvt<T>::to_f(row[e]), (uint32_t)e) : 0;
         if (key <= kth) key = 0;
@@ -428,9 +439,12 @@ __device__ __forceinline__ unsigned long long merge_window(unsigned long long be
   for (int f0 = 0; f0 < flagged; f0 += 32) {
     const int th = sc.threads[min(f0 + lane, flagged - 1)], e0 = base0 + th * VE;
     const uint32_t* w = reinterpret_cast<const uint32_t*>(wm + th * kWinRow);
+    // Behind the list's last an equal value does not count.
+    const Bound<T> last(order_value((uint32_t)(kth >> 32)));
+    const bool behind = kth != 0 && e0 > (int)(0xFFFFFFFFu - (uint32_t)kth);
     uint32_t pass = 0;
 #pragma unroll
-    for (int i = 0; i < kWinRow / 4 - 1; ++i) pass |= bound.reach(w[i]) << i;
+    for (int i = 0; i < kWinRow / 4 - 1; ++i) pass |= (behind ? last.beyond(w[i]) : bound.reach(w[i])) << i;
     // Chunks in which the thread has elements.
     const int have = f0 + lane < flagged && e0 < V ? min(nch, (V - e0 + CV * VE - 1) / (CV * VE)) : 0;
     pass &= sizeof(T) == 4 ? (1u << have) - 1 : ((1u << ((have + 1) >> 1)) - 1) | ((1u << (have >> 1)) - 1) << 16;
@@ -447,7 +461,7 @@ __device__ __forceinline__ unsigned long long merge_window(unsigned long long be
         sc.queue_max[queued + __popc(b & lt)] = o;
       }
       queued += __popc(b);
-      if (queued > 32) drain();
+      if (queued >= 32) drain();
     }
   }
   if (queued > 0) drain();
@@ -828,12 +842,14 @@ int64_t row_vecs(int64_t V, int dtype) {
   return (V + ve - 1 + ve - 1) / ve;
 }
 int64_t row_chunks(int64_t V, int dtype) { return (row_vecs(V, dtype) + kThreads * kU - 1) / (kThreads * kU); }
-// A CTA per row once there are four rounds of them; fewer rows are cut so that
-// there are about as many segments.
+// Rows are cut while the segments' CTAs still have an SM each.  Measured (us; bf16,
+// eight alternatives; 1 / 2 / 4 / 8 segments): 131,072 logits, 1 row 14.2 / 10.6 / 8.6
+// / 8.0, 64 rows 14.3 / 11.5 / 11.4 / 16.2, 128 rows 14.7 / 15.5 / 19.2 / 23.9, 444
+// rows 27 / 33 / 49 / 78; 32,000 logits, 1 row 7.9 / 7.4 / 7.2, 128 rows 8.3 / 9.2 /
+// 14.0, 1,300 rows 24 / 49 / 88.
 int row_segs(int64_t N, int64_t V, int dtype) {
-  const int64_t want = 4 * kCtasPerSm * (int64_t)num_sms();
   int segs = 1;
-  while (segs < kMaxSegs && N * segs < want && 2 * segs <= row_chunks(V, dtype)) segs *= 2;
+  while (segs < kMaxSegs && 2 * N * segs <= num_sms() && 2 * segs <= row_chunks(V, dtype)) segs *= 2;
   return segs;
 }
 constexpr int kNV = 8;  // vectors of a thread, backward
