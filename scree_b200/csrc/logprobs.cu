@@ -749,9 +749,29 @@ struct BwdArgs {
   void* dx;                                 // (N, V) contiguous
 };
 
+// The 16 bytes of a and b (the 16 behind a) from byte `bytes` < 16 on.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int bytes) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (bytes & 8) {
+#pragma unroll
+    for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+  }
+  const int bits = (bytes & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
 // dx = -p (gs + gH (H + log p)), then the given token and the alternatives.
 // HBM-bound: one read and one write of each logit; 6,144 x 128,000 in 16 bits: 530 us,
-// 5.9 TB/s.
+// 5.9 TB/s (16 vectors a thread: 700, 4: 549; plain loads: 542).  Where a row begins
+// at another place of a 16-byte block than dx's does (rows of a padded vocabulary),
+// 16-bit types are stored in dx's vectors, each put together from two of the row's:
+// 8,192 x 50,257 of 50,304 461 us (element by element 978; without padding 324); fp32
+// element by element: 4,096 rows 300 (in vectors 329; without padding 258).
 template <typename T, int NV>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a) {
   constexpr int VE = Lv<T>::N;
@@ -760,12 +780,31 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   const int slice = blockIdx.x % (unsigned)a.slices;
   const T* row = reinterpret_cast<const T*>(a.x) + n * a.row_stride;
   T* out = reinterpret_cast<T*>(a.dx) + n * (int64_t)a.V;
-  const int mis = (int)(((uintptr_t)row & 15) / sizeof(T));
-  const bool same = (((uintptr_t)row ^ (uintptr_t)out) & 15) == 0;
+  constexpr bool kByRow = sizeof(T) == 4;  // vectors of the row, not of dx
+  const int at = (int)(((uintptr_t)row & 15) / sizeof(T));
+  const int mis = kByRow ? at : (int)(((uintptr_t)out & 15) / sizeof(T));
+  const int k = (at - mis) & (VE - 1);  // where dx's vectors begin in the row's
+  const bool same = !kByRow || (((uintptr_t)row ^ (uintptr_t)out) & 15) == 0;
   const int v0 = slice * kThreads * NV;  // first vector of the slice
   uint4 d[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) d[i] = load_vec<T>(row, (v0 + i * kThreads + (int)threadIdx.x) * VE - mis, a.V);
+  for (int i = 0; i < NV; ++i) {
+    const int e = (v0 + i * kThreads + (int)threadIdx.x) * VE - mis - k;
+    d[i] = e >= 0 && e + VE <= a.V ? __ldcs(reinterpret_cast<const uint4*>(row + e)) : load_vec<T>(row, e, a.V);
+  }
+  if (!kByRow && k != 0) {  // the rest of a vector is in the next lane's
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint4 b;
+      b.x = __shfl_down_sync(0xffffffffu, d[i].x, 1);
+      b.y = __shfl_down_sync(0xffffffffu, d[i].y, 1);
+      b.z = __shfl_down_sync(0xffffffffu, d[i].z, 1);
+      b.w = __shfl_down_sync(0xffffffffu, d[i].w, 1);
+      if (lane == 31) b = load_vec<T>(row, (v0 + i * kThreads + (int)threadIdx.x + 1) * VE - mis - k, a.V);
+      d[i] = shifted(d[i], b, k * (int)sizeof(T));
+    }
+  }
   // The given token and the alternatives as one list of (index, weight): entry 0
   // is the target, entry 1 + j alternative j; index -1 has no weight.
   auto entry = [&](int j, int64_t& idx) -> float {

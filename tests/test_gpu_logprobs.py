@@ -341,3 +341,28 @@ def test_rows_masked_but_for_a_few_tokens(cuda, kept):
     else:
         assert (got.logp == -float("inf")).all() and (got.entropy == 0).all()
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [5, 1003, 8192])
+def test_gradient_of_rows_at_every_alignment(cuda, dtype, V):
+    """dx is contiguous; the logits' rows begin anywhere in their 16-byte blocks, NaN between them."""
+    from scree_b200.kernels import native
+
+    N = 9
+    x, t = _logits(N, V, dtype, cuda, seed=V)
+    g = torch.Generator().manual_seed(1)
+    gl, gh, gt = (torch.randn(s, generator=g).to(cuda) for s in ((N,), (N,), (N, 2)))
+    want, tol = _grad_ref(x.double(), t, 2, gl.double(), gh.double(), gt.double())
+    tiny = 2.0**-25 if dtype == torch.float16 else 0.0
+    for pad in range(0, 9):
+        for shift in (0, 3):
+            buf = torch.full((shift + N * (V + pad),), float("nan"), dtype=dtype, device=cuda)
+            rows = buf[shift:].view(N, V + pad)[:, :V]
+            rows.copy_(x)
+            y = rows.detach().requires_grad_(True)
+            r = native.token_logprobs_autograd(y, t, 2)
+            torch.autograd.backward([r.logp, r.entropy, r.top_logp], [gl, gh, gt])
+            err = (y.grad.double() - want).abs()
+            assert (err <= tol + HALF_ULP[dtype] * (want.abs() + tol) + tiny).all(), (pad, shift)
+    assert _status() == 0
