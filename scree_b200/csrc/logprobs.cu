@@ -156,11 +156,14 @@ __device__ __forceinline__ void stat_move(Stat& s, float to) {
   s.s1 *= w;
   s.m = to;
 }
-// Joined over groups of W lanes.
+__device__ __forceinline__ float max_nan_warp(float v) {
+  float d;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
+// Joined over the first W lanes (in lane 0; the others empty, or W = 32: in all).
 template <int W = 32> __device__ __forceinline__ Stat stat_warp(Stat s) {
-  float m = s.m;
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float m = max_nan_warp(s.m);
   stat_move(s, m);
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) {
@@ -628,7 +631,6 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
           if (a.top > 0)
             for (int j = 1; j < a.segs; ++j) best = lane_join(best, so.keys[j][lane], lane);
         }
-        s.m = __shfl_sync(0xffffffffu, s.m, 0);
         s.s1 = __shfl_sync(0xffffffffu, s.s1, 0);
         finish_row<T>(a, n, s, best, t, Cvt<T>::to_f(xt), lane);
         break;
