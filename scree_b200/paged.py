@@ -52,8 +52,6 @@ class PagedCache:
     _pools: Any = field(default=None, repr=False, compare=False)
 
     def __post_init__(self) -> None:
-        if self._pools is not None:
-            return  # derived from a checked cache
         for name in ("k", "v", "table", "lengths", "refs"):
             _require_cuda(getattr(self, name), "PagedCache")
         if self.k.ndim != 5 or self.k.shape != self.v.shape or self.k.dtype != self.v.dtype:
@@ -115,7 +113,9 @@ def _book_call(cache: PagedCache, fn, name: str, *args) -> PagedCache:
     rc = fn(ctypes.byref(book), *args, *pools.work, _lib.stream_ptr(pools.device))
     if rc:
         _lib.check(rc, name)
-    return PagedCache(cache.k, cache.v, table, lengths, refs, cache._work, pools)
+    out = object.__new__(PagedCache)  # nothing to check: the same pools, workspace and shapes
+    out.__dict__.update(cache.__dict__, table=table, lengths=lengths, refs=refs)
+    return out
 
 
 def paged_reserve(cache: PagedCache, slots, counts) -> PagedCache:
@@ -259,7 +259,7 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     if sd != 1 or sr % 8 or sh % 8 or sr * sh == 0 or qt.data_ptr() % 16:
         qt = qt.clone(memory_format=torch.contiguous_format)  # contiguous() would keep a misaligned base
         sr, sh, _ = qt.stride()
-    out = torch.empty((T, H, D), dtype=dtype, device=dev)
+    out = torch.empty_like(qt, memory_format=torch.contiguous_format)  # (half the time of empty)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T:
         lib = _lib.load()
