@@ -524,9 +524,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_accept_kernel(const Book b,
   // One warp per entry: lanes read the path and the draft's pages side by side.
   // The last eight warps copy refs meanwhile.
   const int lane = threadIdx.x & 31;
-  constexpr int kCopiers = 8, kCheckers = kPlanThreads / 32 - kCopiers;
-  if (threadIdx.x >> 5 >= kCheckers) copy_and_count(b, false, (threadIdx.x >> 5) - kCheckers, kCopiers);
-  for (int i = threadIdx.x >> 5; i < n && threadIdx.x >> 5 < kCheckers; i += kCheckers) {
+  constexpr int kCopyWarps = 8, kCheckWarps = kPlanThreads / 32 - kCopyWarps;
+  if (threadIdx.x >> 5 >= kCheckWarps) copy_and_count(b, false, (threadIdx.x >> 5) - kCheckWarps, kCopyWarps);
+  for (int i = threadIdx.x >> 5; i < n && threadIdx.x >> 5 < kCheckWarps; i += kCheckWarps) {
     const int s = slots[i];
     if ((unsigned)s >= (unsigned)b.S) continue;  // reported above
     const int64_t len = b.lengths[s], m = drafted[i];
