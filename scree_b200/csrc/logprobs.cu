@@ -31,7 +31,7 @@
 // is passed over, so floods of equal values end early.
 //
 // Numerics: sums in fp32, exponents in units of log2 (one FMA and one ex2 per
-// element; the product x log2e is not rounded before m is subtracted).
+// element; the product x log2e is not rounded before m is subtracted; see kFar).
 #include <algorithm>
 #include "common.cuh"
 #include "sm100.cuh"
@@ -100,12 +100,15 @@ template <typename T> __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
-// -inf must not meet its own weight, 0 * -inf = NaN: elements below kLow are
-// raised to it, two at a time for the 16-bit types.  With |m| < kMax their weight
+// x log2e - m log2e in one FMA rounds m log2e first, which is worth 2^-24 |m|: of a
+// maximum of 1024 and more in magnitude (a row, or all that a thread has seen of it,
+// masked with a large number) x - m is taken first.
+constexpr float kFar = 1024.f;
+// -inf must not meet its own weight, 0 * -inf = NaN: elements near the
+// type's lowest value are raised to `low`, two at a time for the 16-bit types.  With |m| < kFar their weight
 // is 0 either way and (x - m) log2e is finite.  NaN stays.
 template <typename T> struct Far;
 template <> struct Far<__nv_bfloat16> {
-  static constexpr float kMax = 1e36f;
   static __device__ __forceinline__ uint32_t two(uint32_t w) {
     const uint32_t low = 0xFE96FE96u;  // -9.97e37
     const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low));
@@ -114,7 +117,6 @@ template <> struct Far<__nv_bfloat16> {
   static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w)); }
 };
 template <> struct Far<__half> {
-  static constexpr float kMax = 60000.f;
   static __device__ __forceinline__ uint32_t two(uint32_t w) {
     const uint32_t low = 0xFBFFFBFFu;  // -65504
     const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&w), *reinterpret_cast<const __half2*>(&low));
@@ -123,7 +125,6 @@ template <> struct Far<__half> {
   static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w)); }
 };
 template <> struct Far<float> {
-  static constexpr float kMax = 1e36f;
   static __device__ __forceinline__ uint32_t one(uint32_t w) { return __float_as_uint(max_nan(__uint_as_float(w), -1e38f)); }
   static __device__ __forceinline__ uint4 raise(const uint4& v) { return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w)); }
 };
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
 #pragma unroll
           for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
           if (!(cm <= st.m)) stat_move(st, cm);
-          if (!(fabsf(st.m) >= Far<T>::kMax)) {
+          if (!(fabsf(st.m) >= kFar)) {
             const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
             uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
 #pragma unroll
@@ -703,8 +704,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
             f2_unpack(f2_add(s2[0], s2[1]), x, y);
             st.s2 += x + y;
           } else if (st.m != -INFINITY) {  // (nothing but -inf so far, or no element in the chunk)
-            // A maximum near the type's lowest value (a masked row), where m log2e may
-            // overflow and -inf differs from the lowest value; or an infinity.
+            // A far maximum (-inf differs from the lowest value here), or an infinity.
 #pragma unroll 1
             for (int i = 0; i < kU; ++i) {
               float f[VE];
@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   const bool empty = nm.x == -INFINITY;  // nothing left in the row: no gradient
   const float base = sm_gs + gh * a.entropy[n];
   const float l2 = (nm.x + nm.y) * kLog2e, s2 = nm.y * kLog2e;
-  const bool far = fabsf(nm.x) >= 1e37f;  // the product with log2e may overflow (rows of the lowest value)
+  const bool far = fabsf(nm.x) >= kFar;
   auto grad = [&](float x) {
     const float d2 = far ? fmaf(x - nm.x, kLog2e, -s2) : fmaf(x, kLog2e, -l2);  // log2 p
     // The bound only matters at p = 0, where it keeps 0 * inf out.

@@ -366,3 +366,32 @@ def test_gradient_of_rows_at_every_alignment(cuda, dtype, V):
             err = (y.grad.double() - want).abs()
             assert (err <= tol + HALF_ULP[dtype] * (want.abs() + tol) + tiny).all(), (pad, shift)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e30, 3000.0])
+def test_rows_masked_with_large_numbers(cuda, dtype, mask):
+    """Whole rows, and all that a thread reads before a row's last quarter, at one large number."""
+    from scree_b200.kernels import native
+
+    if dtype == torch.float16 and abs(mask) > 6e4:
+        mask = -6e4
+    N, V, k = 4, 30011, 6
+    x, t = _logits(N, V, dtype, cuda, seed=11)
+    x[:, :3 * V // 4] = mask
+    x[1] = mask                      # a whole row
+    x[2, 5] = 2.0                    # one token early on
+    y = x.detach().requires_grad_(True)
+    got = native.token_logprobs_autograd(y, t, k)
+    _check(x, t, k, native.TokenLogprobs(*(r.detach() for r in got)), x.double())
+    # The row of equal values is uniform whatever they are.
+    flat = native.TokenLogprobs(*(r.detach()[1:2] for r in got))
+    assert abs(flat.logp.item() + np.log(V)) <= 2.0**-15 and abs(flat.entropy.item() - np.log(V)) <= 2.0**-12
+    g = torch.Generator().manual_seed(2)
+    gl, gh, gt = (torch.randn(s, generator=g).to(cuda) for s in ((N,), (N,), (N, k)))
+    torch.autograd.backward([got.logp, got.entropy, got.top_logp], [gl, gh, gt])
+    want, tol = _grad_ref(x.double(), t, k, gl.double(), gh.double(), gt.double())
+    tiny = 2.0**-25 if dtype == torch.float16 else 0.0
+    err = (y.grad.double() - want).abs()
+    assert (err <= tol + HALF_ULP[dtype] * (want.abs() + tol) + tiny).all()
+    assert _status() == 0
