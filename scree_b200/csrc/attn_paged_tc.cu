@@ -477,10 +477,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int tile = split ? 2 * j + x : j;
         const int k0 = (e.t0 + tile) * BN;
         const bool edge = k0 + BN > e.c0;
+        ok = wait(&s_full[x], sc + j);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         if (edge) {
           // V row r of the tile: cleared past the end; of a drafted token, without
           // its infinities and NaN.  Both tiles' warps do this, each before it lets
           // its product start; whoever clears an element has set the mark first.
+          // The scores come first: their MMA is issued behind the products of two
+          // tiles earlier (or of the pieces before), which have taken every V tile up
+          // to there, so the place's last fill, three tiles back, has landed and the
+          // parity names this tile's phase alone.
           const int vpos = vc + tile, st = vpos % C::VSTAGES;
           ok = wait(&v_full[st], vpos / C::VSTAGES);
           if (!__all_sync(0xffffffffu, ok)) {
@@ -509,12 +519,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async_smem();
         }
-        ok = wait(&s_full[x], sc + j);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
         float s[BN];
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) tmem_ld32(col_s + c * 32, *reinterpret_cast<float(*)[32]>(&s[c * 32]));
