@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mc = mx * p.sl2;
         alpha[r] = 1.f;
         if (mc > m[r] + 8.f) {
-          alpha[r] = ex2_approx(m[r] - mc);
+          alpha[r] = ex2_weight(m[r] - mc);
           m[r] = mc;
           need = true;
         }
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, o));
       m2 = fmaxf(m2, mx);
-      const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_approx(mx - ref), wt = ex2_approx(ml.x - ref);
+      const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_weight(mx - ref), wt = ex2_weight(ml.x - ref);
       mx = m2;
       sum = sum * scale + wt * ml.y;  // (a lane's own pieces)
 #pragma unroll
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = ex2_approx(sm_ml[w].x - ref);
+        const float f = ex2_weight(sm_ml[w].x - ref);
         sum = fmaf(f, sm_ml[w].y, sum);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(f, sm_o[w][lane * E + e], acc[e]);

@@ -176,6 +176,11 @@ __device__ __forceinline__ unsigned long long paged_visible(const PagedParams& p
   return left >= N ? v : left <= 0 ? 0ull : v & ((1ull << left) - 1);
 }
 
+// 2^x, x <= 0, as the weight of what has been summed so far.  It is never 0: an
+// infinity that a row has taken in stays one (0 * inf = NaN), whatever comes behind it
+// and wherever the run is cut.  2^-149 of a finite sum is below its rounding.
+__device__ __forceinline__ float ex2_weight(float x) { return fmaxf(ex2_approx(x), __uint_as_float(1u)); }
+
 // All ones in the exponent: infinity or NaN, of either half of a word.
 template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   constexpr uint32_t E = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;

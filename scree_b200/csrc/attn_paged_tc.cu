@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool need = false;
         if (m_cand > m_used + 8.0f) {
           need = true;
-          alpha = ex2_approx(m_used - m_cand);
+          alpha = ex2_weight(m_used - m_cand);
           m_used = m_cand;
         }
         const float m_eff = m_used == -INFINITY ? 0.f : m_used;
@@ -617,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();
           mbar_arrive(ml_free);
           const float m = fmaxf(m_used, o.x), ref = m == -INFINITY ? 0.f : m;
-          fa = ex2_approx(m_used - ref);
-          fb = ex2_approx(o.x - ref);
+          fa = ex2_weight(m_used - ref);
+          fb = ex2_weight(o.x - ref);
           l = fa * l + fb * o.y;
           m_used = m;
         }
@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
       for (int e = 0; e < E; ++e) v[j][e] = po[(part * (D / 4) + warp * E + e) * BM + r];
     }
     const float m2 = fmaxf(mx, fmaxf(ml[0].x, ml[1].x));
-    const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_approx(mx - ref);
+    const float ref = m2 == -INFINITY ? 0.f : m2, scale = ex2_weight(mx - ref);
     mx = m2;
     sum *= scale;
 #pragma unroll
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_tc_join_kernel(con
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       if (j0 + j >= np) continue;
-      const float f = ex2_approx(ml[j].x - ref);
+      const float f = ex2_weight(ml[j].x - ref);
       sum = fmaf(f, ml[j].y, sum);
 #pragma unroll
       for (int e = 0; e < E; ++e) {

@@ -32,3 +32,40 @@ def test_masked_tiles_of_long_and_short_pieces(cuda, D, dtype):
         again, lse2 = run()
         assert torch.equal(again.values, out.values) and torch.equal(lse2, lse)
     assert _status() == 0
+
+
+def _far_apart(cuda, news, D, dtype, low, seed=2):
+    """Sequences without context whose tokens before `low` (of the long ones) have scores of
+    about -96 and infinities in V, the others +96: 2^-277 apart, below the smallest float."""
+    cache, slots, hs = _make(cuda, news, 16, 1, D, dtype, seed=seed)
+    for s, n in zip(hs, news):
+        if n <= low:
+            continue
+        pos = torch.arange(n, device=cuda)
+        ids = cache.table[int(s)].long()[pos // 16]
+        b = (96.0 / D**0.5) * torch.where(pos < low, -1.0, 1.0)
+        cache.k[0, ids, 0, pos % 16] = b[:, None].to(dtype).expand(n, D)
+        cache.v[0, ids[3], 0, 3, :2] = float("inf")
+        cache.v[0, ids[low - 1], 0, (low - 1) % 16, 2] = float("-inf")
+    q = torch.ones((sum(news), 1, D), dtype=dtype, device=cuda)
+    return cache, slots, hs, q
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,news,low", [
+    (64, [40, 1, 1, 1], 32), (128, [20, 1], 16), (64, [40] * 200 + [1] * 330, 32),  # single rows: cut at each group; runs
+    (128, [300], 128), (64, [300], 128), (128, [300] * 40, 128)])                    # tiles of 128: cut at each tile; runs
+def test_visible_infinities_do_not_depend_on_the_cut(cuda, D, news, low, dtype):
+    """An infinity of a drafted token's V reaches the rows that see it, however small its weight."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+
+    cache, slots, hs, q = _far_apart(cuda, news, D, dtype, low)
+    offs = _i32(np.concatenate([[0], np.cumsum(news)]).tolist(), cuda)
+    out, lse = paged.paged_attention(scree.Array(q, offs), cache, 0, slots, return_lse=True)
+    ref = _reference(q, cache, 0, hs, news, news, _causal(news))
+    assert np.isposinf(ref[0][low:news[0], 0, :2]).all() and np.isneginf(ref[0][low:news[0], 0, 2]).all()
+    _compare(out.values, lse, ref)
+    got = out.values.float().cpu().numpy()
+    assert np.array_equal(np.isposinf(got), np.isposinf(ref[0])) and np.array_equal(np.isneginf(got), np.isneginf(ref[0]))
+    assert _status() == 0
