@@ -625,25 +625,67 @@ __device__ __forceinline__ int64_t warp_find_seq(const void* offs, int is64, int
   return lo;
 }
 
+// Up to so many entries each block of a write looks for a slot that is named twice;
+// of more, one block does in a launch of its own.  One token an entry, by the blocks /
+// by a launch (us; neither: 3.5, 3.9, 6.7, 29): 256 entries 3.8 / 4.9, 1,024 5.0 / 5.6,
+// 4,096 13.3 / 9.3, 16,384 107 / 35.
+constexpr int64_t kCompareEntries = 1024;
+
+// Records that two entries with tokens name one slot; by one block, ahead of the write.
+__global__ void __launch_bounds__(kPlanThreads)
+    check_entries_kernel(const int32_t* slots, const void* offs, int is64, int64_t B, int S, int* status) {
+  __shared__ SlotSet set;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  for (int i = threadIdx.x; i < kMaxSlots / 32; i += blockDim.x) set.bits[i] = 0;
+  __syncthreads();
+  bool twice = false;
+  constexpr int C = 4;  // loads under way
+  for (int64_t i0 = threadIdx.x; i0 < B; i0 += C * kPlanThreads) {
+    int s[C];
+    bool some[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = i0 + c * kPlanThreads;
+      s[c] = i < B ? slots[i] : -1;
+      some[c] = i < B && load_offset(offs, is64, i + 1) > load_offset(offs, is64, i);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      // (Neighbouring slots in words of their own.)
+      const uint32_t bit = 1u << ((unsigned)s[c] / (kMaxSlots / 32) & 31);
+      if ((unsigned)s[c] < (unsigned)S && some[c])
+        twice |= (atomicOr(&set.bits[s[c] % (kMaxSlots / 32)], bit) & bit) != 0;
+    }
+  }
+  if (__syncthreads_or(twice) && threadIdx.x == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
+}
+
 // One warp per token: its K and V rows.  The rows of entry b are the last
 // offs[b+1] - offs[b] of its slot.  The first loads of the rows are under way
 // while the chain offsets -> slot -> length -> page id finds where they go.
-// 16,384 tokens of 8 x 128 16-bit elements: 23.3 us, 5.8 TB/s; 4,096: 7.6; six: 3.0,
-// which is the chain.
+// Entries with tokens that name one slot would write the same rows: none of them
+// does.  The block's threads look for such entries side by side, behind the loads of
+// the chain.
+// 64 entries of 256 tokens of 8 x 128 16-bit elements: 23.3 us, 5.8 TB/s; of 64: 6.7;
+// one of six: 2.9, which is the chain.
 template <int W>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     paged_write_kernel(const Pools pl, int layer, const char* k, int64_t k_rb, int64_t k_hb, const char* v,
                        int64_t v_rb, int64_t v_hb, const void* offs, int is64, int64_t B, int64_t T,
                        const int32_t* slots, const int32_t* table, const int32_t* lengths, int S, int M, int P,
                        int page, int* status) {
   using V = typename Vec<W>::T;
+  constexpr int kWarps = kThreads / 32;
+  __shared__ int sm_slot[kWarps], sm_entry[kWarps];
+  __shared__ uint32_t sm_twice;  // of the warps: their slot is another entry's too
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  if (status != nullptr && *reinterpret_cast<volatile int*>(status) != 0) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (t >= T) return;
-  const unsigned vpr = (unsigned)(pl.row_bytes / W), all = vpr * (unsigned)pl.H;
+  const bool stopped = status != nullptr && *reinterpret_cast<volatile int*>(status) != 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+  const unsigned vpr = (unsigned)(pl.row_bytes / W), all = t < T ? vpr * (unsigned)pl.H : 0;
+  const int first = threadIdx.x < B ? slots[threadIdx.x] : -1;
   constexpr int U = 4;
   V x[2][U];
   auto load = [&](unsigned i0) {
@@ -657,25 +699,52 @@ __global__ void __launch_bounds__(kThreads)
     }
   };
   load(lane);
-  const int64_t b = warp_find_seq(offs, is64, B, t, lane);
-  const int64_t lo = load_offset(offs, is64, b), hi = load_offset(offs, is64, b + 1);
-  const int s = slots[b];
-  if ((unsigned)s >= (unsigned)S || t < lo || t >= hi || hi > T) {
-    if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
+  // Where the row goes, or the site of what is wrong.
+  int site = 0, s = -1, p = 0;
+  int64_t b = 0;
+  unsigned at = 0, row = 0;
+  if (t < T) {
+    b = warp_find_seq(offs, is64, B, t, lane);
+    const int64_t lo = load_offset(offs, is64, b), hi = load_offset(offs, is64, b + 1);
+    s = slots[b];
+    if ((unsigned)s >= (unsigned)S || t < lo || t >= hi || hi > T) {
+      site = kSitePagedArgs;
+    } else {
+      const int64_t pos = (int64_t)lengths[s] - (hi - t);
+      if (pos < 0 || pos >= (int64_t)M * page) {
+        site = kSitePagedArgs;
+      } else {
+        at = (unsigned)pos / (unsigned)page;
+        row = (unsigned)pos - at * page;
+        p = table[(int64_t)s * M + at];
+        if ((unsigned)p >= (unsigned)P) site = kSitePagedTable;
+      }
+    }
+  }
+  if (B > 1 && B <= kCompareEntries) {
+    if (lane == 0) {
+      sm_slot[warp] = s;
+      sm_entry[warp] = (int)b;
+      if (warp == 0) sm_twice = 0;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < (int)B; i += kThreads) {
+      const int named = i < kThreads ? first : __ldg(slots + i);
+      uint32_t same = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) same |= named == sm_slot[w] && i != sm_entry[w] ? 1u << w : 0u;
+      if (same != 0 && load_offset(offs, is64, i + 1) > load_offset(offs, is64, i)) atomicOr(&sm_twice, same);
+    }
+    __syncthreads();
+    if (site == 0 && (sm_twice >> warp & 1)) site = kSitePagedArgs;
+  }
+  if (stopped || t >= T) return;
+  if (site != 0) {
+    if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, site);
     return;
   }
-  const int64_t pos = (int64_t)lengths[s] - (hi - t);
-  if (pos < 0 || pos >= (int64_t)M * page) {
-    if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
-    return;
-  }
-  const unsigned at = (unsigned)pos / (unsigned)page;
-  const int p = table[(int64_t)s * M + at];
-  if ((unsigned)p >= (unsigned)P) {
-    if (lane == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedTable);
-    return;
-  }
-  const int64_t to = layer * pl.layer_bytes + p * pl.page_bytes + (int64_t)((unsigned)pos - at * page) * pl.row_bytes;
+  const int64_t to = layer * pl.layer_bytes + p * pl.page_bytes + (int64_t)row * pl.row_bytes;
   const int64_t dst_hb = (int64_t)page * pl.row_bytes;
   for (unsigned i0 = lane; i0 < all; i0 += 32 * U) {
     if (i0 != (unsigned)lane) load(i0);
@@ -941,6 +1010,11 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
                                           (uintptr_t)v_row_bytes, (uintptr_t)v_head_bytes});
   const unsigned grid = (unsigned)((T + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t s = (cudaStream_t)stream;
+  if (B > kCompareEntries) {
+    SCREE_CUDA_TRY(launch_dependent(check_entries_kernel, dim3(1), dim3(kPlanThreads), 0, s, 1, slots, offsets,
+                                    offs_is_i64, B, (int)S, device_status_ptr()));
+    count_launch();
+  }
 #define SCREE_WRITE(WW)                                                                                   \
   SCREE_CUDA_TRY(launch_dependent(                                                                        \
       paged_write_kernel<WW>, dim3(grid), dim3(kThreads), 0, s, 1, pl, (int)layer, (const char*)k,        \

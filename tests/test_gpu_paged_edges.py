@@ -69,3 +69,67 @@ def test_visible_infinities_do_not_depend_on_the_cut(cuda, D, news, low, dtype):
     got = out.values.float().cpu().numpy()
     assert np.array_equal(np.isposinf(got), np.isposinf(ref[0])) and np.array_equal(np.isneginf(got), np.isneginf(ref[0]))
     assert _status() == 0
+
+
+# --------------------------------------------------------------------------- writes
+
+
+def _rows_cache(cuda, S, n=2, layers=1):
+    """S slots of n tokens each; every pool element 7."""
+    from scree_b200 import paged
+
+    cache = paged.paged_cache(layers, S + 4, 4, 1, 8, S, 3, dtype=torch.float16, device=cuda)
+    cache = paged.paged_reserve(cache, torch.arange(S, dtype=torch.int32, device=cuda),
+                                torch.full((S,), n, dtype=torch.int32, device=cuda))
+    cache.k.fill_(7)
+    cache.v.fill_(7)
+    return cache
+
+
+def _held(cache, slot, n):
+    return cache.k[0, cache.table[slot, 0].item(), 0, :n], cache.v[0, cache.table[slot, 0].item(), 0, :n]
+
+
+@pytest.mark.parametrize("B", [3, 40, 300, 1024, 1500, 9000])
+def test_write_refuses_a_slot_named_twice(cuda, B):
+    """By any two entries that have tokens, wherever they stand; their rows stay as they were."""
+    import scree_b200 as scree
+    from scree_b200 import _lib, paged
+
+    cache = _rows_cache(cuda, B)
+    slots = np.random.default_rng(B).permutation(B)
+    for a, b in ((0, B - 1), (B // 2, 0), (B - 1, B - 2)):
+        cache.k.fill_(7)  # (entries that name a slot of their own are written)
+        cache.v.fill_(7)
+        news = np.ones(B, np.int64)
+        news[b] = 2
+        offs = _i32(np.concatenate([[0], np.cumsum(news)]).tolist(), cuda)
+        named = slots.copy()
+        named[a] = named[b]
+        rows = torch.ones((int(news.sum()), 1, 8), dtype=torch.float16, device=cuda)
+        paged.paged_write(cache, 0, _i32(named.tolist(), cuda), scree.Array(rows, offs), scree.Array(rows, offs))
+        st = _lib.device_status()
+        assert st >> 16 == _lib.DEVERR_BAD_INPUT and st & 0xFFFF == 60
+        for pool in _held(cache, int(named[b]), 2):
+            assert (pool == 7).all()
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("B", [3, 300, 1500])
+def test_write_takes_entries_without_tokens_whatever_they_name(cuda, B):
+    """The places of a batch that are not in use may all name one slot."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+
+    cache = _rows_cache(cuda, B)
+    news = np.zeros(B, np.int64)
+    news[[0, B // 2]] = 1
+    slots = np.full(B, 1)
+    slots[0] = 2
+    offs = torch.tensor(np.concatenate([[0], np.cumsum(news)]), device=cuda)
+    rows = torch.arange(2 * 8, device=cuda).view(2, 1, 8).to(torch.float16)
+    paged.paged_write(cache, 0, _i32(slots.tolist(), cuda), scree.Array(rows, offs), scree.Array(-rows, offs))
+    for slot, t in ((2, 0), (1, 1)):
+        k, v = _held(cache, slot, 2)
+        assert torch.equal(k[1], rows[t, 0]) and torch.equal(v[1], -rows[t, 0]) and (k[0] == 7).all()
+    assert (cache.k == 7).sum() == cache.k.numel() - 16 + 1 and _status() == 0  # (one new element is a 7)
