@@ -357,13 +357,23 @@ int scree_paged_compact(const scree_paged_book* book, const scree_paged_pools* p
                         void* workspace, size_t workspace_bytes, void* stream);
 /* Writes K and V rows of one layer: rows [offsets[b], offsets[b+1]) of k / v
  * (T, H, D) go to the last tokens of slot slots[b].  Strides in BYTES, unit
- * stride inside a head. */
+ * stride inside a head.  Rows that cannot be placed are not written and set the
+ * status word: those of entries that name one slot (entries without tokens may name
+ * any) or more tokens than the slot holds, site 60. */
 int scree_paged_write(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
                       int64_t S, int64_t M, int64_t P, int64_t page, int64_t layer,
                       const int32_t* slots, const void* k, int64_t k_row_bytes,
                       int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
                       int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
                       int64_t T, void* stream);
+/* The same with the cache's refs (or NULL): rows on a page that several slots hold
+ * are not written either, site 62. */
+int scree_paged_write_ex(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
+                         const int32_t* refs, int64_t S, int64_t M, int64_t P, int64_t page,
+                         int64_t layer, const int32_t* slots, const void* k, int64_t k_row_bytes,
+                         int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
+                         int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
+                         int64_t T, void* stream);
 /* Who sees whom in trees of drafted tokens: parents (T,) int32, index of each
  * node's parent within its sequence (smaller than its own) or negative for a
  * root; bit j of row t of mask (T, words) = node j is t or an ancestor of t. */

@@ -30,7 +30,7 @@ constexpr int kMaxSlots = 65536;
 constexpr int kHereEntries = 2048, kHereWarps = 32;  // see apply_by_plan
 constexpr int kSitePagedArgs = 60;    // a slot, count, length or path out of range
 constexpr int kSitePagedFull = 61;    // not enough free pages
-constexpr int kSitePagedShared = 62;  // a draft on pages that other slots hold
+constexpr int kSitePagedShared = 62;  // a draft, or rows to write, on pages that other slots hold
 constexpr int kSitePagedTable = 63;   // a page id out of range
 
 // Decisions of a plan (int32 words at the start of the workspace), then
@@ -667,14 +667,14 @@ __global__ void __launch_bounds__(kPlanThreads)
 // Entries with tokens that name one slot would write the same rows: none of them
 // does.  The block's threads look for such entries side by side, behind the loads of
 // the chain.
-// 64 entries of 256 tokens of 8 x 128 16-bit elements: 23.3 us, 5.8 TB/s; of 64: 6.7;
-// one of six: 2.9, which is the chain.
+// 64 entries of 256 tokens of 8 x 128 16-bit elements: 24.6 us, 5.5 TB/s; of 64: 6.8;
+// one of six: 2.9, which is the chain.  (Without the look at refs 23.3, 6.7 and 2.9.)
 template <int W>
 __global__ void __launch_bounds__(kThreads, 4)
     paged_write_kernel(const Pools pl, int layer, const char* k, int64_t k_rb, int64_t k_hb, const char* v,
                        int64_t v_rb, int64_t v_hb, const void* offs, int is64, int64_t B, int64_t T,
-                       const int32_t* slots, const int32_t* table, const int32_t* lengths, int S, int M, int P,
-                       int page, int* status) {
+                       const int32_t* slots, const int32_t* table, const int32_t* lengths, const int32_t* refs, int S,
+                       int M, int P, int page, int* status) {
   using V = typename Vec<W>::T;
   constexpr int kWarps = kThreads / 32;
   __shared__ int sm_slot[kWarps], sm_entry[kWarps];
@@ -718,6 +718,7 @@ __global__ void __launch_bounds__(kThreads, 4)
         row = (unsigned)pos - at * page;
         p = table[(int64_t)s * M + at];
         if ((unsigned)p >= (unsigned)P) site = kSitePagedTable;
+        else if (refs != nullptr && refs[p] > 1) site = kSitePagedShared;
       }
     }
   }
@@ -986,12 +987,12 @@ extern "C" int scree_paged_compact(const scree_paged_book* book, const scree_pag
   return launch_apply<kCompact>(b, pl, nullptr, nullptr, nullptr, 0, 0, (book->P / 2 + 1) * pl.L * 2 * 8, s);
 }
 
-extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
-                                 int64_t S, int64_t M, int64_t P, int64_t page, int64_t layer,
-                                 const int32_t* slots, const void* k, int64_t k_row_bytes,
-                                 int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
-                                 int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
-                                 int64_t T, void* stream) {
+extern "C" int scree_paged_write_ex(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
+                                    const int32_t* refs, int64_t S, int64_t M, int64_t P, int64_t page,
+                                    int64_t layer, const int32_t* slots, const void* k, int64_t k_row_bytes,
+                                    int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
+                                    int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
+                                    int64_t T, void* stream) {
   SCREE_CHECK_ARG(S >= 1 && S <= kMaxSlots && M >= 1 && P >= 1 && P < (1ll << 30) && page >= 1 &&
                       M * page < (1ll << 31),
                   "paged_write: bad sizes S=%lld M=%lld P=%lld page=%lld", (long long)S, (long long)M,
@@ -1019,7 +1020,7 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
   SCREE_CUDA_TRY(launch_dependent(                                                                        \
       paged_write_kernel<WW>, dim3(grid), dim3(kThreads), 0, s, 1, pl, (int)layer, (const char*)k,        \
       k_row_bytes, k_head_bytes, (const char*)v, v_row_bytes, v_head_bytes, offsets, offs_is_i64, B, T,   \
-      slots, table, lengths, (int)S, (int)M, (int)P, (int)page, device_status_ptr()))
+      slots, table, lengths, refs, (int)S, (int)M, (int)P, (int)page, device_status_ptr()))
   switch (w) {
     case 16: SCREE_WRITE(16); break;
     case 8: SCREE_WRITE(8); break;
@@ -1030,6 +1031,16 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
 #undef SCREE_WRITE
   count_launch();
   return SCREE_OK;
+}
+
+extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
+                                 int64_t S, int64_t M, int64_t P, int64_t page, int64_t layer,
+                                 const int32_t* slots, const void* k, int64_t k_row_bytes,
+                                 int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
+                                 int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
+                                 int64_t T, void* stream) {
+  return scree_paged_write_ex(pools, table, lengths, nullptr, S, M, P, page, layer, slots, k, k_row_bytes,
+                              k_head_bytes, v, v_row_bytes, v_head_bytes, offsets, offs_is_i64, B, T, stream);
 }
 
 extern "C" int scree_tree_mask(const int32_t* parents, const void* offsets, int offs_is_i64, int64_t B,

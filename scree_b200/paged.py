@@ -179,7 +179,9 @@ def _offsets(arr: Array, device):
 
 def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> None:
     """Writes the rows of sequence b of k / v (T, kv_heads, head_dim) as the K / V of the last
-    tokens of slot slots[b] in one layer."""
+    tokens of slot slots[b] in one layer.  Not written, with the status word set: the rows of
+    sequences that name one slot, or have more tokens than it holds, and rows on a page that
+    other slots hold."""
     kt, vt, pools = k.values, v.values, cache._pools
     S, M, P, page, H, D = pools.sizes
     dev = pools.device
@@ -196,10 +198,10 @@ def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> Non
         kt, vt = kt.contiguous(), vt.contiguous()
         (kr, kh, _), (vr, vh, _) = kt.stride(), vt.stride()
     es = kt.element_size()
-    rc = _lib.load().scree_paged_write(
-        pools.ref, cache.table.data_ptr(), cache.lengths.data_ptr(), S, M, P, page, layer, slots.data_ptr(),
-        kt.data_ptr(), kr * es, kh * es, vt.data_ptr(), vr * es, vh * es, offs.data_ptr(), is64, B, kt.shape[0],
-        _lib.stream_ptr(dev))
+    rc = _lib.load().scree_paged_write_ex(
+        pools.ref, cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(), S, M, P, page, layer,
+        slots.data_ptr(), kt.data_ptr(), kr * es, kh * es, vt.data_ptr(), vr * es, vh * es, offs.data_ptr(), is64, B,
+        kt.shape[0], _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "paged_write")
 

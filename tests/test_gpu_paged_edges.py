@@ -133,3 +133,40 @@ def test_write_takes_entries_without_tokens_whatever_they_name(cuda, B):
         k, v = _held(cache, slot, 2)
         assert torch.equal(k[1], rows[t, 0]) and torch.equal(v[1], -rows[t, 0]) and (k[0] == 7).all()
     assert (cache.k == 7).sum() == cache.k.numel() - 16 + 1 and _status() == 0  # (one new element is a 7)
+
+
+@pytest.mark.parametrize("page,n", [(4, 8), (4, 10), (16, 16)])
+def test_write_refuses_pages_that_other_slots_hold(cuda, page, n):
+    """After a fork the shared pages are no slot's own: written over, the sibling's K / V would go."""
+    import scree_b200 as scree
+    from scree_b200 import _lib, paged
+
+    cache = paged.paged_cache(2, 12, page, 2, 16, 4, 4, dtype=torch.bfloat16, device=cuda)
+    one = _i32([1], cuda)
+    cache = paged.paged_reserve(cache, one, _i32([n], cuda))
+    gen = torch.Generator().manual_seed(n)
+    rows = lambda m: scree.Array(torch.randn((m, 2, 16), generator=gen).to(torch.bfloat16).to(cuda), _i32([0, m], cuda))  # noqa: E731
+    k, v = rows(n), rows(n)
+    paged.paged_write(cache, 1, one, k, v)
+    cache = paged.paged_fork(cache, one, _i32([3], cuda))
+    assert _status() == 0
+    before = cache.k.clone(), cache.v.clone()
+    full = n // page * page
+    for slot in (1, 3):
+        k2, v2 = rows(n), rows(n)
+        paged.paged_write(cache, 1, _i32([slot], cuda), k2, v2)
+        st = _lib.device_status()
+        assert st >> 16 == _lib.DEVERR_BAD_INPUT and st & 0xFFFF == 62
+        ids = cache.table[1, :full // page].long()
+        assert torch.equal(cache.k[:, ids], before[0][:, ids]) and torch.equal(cache.v[:, ids], before[1][:, ids])
+    # What is behind them is a slot's own, and so are all pages once the sibling is gone.
+    grown = paged.paged_reserve(cache, one, _i32([page], cuda))
+    k3, v3 = rows(page), rows(page)
+    paged.paged_write(grown, 1, one, k3, v3)
+    at = [(grown.table[1, i // page].item(), i % page) for i in range(n, n + page)]
+    assert _status() == 0 and all(torch.equal(grown.k[1, p, :, r], k3.values[i]) for i, (p, r) in enumerate(at))
+    alone = paged.paged_free(grown, _i32([3], cuda))
+    k4, v4 = rows(n + page), rows(n + page)
+    paged.paged_write(alone, 0, one, k4, v4)
+    at = [(alone.table[1, i // page].item(), i % page) for i in range(n + page)]
+    assert _status() == 0 and all(torch.equal(alone.v[0, p, :, r], v4.values[i]) for i, (p, r) in enumerate(at))
