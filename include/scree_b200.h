@@ -367,13 +367,14 @@ int scree_paged_write(const scree_paged_pools* pools, const int32_t* table, cons
                       int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
                       int64_t T, void* stream);
 /* The same with the cache's refs (or NULL): rows on a page that several slots hold
- * are not written either, site 62. */
+ * are not written either, site 62; and if v comes with offsets of its own (or NULL) that
+ * are not those of k, nothing is written, site 60. */
 int scree_paged_write_ex(const scree_paged_pools* pools, const int32_t* table, const int32_t* lengths,
                          const int32_t* refs, int64_t S, int64_t M, int64_t P, int64_t page,
                          int64_t layer, const int32_t* slots, const void* k, int64_t k_row_bytes,
                          int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
-                         int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
-                         int64_t T, void* stream);
+                         int64_t v_head_bytes, const void* offsets, const void* v_offsets,
+                         int offs_is_i64, int64_t B, int64_t T, void* stream);
 /* Who sees whom in trees of drafted tokens: parents (T,) int32, index of each
  * node's parent within its sequence (smaller than its own) or negative for a
  * root; bit j of row t of mask (T, words) = node j is t or an ancestor of t. */

@@ -107,7 +107,7 @@ _SIGNATURES = {
     ),
     "scree_paged_write_ex": (
         _I,
-        [_P, _P, _P, _P, _L, _L, _L, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _I, _L, _L, _P],
+        [_P, _P, _P, _P, _L, _L, _L, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _L, _L, _P],
     ),
     "scree_tree_mask": (_I, [_P, _P, _I, _L, _L, _L, _P, _P]),
     "scree_attn_fwd_paged_workspace_size": (_S, [_L, _L, _L, _L, _I]),

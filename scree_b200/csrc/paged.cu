@@ -631,15 +631,20 @@ __device__ __forceinline__ int64_t warp_find_seq(const void* offs, int is64, int
 // 4,096 13.3 / 9.3, 16,384 107 / 35.
 constexpr int64_t kCompareEntries = 1024;
 
-// Records that two entries with tokens name one slot; by one block, ahead of the write.
+// Records that two entries with tokens name one slot, or that k's and v's offsets (or
+// nullptr: the same) differ; by one block, ahead of the write.
 __global__ void __launch_bounds__(kPlanThreads)
-    check_entries_kernel(const int32_t* slots, const void* offs, int is64, int64_t B, int S, int* status) {
+    check_entries_kernel(const int32_t* slots, const void* offs, const void* v_offs, int is64, int64_t B, int S,
+                         int* status) {
   __shared__ SlotSet set;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   for (int i = threadIdx.x; i < kMaxSlots / 32; i += blockDim.x) set.bits[i] = 0;
   __syncthreads();
-  bool twice = false;
+  bool bad = false;
+  if (v_offs != nullptr)
+    for (int64_t i = threadIdx.x; i <= B; i += blockDim.x)
+      bad |= load_offset(offs, is64, i) != load_offset(v_offs, is64, i);
   constexpr int C = 4;  // loads under way
   for (int64_t i0 = threadIdx.x; i0 < B; i0 += C * kPlanThreads) {
     int s[C];
@@ -655,10 +660,10 @@ __global__ void __launch_bounds__(kPlanThreads)
       // (Neighbouring slots in words of their own.)
       const uint32_t bit = 1u << ((unsigned)s[c] / (kMaxSlots / 32) & 31);
       if ((unsigned)s[c] < (unsigned)S && some[c])
-        twice |= (atomicOr(&set.bits[s[c] % (kMaxSlots / 32)], bit) & bit) != 0;
+        bad |= (atomicOr(&set.bits[s[c] % (kMaxSlots / 32)], bit) & bit) != 0;
     }
   }
-  if (__syncthreads_or(twice) && threadIdx.x == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
+  if (__syncthreads_or(bad) && threadIdx.x == 0) record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
 }
 
 // One warp per token: its K and V rows.  The rows of entry b are the last
@@ -991,8 +996,8 @@ extern "C" int scree_paged_write_ex(const scree_paged_pools* pools, const int32_
                                     const int32_t* refs, int64_t S, int64_t M, int64_t P, int64_t page,
                                     int64_t layer, const int32_t* slots, const void* k, int64_t k_row_bytes,
                                     int64_t k_head_bytes, const void* v, int64_t v_row_bytes,
-                                    int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
-                                    int64_t T, void* stream) {
+                                    int64_t v_head_bytes, const void* offsets, const void* v_offsets,
+                                    int offs_is_i64, int64_t B, int64_t T, void* stream) {
   SCREE_CHECK_ARG(S >= 1 && S <= kMaxSlots && M >= 1 && P >= 1 && P < (1ll << 30) && page >= 1 &&
                       M * page < (1ll << 31),
                   "paged_write: bad sizes S=%lld M=%lld P=%lld page=%lld", (long long)S, (long long)M,
@@ -1011,9 +1016,9 @@ extern "C" int scree_paged_write_ex(const scree_paged_pools* pools, const int32_
                                           (uintptr_t)v_row_bytes, (uintptr_t)v_head_bytes});
   const unsigned grid = (unsigned)((T + kThreads / 32 - 1) / (kThreads / 32));
   cudaStream_t s = (cudaStream_t)stream;
-  if (B > kCompareEntries) {
+  if (B > kCompareEntries || v_offsets != nullptr) {
     SCREE_CUDA_TRY(launch_dependent(check_entries_kernel, dim3(1), dim3(kPlanThreads), 0, s, 1, slots, offsets,
-                                    offs_is_i64, B, (int)S, device_status_ptr()));
+                                    v_offsets, offs_is_i64, B, (int)S, device_status_ptr()));
     count_launch();
   }
 #define SCREE_WRITE(WW)                                                                                   \
@@ -1040,7 +1045,7 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
                                  int64_t v_head_bytes, const void* offsets, int offs_is_i64, int64_t B,
                                  int64_t T, void* stream) {
   return scree_paged_write_ex(pools, table, lengths, nullptr, S, M, P, page, layer, slots, k, k_row_bytes,
-                              k_head_bytes, v, v_row_bytes, v_head_bytes, offsets, offs_is_i64, B, T, stream);
+                              k_head_bytes, v, v_row_bytes, v_head_bytes, offsets, nullptr, offs_is_i64, B, T, stream);
 }
 
 extern "C" int scree_tree_mask(const int32_t* parents, const void* offsets, int offs_is_i64, int64_t B,

@@ -180,8 +180,8 @@ def _offsets(arr: Array, device):
 def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> None:
     """Writes the rows of sequence b of k / v (T, kv_heads, head_dim) as the K / V of the last
     tokens of slot slots[b] in one layer.  Not written, with the status word set: the rows of
-    sequences that name one slot, or have more tokens than it holds, and rows on a page that
-    other slots hold."""
+    sequences that name one slot, or have more tokens than it holds, rows on a page that other
+    slots hold, and all rows if k and v have different offsets."""
     kt, vt, pools = k.values, v.values, cache._pools
     S, M, P, page, H, D = pools.sizes
     dev = pools.device
@@ -193,6 +193,13 @@ def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> Non
         raise TypeError("k and v must be on the cache's device")
     offs, is64, B = _offsets(k, dev)
     slots = _ints(slots, B, "slots", dev)
+    v_offs = None
+    if v.offsets is not k.offsets:  # compared on the device, so that nothing is read from it
+        v_offs, v_is64, v_batch = _offsets(v, dev)
+        if v_batch != B:
+            raise ValueError(f"k and v must have identical offsets ({B} and {v_batch} sequences)")
+        if v_is64 != is64:
+            v_offs = v_offs.to(offs.dtype)
     (kr, kh, kd), (vr, vh, vd) = kt.stride(), vt.stride()
     if kd != 1 or vd != 1:
         kt, vt = kt.contiguous(), vt.contiguous()
@@ -200,8 +207,8 @@ def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> Non
     es = kt.element_size()
     rc = _lib.load().scree_paged_write_ex(
         pools.ref, cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(), S, M, P, page, layer,
-        slots.data_ptr(), kt.data_ptr(), kr * es, kh * es, vt.data_ptr(), vr * es, vh * es, offs.data_ptr(), is64, B,
-        kt.shape[0], _lib.stream_ptr(dev))
+        slots.data_ptr(), kt.data_ptr(), kr * es, kh * es, vt.data_ptr(), vr * es, vh * es, offs.data_ptr(),
+        None if v_offs is None else v_offs.data_ptr(), is64, B, kt.shape[0], _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "paged_write")
 

@@ -170,3 +170,28 @@ def test_write_refuses_pages_that_other_slots_hold(cuda, page, n):
     paged.paged_write(alone, 0, one, k4, v4)
     at = [(alone.table[1, i // page].item(), i % page) for i in range(n + page)]
     assert _status() == 0 and all(torch.equal(alone.v[0, p, :, r], v4.values[i]) for i, (p, r) in enumerate(at))
+
+
+def test_write_compares_the_offsets_of_k_and_v(cuda):
+    """v's rows of a sequence are those of its own offsets: other ones than k's are refused."""
+    import scree_b200 as scree
+    from scree_b200 import _lib, paged
+
+    cache = _rows_cache(cuda, 4, n=3)
+    slots = _i32([2, 0, 3], cuda)
+    rows = torch.arange(6 * 8, device=cuda).view(6, 1, 8).to(torch.float16)
+    k = scree.Array(rows, _i32([0, 2, 3, 6], cuda))
+    for offs in ([0, 1, 3, 6], [0, 2, 4, 6], [0, 2, 2, 6]):
+        cache.k.fill_(7)
+        cache.v.fill_(7)
+        paged.paged_write(cache, 0, slots, k, scree.Array(rows, _i32(offs, cuda)))
+        st = _lib.device_status()
+        assert st >> 16 == _lib.DEVERR_BAD_INPUT and st & 0xFFFF == 60
+        assert (cache.k == 7).all() and (cache.v == 7).all()
+    with pytest.raises(ValueError, match="identical offsets"):
+        paged.paged_write(cache, 0, slots, k, scree.Array(rows, _i32([0, 2, 6], cuda)))
+    for same in (k.offsets.clone(), k.offsets.long(), k.offsets.cpu()):  # equal ones of another tensor
+        cache.v.fill_(7)
+        paged.paged_write(cache, 0, slots, k, scree.Array(rows, same))
+        assert torch.equal(_held(cache, 3, 3)[1], rows[3:, 0]) and torch.equal(_held(cache, 0, 3)[1][2], rows[2, 0])
+    assert _status() == 0
