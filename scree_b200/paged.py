@@ -167,6 +167,11 @@ def paged_compact(cache: PagedCache) -> PagedCache:
     return _book_call(cache, _lib.load().scree_paged_compact, "paged_compact", cache._pools.ref)
 
 
+def _ragged_tokens(name, *arrays):
+    if any(a.ragged_dim != 0 for a in arrays):
+        raise NotImplementedError(f"{name} supports ragged_dim=0 only in v0.1")
+
+
 def _offsets(arr: Array, device):
     """Offsets on the device, whether they are int64, sequences."""
     offs = arr.offsets
@@ -182,6 +187,7 @@ def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> Non
     tokens of slot slots[b] in one layer.  Not written, with the status word set: the rows of
     sequences that name one slot, or have more tokens than it holds, rows on a page that other
     slots hold, and all rows if k and v have different offsets."""
+    _ragged_tokens("paged_write", k, v)
     kt, vt, pools = k.values, v.values, cache._pools
     S, M, P, page, H, D = pools.sizes
     dev = pools.device
@@ -247,6 +253,7 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     the LSE (T, heads) fp32 when ``return_lse``)."""
     qt, pools = q.values, cache._pools
     _require_cuda(qt, "paged_attention")
+    _ragged_tokens("paged_attention", q)
     S, M, P, page, Hkv, D = pools.sizes
     dev, dtype = qt.device, qt.dtype
     assert dtype in (torch.float16, torch.bfloat16), "fp16 or bf16 only"

@@ -195,3 +195,21 @@ def test_write_compares_the_offsets_of_k_and_v(cuda):
         paged.paged_write(cache, 0, slots, k, scree.Array(rows, same))
         assert torch.equal(_held(cache, 3, 3)[1], rows[3:, 0]) and torch.equal(_held(cache, 0, 3)[1][2], rows[2, 0])
     assert _status() == 0
+
+
+def test_arrays_must_be_ragged_in_their_tokens(cuda):
+    """Offsets that count heads are not offsets of tokens, even where the numbers would do."""
+    import scree_b200 as scree
+    from scree_b200 import paged
+
+    cache = paged.paged_cache(1, 4, 16, 2, 64, 1, 2, device=cuda)
+    cache = paged.paged_reserve(cache, _i32([0], cuda), _i32([2], cuda))
+    t = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device=cuda)
+    offs = _i32([0, 2], cuda)
+    heads, tokens = scree.Array(t, offs, ragged_dim=1), scree.Array(t, offs)
+    for k, v in ((heads, tokens), (tokens, heads)):
+        with pytest.raises(NotImplementedError, match="ragged_dim"):
+            paged.paged_write(cache, 0, _i32([0], cuda), k, v)
+    with pytest.raises(NotImplementedError, match="ragged_dim"):
+        paged.paged_attention(heads, cache, 0, _i32([0], cuda))
+    assert paged.paged_attention(tokens, cache, 0, _i32([0], cuda)).ragged_dim == 0 and _status() == 0
