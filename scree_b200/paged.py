@@ -48,7 +48,6 @@ class PagedCache:
     table: Any
     lengths: Any
     refs: Any
-    _work: Any = field(default=None, repr=False, compare=False)  # plan workspace, shared by derived caches
     _pools: Any = field(default=None, repr=False, compare=False)
 
     def __post_init__(self) -> None:
@@ -67,13 +66,11 @@ class PagedCache:
             raise ValueError("all tensors of a cache must be on one device")
         L, P, H, page, D = self.k.shape
         S, M = self.table.shape
-        work = torch.empty(_lib.load().scree_paged_workspace_size(S, P), dtype=torch.uint8, device=self.k.device)
         pools = _lib.PagedPools(self.k.data_ptr(), self.v.data_ptr(), L, H, D * self.k.element_size())
         # What every call of this cache and those derived from it passes on.
         pools.sizes = (S, M, P, page, H, D)
         pools.dtype, pools.device = self.k.dtype, self.k.device
-        pools.ref, pools.work = ctypes.byref(pools), (work.data_ptr(), work.numel())
-        object.__setattr__(self, "_work", work)
+        pools.ref, pools.work_bytes = ctypes.byref(pools), _lib.load().scree_paged_workspace_size(S, P)
         object.__setattr__(self, "_pools", pools)
 
     @property
@@ -110,10 +107,13 @@ def _book_call(cache: PagedCache, fn, name: str, *args) -> PagedCache:
     S, M, P, page, _, _ = pools.sizes
     book = _lib.PagedBook(t.data_ptr(), le.data_ptr(), r.data_ptr(), table.data_ptr(), lengths.data_ptr(),
                           refs.data_ptr(), S, M, P, page)
-    rc = fn(ctypes.byref(book), *args, *pools.work, _lib.stream_ptr(pools.device))
+    # The plan's workspace is the call's own, of the stream it runs on: another call, on another
+    # stream or thread, cannot come between the plan and its apply.
+    work = r.new_empty(pools.work_bytes // 4)
+    rc = fn(ctypes.byref(book), *args, work.data_ptr(), pools.work_bytes, _lib.stream_ptr(pools.device))
     if rc:
         _lib.check(rc, name)
-    out = object.__new__(PagedCache)  # nothing to check: the same pools, workspace and shapes
+    out = object.__new__(PagedCache)  # nothing to check: the same pools and shapes
     out.__dict__.update(cache.__dict__, table=table, lengths=lengths, refs=refs)
     return out
 

@@ -1,0 +1,47 @@
+"""A cache's calls share no workspace: what one has planned and not yet applied is not
+another's to overwrite, on whatever stream or thread that one runs.  No GPU: the library call
+is a stand-in that starts a second call in the middle of the first."""
+
+import ctypes
+
+import torch
+
+from scree_b200 import _lib, paged
+
+
+def _cache(monkeypatch):
+    monkeypatch.setattr(paged, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda device=None: 0)
+    kv = torch.zeros((1, 6, 1, 4, 8))
+    i32 = dict(dtype=torch.int32)
+    return paged.PagedCache(k=kv, v=kv.clone(), table=torch.full((3, 2), -1, **i32), lengths=torch.zeros(3, **i32),
+                            refs=torch.zeros(6, **i32))
+
+
+def test_calls_in_flight_have_workspaces_of_their_own(monkeypatch):
+    cache = _cache(monkeypatch)
+    need = _lib.load().scree_paged_workspace_size(3, 6)
+    spans = []
+
+    def call(book, workspace, size, stream):
+        assert size >= need and workspace % 16 == 0
+        spans.append((workspace, workspace + size))
+        if len(spans) < 3:
+            paged._book_call(cache, call, "inner")
+        return 0
+
+    out = paged._book_call(cache, call, "outer")
+    assert len(spans) == 3
+    for i, a in enumerate(spans):
+        for b in spans[:i]:
+            assert a[1] <= b[0] or b[1] <= a[0]
+    # A derived cache keeps nothing of its call but the new bookkeeping.
+    fresh = {k for k, v in out.__dict__.items() if v is not cache.__dict__.get(k)}
+    assert fresh == {"table", "lengths", "refs"}
+
+
+def test_a_cache_holds_no_memory_but_its_tensors(monkeypatch):
+    cache = _cache(monkeypatch)
+    held = [k for k, v in cache.__dict__.items() if isinstance(v, torch.Tensor)]
+    assert sorted(held) == ["k", "lengths", "refs", "table", "v"]
+    assert isinstance(cache._pools, ctypes.Structure)
