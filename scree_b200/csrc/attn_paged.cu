@@ -598,7 +598,7 @@ extern "C" int scree_attn_fwd_paged(const void* q, int64_t q_rs, int64_t q_hs, c
   SCREE_CHECK_ARG(H_kv >= 1 && H >= 1 && H % H_kv == 0 && H < 65536,
                   "attn_fwd_paged: query heads (%lld) must be a multiple of K/V heads (%lld)", (long long)H,
                   (long long)H_kv);
-  SCREE_CHECK_ARG(B >= 1 && B <= kPagedMaxSeqs && T >= 0 && T < (1ll << 31) && T * (H / H_kv) < (1ll << 31),
+  SCREE_CHECK_ARG(B >= (T > 0) && B <= kPagedMaxSeqs && T >= 0 && T < (1ll << 31) && T * (H / H_kv) < (1ll << 31),
                   "attn_fwd_paged: bad sizes B=%lld (at most %d) T=%lld", (long long)B, kPagedMaxSeqs, (long long)T);
   if (D != 32 && D != 64 && D != 128) {
     set_last_error("attn_fwd_paged: head_dim %d unsupported (32, 64, 128)", D);

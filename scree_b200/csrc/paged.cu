@@ -1002,7 +1002,7 @@ extern "C" int scree_paged_write_ex(const scree_paged_pools* pools, const int32_
                       M * page < (1ll << 31),
                   "paged_write: bad sizes S=%lld M=%lld P=%lld page=%lld", (long long)S, (long long)M,
                   (long long)P, (long long)page);
-  SCREE_CHECK_ARG(B >= 1 && T >= 0 && T < (1ll << 31), "paged_write: bad sizes B=%lld T=%lld", (long long)B,
+  SCREE_CHECK_ARG(B >= (T > 0) && T >= 0 && T < (1ll << 31), "paged_write: bad sizes B=%lld T=%lld", (long long)B,
                   (long long)T);
   Pools pl;
   int rc = make_pools("paged_write", pools, P, page, &pl);
@@ -1050,7 +1050,7 @@ extern "C" int scree_paged_write(const scree_paged_pools* pools, const int32_t* 
 
 extern "C" int scree_tree_mask(const int32_t* parents, const void* offsets, int offs_is_i64, int64_t B,
                                int64_t T, int64_t words, uint64_t* mask, void* stream) {
-  SCREE_CHECK_ARG(B >= 1 && T >= 0 && T < (1ll << 31) && words >= 1 && words < (1 << 20),
+  SCREE_CHECK_ARG(B >= (T > 0) && T >= 0 && T < (1ll << 31) && words >= 1 && words < (1 << 20),
                   "tree_mask: bad sizes B=%lld T=%lld words=%lld", (long long)B, (long long)T, (long long)words);
   if (T == 0) return SCREE_OK;
   SCREE_CHECK_ARG(parents && offsets && mask, "tree_mask: null pointer");

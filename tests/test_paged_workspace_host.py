@@ -45,3 +45,20 @@ def test_a_cache_holds_no_memory_but_its_tensors(monkeypatch):
     held = [k for k, v in cache.__dict__.items() if isinstance(v, torch.Tensor)]
     assert sorted(held) == ["k", "lengths", "refs", "table", "v"]
     assert isinstance(cache._pools, ctypes.Structure)
+
+
+def test_a_step_without_sequences_is_taken_by_every_entry_point():
+    """No entries, no tokens: as reserve, accept, fork and free take n = 0 (they need a GPU)."""
+    lib = _lib.load()
+    pools = ctypes.byref(_lib.PagedPools(16, 16, 1, 2, 128))
+    write = [pools, 16, 16, 4, 4, 16, 16, 0, 16, 16, 256, 128, 16, 256, 128, 16, 0, 0, 0, None]
+    assert lib.scree_paged_write(*write) == _lib.SCREE_OK
+    assert lib.scree_paged_write_ex(*write[:3], 16, *write[3:16], None, *write[16:]) == _lib.SCREE_OK
+    assert lib.scree_tree_mask(16, 16, 0, 0, 0, 1, 16, None) == _lib.SCREE_OK
+    attention = [16, 256, 64, pools, 0, 16, 16, 4, 4, 16, 16, 16, 16, 0, 0, 0, 4, 64, _lib.BF16, 0.125, None, 0, 16, 256,
+                 64, None, 16, 1 << 30, None]
+    assert lib.scree_attn_fwd_paged(*attention) == _lib.SCREE_OK
+    # Tokens of no sequence are not.
+    for args, fn in ((write[:18] + [3] + write[19:], lib.scree_paged_write), ([16, 16, 0, 0, 3, 1, 16, None], lib.scree_tree_mask),
+                     (attention[:15] + [3] + attention[16:], lib.scree_attn_fwd_paged)):
+        assert fn(*args) == _lib.SCREE_ERR_INVALID
