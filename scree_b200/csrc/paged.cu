@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     b = warp_find_seq(offs, is64, B, t, lane);
     const int64_t lo = load_offset(offs, is64, b), hi = load_offset(offs, is64, b + 1);
     s = slots[b];
-    if ((unsigned)s >= (unsigned)S || t < lo || t >= hi || hi > T) {
+    if ((unsigned)s >= (unsigned)S || lo < 0 || t < lo || t >= hi || hi > T) {
       site = kSitePagedArgs;
     } else {
       const int64_t pos = (int64_t)lengths[s] - (hi - t);
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t lo = load_offset(offs, is64, b), hi = load_offset(offs, is64, b + 1);
   unsigned long long* row = mask + t * words;
   for (int w = 0; w < words; ++w) row[w] = 0;
-  if (t < lo || t >= hi || hi > T || hi - lo > (int64_t)words * 64) {
+  if (lo < 0 || t < lo || t >= hi || hi > T || hi - lo > (int64_t)words * 64) {
     record_device_error(status, SCREE_DEVERR_BAD_INPUT, kSitePagedArgs);
     return;
   }

@@ -213,3 +213,24 @@ def test_arrays_must_be_ragged_in_their_tokens(cuda):
     with pytest.raises(NotImplementedError, match="ragged_dim"):
         paged.paged_attention(heads, cache, 0, _i32([0], cuda))
     assert paged.paged_attention(tokens, cache, 0, _i32([0], cuda)).ragged_dim == 0 and _status() == 0
+
+
+def test_offsets_below_zero_are_refused(cuda):
+    """Offsets between the first and the last may be anything: nothing is read in front of the parents."""
+    import scree_b200 as scree
+    from scree_b200 import _lib, paged
+
+    offs = _i32([0, -5, 3], cuda)
+
+    def site():
+        st = _lib.device_status()
+        assert st >> 16 == _lib.DEVERR_BAD_INPUT
+        return st & 0xFFFF
+
+    mask = paged.tree_mask(scree.Array(_i32([2, 2, 2], cuda), offs), max_nodes=8)
+    assert site() == 60 and (mask == 0).all()
+    cache = _rows_cache(cuda, 2, n=10)
+    rows = scree.Array(torch.ones((3, 1, 8), dtype=torch.float16, device=cuda), offs)
+    paged.paged_write(cache, 0, _i32([0, 1], cuda), rows, rows)
+    assert site() == 60 and (cache.k == 7).all()
+    assert _status() == 0
