@@ -414,7 +414,8 @@ int scree_token_logprobs_fwd(const void* logits, int64_t row_stride, const void*
                              float* logp, float* entropy, float* norm, float* top_logp,
                              int64_t* top_ids, void* stream);
 /* d_logits (N, V) contiguous from the gradients of logp, entropy (N,) and
- * top_logp (N, top), each fp32 contiguous or NULL. */
+ * top_logp (N, top), each fp32 contiguous or NULL.  An id outside the vocabulary
+ * sets the status word (SCREE_DEVERR_BAD_INPUT, site 52); nothing is written for it. */
 int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, const void* targets,
                              int targets_is_i64, const float* norm, const float* entropy,
                              const int64_t* top_ids, const float* g_logp, const float* g_entropy,

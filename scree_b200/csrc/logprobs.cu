@@ -52,7 +52,7 @@ constexpr int kWarps = kThreads / 32;      // that work; one more copies, one fi
 constexpr int kMaxSegs = 8;     // a portable cluster
 constexpr int kSiteRing = 51;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kSiteTarget = 50;
+constexpr int kSiteTarget = 50, kSiteAlternative = 52;
 
 template <typename T> struct Lv {  // elements of one 16-byte vector
   static constexpr int N = 16 / sizeof(T);
@@ -749,6 +749,7 @@ struct BwdArgs {
   const int64_t* top_ids;
   const float *g_logp, *g_entropy, *g_top;  // each may be null
   void* dx;                                 // (N, V) contiguous
+  int* status;
 };
 
 // The 16 bytes of a and b (the 16 behind a) from byte `bytes` < 16 on.
@@ -865,7 +866,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
     int64_t idx;
     entry(threadIdx.x, idx);
     const int lo = v0 * VE - mis;
-    if (idx >= 0 && idx >= lo && idx < lo + kThreads * NV * VE) {
+    if (threadIdx.x > 0 && (idx < 0 || idx >= a.V)) {  // an id that is none: nothing to write
+      record_device_error(a.status, SCREE_DEVERR_BAD_INPUT, kSiteAlternative);
+    } else if (idx >= 0 && idx >= lo && idx < lo + kThreads * NV * VE) {
       float g = 0.f;
       for (int j = 0; j < entries; ++j) {
         int64_t other;
@@ -1000,6 +1003,7 @@ extern "C" int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, 
   a.g_entropy = g_entropy;
   a.g_top = top > 0 ? g_top : nullptr;
   a.dx = d_logits;
+  a.status = device_status_ptr();
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == SCREE_F32) return launch_bwd<float>(a, s);
   return dtype == SCREE_BF16 ? launch_bwd<__nv_bfloat16>(a, s) : launch_bwd<__half>(a, s);
