@@ -31,7 +31,7 @@
 // is passed over, so floods of equal values end early.
 //
 // Numerics: sums in fp32, exponents in units of log2 (one FMA and one ex2 per
-// element; the product x log2e is not rounded before m is subtracted; see kFar).
+// element; the product x log2e is not rounded before m is subtracted; see shift).
 #include <algorithm>
 #include "common.cuh"
 #include "sm100.cuh"
@@ -100,10 +100,14 @@ template <typename T> __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
-// x log2e - m log2e in one FMA rounds m log2e first, which is worth 2^-24 |m|: of a
-// maximum of 1024 and more in magnitude (a row, or all that a thread has seen of it,
-// masked with a large number) x - m is taken first.
+// x log2e - m log2e in one FMA rounds m log2e first.  All terms are off by the same
+// 2^shift(m), so sums are kept as they are and the shift is taken out where maxima meet
+// and at the row's end: log p depends on differences alone.  From 1024 on (a row, or all
+// that a thread has seen of it, masked with a large number) x - m is taken first.
 constexpr float kFar = 1024.f;
+__device__ __forceinline__ float shift(float m) {
+  return fabsf(m) >= kFar ? 0.f : fmaf(m, kLog2e, -__fmul_rn(m, kLog2e));
+}
 // -inf must not meet its own weight, 0 * -inf = NaN: elements near the
 // type's lowest value are raised to `low`, two at a time for the 16-bit types.  With |m| < kFar their weight
 // is 0 either way and (x - m) log2e is finite.  NaN stays.
@@ -144,13 +148,16 @@ __device__ __forceinline__ unsigned long long order_key(float x, uint32_t idx) {
   return ((unsigned long long)order_bits(x) << 32) | (0xFFFFFFFFu - idx);
 }
 
-// Running statistics: m, s1, and s2 in units of log2; s1 = 0 when empty.
+// Running statistics: m, s1, and s2 in units of log2, both sums' terms 2^shift(m) too
+// large; s1 = 0 when empty.
 struct Stat {
   float m, s1, s2;
 };
 // s1 and s2 moved from maximum m to the maximum `to` >= m.
 __device__ __forceinline__ void stat_move(Stat& s, float to) {
-  const float d = (s.m - (to == -INFINITY ? 0.f : to)) * kLog2e;
+  float d = __fmul_rn(s.m, kLog2e) - __fmul_rn(to, kLog2e);  // both near: what the terms were taken at
+  if (!(fmaxf(fabsf(s.m), fabsf(to)) < kFar))
+    d = (s.m - (to == -INFINITY ? 0.f : to)) * kLog2e + (shift(to) - shift(s.m));
   const float w = ex2_approx(d);
   // An empty side has d = -inf: its weight is 0 and its (bounded) shift is not used.
   s.s2 = w * (s.s2 + fmaxf(d, -1000.f) * s.s1);
@@ -224,10 +231,10 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, int64_t n, const St
                                            int64_t t, float xt, int lane) {
   // A row with nothing left (every logit -inf): logp = -inf, H = 0.
   const bool empty = s.m == -INFINITY;
-  const float l2 = log2f(s.s1), ls = l2 * kLn2;
+  const float l2 = log2f(s.s1), ls = (l2 - shift(s.m)) * kLn2;
   if (lane == 0) {
     if (a.norm != nullptr) a.norm[n] = make_float2(s.m, empty ? -INFINITY : ls);
-    a.entropy[n] = empty ? 0.f : (l2 - __fdividef(s.s2, s.s1)) * kLn2;
+    a.entropy[n] = empty ? 0.f : (l2 - __fdividef(s.s2, s.s1)) * kLn2;  // (both hold the shift)
     float lp = 0.f;  // negative target: no token given
     if (t >= (int64_t)a.V) {
       record_device_error(a.status, SCREE_DEVERR_BAD_INPUT, kSiteTarget);
@@ -682,7 +689,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) logprobs_kernel(con
           for (int i = 1; i < kU; ++i) cm = max_nan(cm, vec_max<T>(d[i]));
           if (!(cm <= st.m)) stat_move(st, cm);
           if (!(fabsf(st.m) >= kFar)) {
-            const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-st.m * kLog2e, -st.m * kLog2e);
+            const uint64_t l2 = f2_pack(kLog2e, kLog2e), nm = f2_pack(-__fmul_rn(st.m, kLog2e), -__fmul_rn(st.m, kLog2e));
             uint64_t s1[2] = {0, 0}, s2[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < kU; ++i) {

@@ -36,3 +36,33 @@ def test_gradient_of_ids_outside_the_vocabulary(cuda):
         # (norm is torch's here: p to a few units in its last place)
         torch.testing.assert_close(buf[:N * V].view(N, V), want, atol=1e-5, rtol=1e-5)
     assert _status() == 0
+
+
+def _far_logits(N, V, dtype, cuda):
+    """Rows around levels from 20 to 1,000 of either sign (fp32 spacing up to 2^-14 there)."""
+    x, t = _logits(N, V, torch.float32, cuda, seed=21)
+    level = torch.tensor([20.0, 100.0, 333.3, 700.0, 1000.0, -100.0, -700.0, -1000.0], device=cuda)
+    x = x + level.repeat(N // 8)[:, None]
+    return x.clamp(-1020, 1020).to(dtype), t
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [4099, 32000, 131072])
+def test_scores_do_not_depend_on_the_logits_level(cuda, dtype, V):
+    """log p is a function of differences, x - m and log s1, each rounded to fp32 (u = 2^-24);
+    s1's relative error is below 2^-17 wherever the row lies (test_gpu_logprobs.py)."""
+    from scree_b200.kernels.native import token_logprobs
+
+    u, k = 2.0**-24, 5
+    x, t = _far_logits(24, V, dtype, cuda)
+    got = token_logprobs(x, t, top_k=k)
+    d = x.double() - x.double().amax(1, keepdim=True)
+    rest = torch.logsumexp(d, 1, keepdim=True)
+    lp = d - rest
+    tol = 2.0**-17 + 4 * u * (rest.abs() + d.abs())
+    at = lambda z, i: z.gather(1, i)  # noqa: E731
+    assert ((got.logp[:, None].double() - at(lp, t[:, None])).abs() <= at(tol, t[:, None])).all()
+    assert ((got.top_logp.double() - at(lp, got.top_ids)).abs() <= at(tol, got.top_ids)).all()
+    H = -(lp.exp() * lp).sum(1)
+    assert ((got.entropy.double() - H).abs() <= 2.0**-16 * (1 - (lp.exp() * d).sum(1))).all()
+    assert _status() == 0
