@@ -840,13 +840,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a)
   const float2 nm = a.norm[n];
   const float gh = a.g_entropy != nullptr ? a.g_entropy[n] : 0.f;
   const bool empty = nm.x == -INFINITY;  // nothing left in the row: no gradient
-  const float base = sm_gs + gh * a.entropy[n];
-  const float l2 = (nm.x + nm.y) * kLog2e, s2 = nm.y * kLog2e;
+  // log2 p = x log2e - l2, l2 = (m + log s1) log2e rounded once: what that leaves out, rest,
+  // is the row's, and so goes into the row's factors.  Far maxima: (x - m) log2e - s2.
   const bool far = fabsf(nm.x) >= kFar;
+  const float m2 = __fmul_rn(nm.x, kLog2e), s2 = __fmul_rn(nm.y, kLog2e), l2 = __fadd_rn(m2, s2);
+  float rest = fmaf(nm.y, kLog2e, -s2);
+  if (!far) {
+    const float part = __fsub_rn(l2, m2);
+    rest += fmaf(nm.x, kLog2e, -m2) + (__fsub_rn(m2, __fsub_rn(l2, part)) + __fsub_rn(s2, part));
+  }
+  const float y = -rest * kLn2, c = fmaf(y, fmaf(0.5f, y, 1.f), 1.f);  // c = 2^-rest, |rest| < 2^-12
+  const float base = c * fmaf(gh, a.entropy[n] + y, sm_gs), ghc = c * gh;
   auto grad = [&](float x) {
-    const float d2 = far ? fmaf(x - nm.x, kLog2e, -s2) : fmaf(x, kLog2e, -l2);  // log2 p
+    const float d2 = far ? fmaf(x - nm.x, kLog2e, -s2) : fmaf(x, kLog2e, -l2);  // log2 p + rest
     // The bound only matters at p = 0, where it keeps 0 * inf out.
-    return -ex2_approx(d2) * fmaf(gh, fmaxf(d2, -1000.f) * kLn2, base);
+    return -ex2_approx(d2) * fmaf(ghc, fmaxf(d2, -1000.f) * kLn2, base);
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {

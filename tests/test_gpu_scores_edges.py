@@ -66,3 +66,30 @@ def test_scores_do_not_depend_on_the_logits_level(cuda, dtype, V):
     H = -(lp.exp() * lp).sum(1)
     assert ((got.entropy.double() - H).abs() <= 2.0**-16 * (1 - (lp.exp() * d).sum(1))).all()
     assert _status() == 0
+
+
+@pytest.mark.parametrize("V", [4099, 32000, 131072])
+def test_gradient_does_not_depend_on_the_logits_level(cuda, V):
+    """p's relative error comes from the same differences; fp32 logits keep it visible."""
+    from scree_b200.kernels.native import token_logprobs_autograd
+
+    u, k, N = 2.0**-24, 3, 24
+    x, t = _far_logits(N, V, torch.float32, cuda)
+    gen = torch.Generator().manual_seed(6)
+    gl, gh, gt = (torch.randn(s, generator=gen).to(cuda) for s in ((N,), (N,), (N, k)))
+    y = x.detach().requires_grad_(True)
+    r = token_logprobs_autograd(y, t, k)
+    torch.autograd.backward([r.logp, r.entropy, r.top_logp], [gl, gh, gt])
+    d = x.double() - x.double().amax(1, keepdim=True)
+    rest = torch.logsumexp(d, 1, keepdim=True)
+    lp = d - rest
+    p = lp.exp()
+    H = -(p * lp).sum(1, keepdim=True)
+    one = torch.zeros_like(p).scatter_add_(1, t[:, None], gl.double()[:, None]).scatter_add_(1, r.top_ids, gt.double())
+    gs = one.sum(1, keepdim=True)
+    ent = gh.double()[:, None] * (lp + H)
+    want = one - p * (gs + ent)
+    rel = 2.0**-17 + 8 * u * (d.abs() + rest.abs())
+    tol = p * (gs.abs() + ent.abs() + gh.double().abs()[:, None]) * rel + u * (one.abs() + want.abs())
+    assert ((y.grad.double() - want).abs() <= tol).all()
+    assert _status() == 0
