@@ -21,6 +21,7 @@ import math
 from typing import Any, NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -588,7 +589,8 @@ def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
     tokens of (N, V) logits, fp16 / bf16 / fp32 with any row stride; one read of the
     logits.  A negative target means that no token is given (logp 0); a target >= V
     sets the device status word.  Equal logits rank by lower index; a row whose logits
-    are all -inf has logp -inf and entropy 0.  No reference counterpart."""
+    are all -inf has logp -inf and entropy 0.  Not differentiable (see token_logprobs_autograd).
+    No reference counterpart."""
     _, _, logp, entropy, _, top_logp, top_ids = _logprobs_fwd(logits, targets, top_k, False)
     return TokenLogprobs(logp, entropy, top_logp, top_ids)
 
@@ -603,6 +605,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
         logits, targets, norm, entropy, top_ids = ctx.saved_tensors
         N, V = logits.shape
@@ -621,5 +624,5 @@ class _TokenLogprobs(torch.autograd.Function):
 
 def token_logprobs_autograd(logits, targets, top_k: int = 0) -> TokenLogprobs:
     """Differentiable token_logprobs: the gradient of the logits from those of logp,
-    entropy and top_logp, in one pass over the logits."""
+    entropy and top_logp, in one pass over the logits.  Once: a second derivative is refused."""
     return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top_k))

@@ -93,3 +93,20 @@ def test_gradient_does_not_depend_on_the_logits_level(cuda, V):
     tol = p * (gs.abs() + ent.abs() + gh.double().abs()[:, None]) * rel + u * (one.abs() + want.abs())
     assert ((y.grad.double() - want).abs() <= tol).all()
     assert _status() == 0
+
+
+def test_a_second_derivative_is_refused(cuda):
+    """The gradient is a kernel's output and no function of the logits to autograd: a term made of
+    it would lose its own gradient."""
+    from scree_b200.kernels.native import token_logprobs_autograd
+
+    x, t = _logits(3, 50, torch.float32, cuda)
+    y = x.detach().requires_grad_(True)
+    w = torch.ones(3, device=cuda, requires_grad=True)
+    r = token_logprobs_autograd(y, t)
+    (g,) = torch.autograd.grad((r.logp * w).sum(), y, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (g.square().sum() + y.square().sum()).backward()
+    y.grad = None
+    token_logprobs_autograd(y, t).logp.sum().backward(create_graph=False)
+    assert y.grad is not None and _status() == 0
