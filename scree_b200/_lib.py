@@ -248,7 +248,7 @@ def stream_ptr(device=None) -> int:
     global _raw_stream
     import torch
 
-    if device is None or device.index is None:
+    if not isinstance(device, torch.device) or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     if _raw_stream is None:
         # The same value without making a Stream object (2 us of a small call's time).
