@@ -71,6 +71,8 @@ class PagedCache:
         pools.sizes = (S, M, P, page, H, D)
         pools.dtype, pools.device = self.k.dtype, self.k.device
         pools.ref, pools.work_bytes = ctypes.byref(pools), _lib.load().scree_paged_workspace_size(S, P)
+        pools.work_at = -(-4 * (S * M + S + P) // 16) * 16  # bytes, in a call's allocation
+        pools.ints = (pools.work_at + pools.work_bytes) // 4
         object.__setattr__(self, "_pools", pools)
 
     @property
@@ -102,15 +104,19 @@ def _ints(t, n, what, device):
 
 
 def _book_call(cache: PagedCache, fn, name: str, *args) -> PagedCache:
-    t, le, r, pools = cache.table, cache.lengths, cache.refs, cache._pools
-    table, lengths, refs = torch.empty_like(t), torch.empty_like(le), torch.empty_like(r)
+    pools = cache._pools
     S, M, P, page, _, _ = pools.sizes
-    book = _lib.PagedBook(t.data_ptr(), le.data_ptr(), r.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                          refs.data_ptr(), S, M, P, page)
-    # The plan's workspace is the call's own, of the stream it runs on: another call, on another
-    # stream or thread, cannot come between the plan and its apply.
-    work = r.new_empty(pools.work_bytes // 4)
-    rc = fn(ctypes.byref(book), *args, work.data_ptr(), pools.work_bytes, _lib.stream_ptr(pools.device))
+    # One allocation: the new bookkeeping, and behind it the plan's workspace.  That is the call's
+    # own, of the stream it runs on: another call, on another stream or thread, cannot come between
+    # the plan and its apply.
+    buf = cache.refs.new_empty(pools.ints)
+    table = buf.as_strided((S, M), (M, 1), 0)
+    lengths = buf.as_strided((S,), (1,), S * M)
+    refs = buf.as_strided((P,), (1,), S * M + S)
+    at = buf.data_ptr()
+    book = _lib.PagedBook(cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(), at, at + 4 * S * M,
+                          at + 4 * (S * M + S), S, M, P, page)
+    rc = fn(ctypes.byref(book), *args, at + pools.work_at, pools.work_bytes, _lib.stream_ptr(pools.device))
     if rc:
         _lib.check(rc, name)
     out = object.__new__(PagedCache)  # nothing to check: the same pools and shapes
@@ -167,11 +173,6 @@ def paged_compact(cache: PagedCache) -> PagedCache:
     return _book_call(cache, _lib.load().scree_paged_compact, "paged_compact", cache._pools.ref)
 
 
-def _ragged_tokens(name, *arrays):
-    if any(a.ragged_dim != 0 for a in arrays):
-        raise NotImplementedError(f"{name} supports ragged_dim=0 only in v0.1")
-
-
 def _offsets(arr: Array, device):
     """Offsets on the device, whether they are int64, sequences."""
     offs = arr.offsets
@@ -187,7 +188,8 @@ def paged_write(cache: PagedCache, layer: int, slots, k: Array, v: Array) -> Non
     tokens of slot slots[b] in one layer.  Not written, with the status word set: the rows of
     sequences that name one slot, or have more tokens than it holds, rows on a page that other
     slots hold, and all rows if k and v have different offsets."""
-    _ragged_tokens("paged_write", k, v)
+    if k.ragged_dim != 0 or v.ragged_dim != 0:
+        raise NotImplementedError("paged_write supports ragged_dim=0 only in v0.1")
     kt, vt, pools = k.values, v.values, cache._pools
     S, M, P, page, H, D = pools.sizes
     dev = pools.device
@@ -253,7 +255,8 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     the LSE (T, heads) fp32 when ``return_lse``)."""
     qt, pools = q.values, cache._pools
     _require_cuda(qt, "paged_attention")
-    _ragged_tokens("paged_attention", q)
+    if q.ragged_dim != 0:
+        raise NotImplementedError("paged_attention supports ragged_dim=0 only in v0.1")
     S, M, P, page, Hkv, D = pools.sizes
     dev, dtype = qt.device, qt.dtype
     assert dtype in (torch.float16, torch.bfloat16), "fp16 or bf16 only"

@@ -35,6 +35,12 @@ def test_calls_in_flight_have_workspaces_of_their_own(monkeypatch):
     for i, a in enumerate(spans):
         for b in spans[:i]:
             assert a[1] <= b[0] or b[1] <= a[0]
+    for t, like in ((out.table, cache.table), (out.lengths, cache.lengths), (out.refs, cache.refs)):
+        assert t.shape == like.shape and t.dtype == like.dtype and t.is_contiguous()
+        end = t.data_ptr() + 4 * t.numel()
+        assert end <= spans[0][0] or spans[0][1] <= t.data_ptr()
+        assert all(end <= o.data_ptr() or o.data_ptr() + 4 * o.numel() <= t.data_ptr()
+                   for o in (out.table, out.lengths, out.refs) if o is not t)
     # A derived cache keeps nothing of its call but the new bookkeeping.
     fresh = {k for k, v in out.__dict__.items() if v is not cache.__dict__.get(k)}
     assert fresh == {"table", "lengths", "refs"}
