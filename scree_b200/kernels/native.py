@@ -595,6 +595,25 @@ def token_logprobs(logits, targets, top_k: int = 0) -> TokenLogprobs:
     return TokenLogprobs(logp, entropy, top_logp, top_ids)
 
 
+def _logprobs_bwd(ctx, g_logp, g_entropy, g_top, _):
+    logits, targets, norm, entropy, top_ids = ctx.saved_tensors
+    N, V = logits.shape
+    f32 = lambda g: g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) \
+        else g.to(torch.float32).contiguous()  # noqa: E731
+    g_logp, g_entropy, g_top = f32(g_logp), f32(g_entropy), f32(g_top)
+    dx = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    rc = _lib.load().scree_token_logprobs_bwd(
+        logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0,
+        norm.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), _ptr(g_logp), _ptr(g_entropy), _ptr(g_top),
+        N, V, top_ids.shape[1], _lib.dtype_code(logits.dtype), dx.data_ptr(), _lib.stream_ptr(logits.device))
+    if rc:
+        _lib.check(rc, "token_logprobs backward")
+    return dx, None, None
+
+
+_logprobs_bwd_once = once_differentiable(_logprobs_bwd)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k):
@@ -605,21 +624,9 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, g_top, _):
-        logits, targets, norm, entropy, top_ids = ctx.saved_tensors
-        N, V = logits.shape
-        f32 = lambda g: g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) \
-            else g.to(torch.float32).contiguous()  # noqa: E731
-        g_logp, g_entropy, g_top = f32(g_logp), f32(g_entropy), f32(g_top)
-        dx = torch.empty_like(logits, memory_format=torch.contiguous_format)
-        rc = _lib.load().scree_token_logprobs_bwd(
-            logits.data_ptr(), logits.stride(0), targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0,
-            norm.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), _ptr(g_logp), _ptr(g_entropy), _ptr(g_top),
-            N, V, top_ids.shape[1], _lib.dtype_code(logits.dtype), dx.data_ptr(), _lib.stream_ptr(logits.device))
-        if rc:
-            _lib.check(rc, "token_logprobs backward")
-        return dx, None, None
+    def backward(ctx, *grads):
+        # Only where a graph of the gradient is wanted does it need the refusal of a second one.
+        return (_logprobs_bwd_once if torch.is_grad_enabled() else _logprobs_bwd)(ctx, *grads)
 
 
 def token_logprobs_autograd(logits, targets, top_k: int = 0) -> TokenLogprobs:
