@@ -16,13 +16,17 @@
 //
 // Bound: HBM, 4 D bytes per key and K/V head (R = 16 rows of mma.sync work per
 // key hide under that).  64 sequences of 2048 keys on average, lengths spread 0.6
-// log-normal, 8 K/V heads of 128: 112 us for 621 MB, 5.5 TB/s; the SMs end between 90
+// log-normal, 8 K/V heads of 128: 113 us for 621 MB, 5.5 TB/s; the SMs end between 90
 // and 104 us, the join takes the rest.  (The last sixth of the groups handed out from
 // a counter instead: 117.6 us against 115.9 on the same build, its join slower.)  A group is as many keys as make 8 KB of K and V: the
 // chain scores -> maximum -> exponentials -> product takes a warp about 1,000
 // cycles whatever the number of keys, and with 16 keys at D = 64 that, not HBM,
 // set the pace (2 x 131071 keys: main kernel 25 us against 21).  It is loaded in
 // boxes of 16 keys, which never span pages.
+//
+// P goes to the product with V in the queries' 16-bit type, as mma.sync takes it and as
+// in attn_fwd.cu: each weight is off by half a unit of that type, the row sums l and the
+// pieces are fp32.
 #include <algorithm>
 #include "attn_paged.cuh"
 
@@ -518,12 +522,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 
 // Which kernel: this one pads a tile's rows to 16 and reads the cache once per tile;
 // the tensor-core one pads them to 128 and runs at its softmax's pace.  Measured (us,
-// this / that; D 128, 4 query heads a K/V head), for 16 sequences of 4096 keys at 8,
-// 16, 24 and 40 rows: 61 / 69, 63 / 71, 102 / 73, 100 / 74; for 64 of 2048 keys: 100 /
-// 143, 106 / 144, 189 / 145, 277 / 147.  (Two tiles of 16 rows in one pass of this
-// kernel, its registers spilling: 85 and 143 at 24 rows.)  The rows of a sequence are
-// known on the device only; their mean decides.  A tensor-core tile holds whole
-// tokens, so at most 128 heads a group.
+// this / that) at 16, 32 and 64 rows a K/V head:
+//   D 128, 8 K/V heads    512 x 64 keys   61 / 206,   94 / 205,  172 / 206
+//   (4 query heads each)  128 x 256       48 / 100,   70 / 100,  109 / 103
+//                         64 x 2,048     106 / 138,  190 / 143,  358 / 144
+//                         16 x 4,096      62 / 69,   102 / 72,   154 / 72
+//                         1,024 x 1,024  718 / 1218, 1412 / 1208, 2791 / 1250
+//   D 64, 2 K/V heads     512 x 64        25 / 52,    35 / 52,    47 / 52
+//   (8 query heads each)  64 x 2,048      25 / 38,    33 / 39,    49 / 39
+//                         16 x 4,096      21 / 26,    27 / 26,    31 / 26
+//                         1,024 x 1,024  112 / 256,  191 / 257,  354 / 264
+// (D 32 as D 64; one query head a K/V head as four.)  One tile of rows is better here
+// throughout, and the rule's limit.  Two are better here too at D 64 and over short
+// contexts, which the rule leaves aside: it goes by the rows alone.  The rows of a
+// sequence are known on the device only; their mean decides.  A tensor-core tile holds
+// whole tokens, so at most 128 heads a group.
 bool few_rows(int64_t B, int64_t T, int64_t H, int64_t H_kv) {
   return T * (H / H_kv) <= R * B || H / H_kv > 128;
 }

@@ -32,10 +32,11 @@
 // rows that do see them get them back when the piece is stored.
 //
 // Bound: the chain scores -> softmax -> product of a pair of tiles, 2.3 us per 128
-// keys (the tensor pipe is active 45% of the time, HBM 33%), then the start and end
-// of a run: finding its pieces, 7.5 us with the first tile; storing a piece, 4 us;
-// the join, 14.  16 sequences of 4096 keys, 61 drafted tokens, 32 heads over 8 of
-// 128: 111 us, 0.62 PFLOP/s of visible pairs; its bytes alone would take 54.
+// keys (the tensor pipe is active 42% of the time, HBM at 38% of its peak), then the
+// start and end of a run: finding its pieces, 7.5 us with the first tile; storing a
+// piece, 4 us; the join, 14.  16 sequences of 4096 keys, 61 drafted tokens, 32 heads over
+// 8 of 128: 113 us, 0.61 PFLOP/s of visible pairs; its bytes alone would take 54.  P is
+// held in the queries' 16-bit type, as the tensor cores take it; l and O are fp32.
 #include <algorithm>
 #include "attn_paged.cuh"
 

@@ -14,8 +14,8 @@
 // and a tenth warp joins them, two rows behind at most.  Of few rows each is cut
 // into segments for the CTAs of a cluster, which hand their results to its first
 // CTA through shared memory.  6,144 x 128,000 in 16 bits: 270 us (5.8 TB/s), with
-// four alternatives 276; 4,099 x 65,539 with eight: 106; 16,384 x 16,384: 115, with
-// four 195 (the tenth warp's pace: 5 us a row); 1 x 131,072 with twenty: 8.4.  (With
+// four alternatives 274; 4,099 x 65,539 with eight: 107; 16,384 x 16,384: 111, with
+// four 182 (the tenth warp's pace: 5 us a row); 1 x 131,072 with twenty: 8.4.  (With
 // the eight warps joining and merging at barriers between rows: 276, 332, 152, 178,
 // 318 and 11.6.)
 //
@@ -776,12 +776,12 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int byt
 }
 
 // dx = -p (gs + gH (H + log p)), then the given token and the alternatives.
-// HBM-bound: one read and one write of each logit; 6,144 x 128,000 in 16 bits: 530 us,
-// 5.9 TB/s (16 vectors a thread: 700, 4: 549; plain loads: 542).  Where a row begins
+// HBM-bound: one read and one write of each logit; 6,144 x 128,000 in 16 bits: 527 us,
+// 6.0 TB/s (16 vectors a thread: 700, 4: 549; plain loads: 542).  Where a row begins
 // at another place of a 16-byte block than dx's does (rows of a padded vocabulary),
 // 16-bit types are stored in dx's vectors, each put together from two of the row's:
-// 8,192 x 50,257 of 50,304 461 us (element by element 978; without padding 324); fp32
-// element by element: 4,096 rows 300 (in vectors 329; without padding 258).
+// 8,192 x 50,257 of 50,304 453 us (element by element 978; without padding 324); fp32
+// element by element: 4,096 rows 289 (in vectors 329; without padding 258).
 template <typename T, int NV>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs a) {
   constexpr int VE = Lv<T>::N;

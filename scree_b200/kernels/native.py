@@ -571,7 +571,7 @@ def _logprobs_fwd(logits, targets, top_k, want_norm):
         targets = targets.contiguous()
     f32 = torch.float32
     logp = torch.empty(N, dtype=f32, device=dev)
-    entropy = torch.empty_like(logp)  # (half the time of empty)
+    entropy = torch.empty_like(logp)  # (1.3 us, empty 1.6)
     norm = torch.empty((N, 2), dtype=f32, device=dev) if want_norm else None  # for the gradient
     top_logp = torch.empty((N, max(top_k, 0)), dtype=f32, device=dev)
     top_ids = torch.empty_like(top_logp, dtype=torch.int64)

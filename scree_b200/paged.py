@@ -15,10 +15,11 @@ A ``PagedCache`` is immutable like ``Array``: every call returns a new one with
 new bookkeeping tensors; the K / V pools are shared and updated in place.
 Slots, counts and paths are int32 CUDA tensors and nothing here reads them on
 the host.  What a call cannot do (a slot out of range or named twice, too few
-free pages, a draft on shared pages) leaves the bookkeeping as it was and sets
-the device status word, which ``scree_b200._lib.raise_device_status()`` turns
-into ``ScreeError``.  All calls on one cache must be ordered on the GPU (one
-stream, or streams that wait for one another).
+free pages, a draft on shared pages) leaves the bookkeeping as it was, or the
+rows unwritten, and sets the device status word, which
+``scree_b200._lib.raise_device_status()`` turns into ``ScreeError``.  All calls
+on one cache must be ordered on the GPU (one stream, or streams that wait for
+one another).
 """
 
 from __future__ import annotations
@@ -251,8 +252,11 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     their own number those that their row of ``mask`` names (``tree_mask``, or any (T, words)
     int64 bits), or the earlier ones and themselves if mask is None.  A query that sees nothing
     gets 0 and LSE -inf.  heads is a multiple of the cache's kv_heads; head_dim 32, 64 or 128;
-    page_size a multiple of 16; at most 4096 sequences.  Returns an Array on q's offsets (and
-    the LSE (T, heads) fp32 when ``return_lse``)."""
+    page_size a multiple of 16; at most 4096 sequences.  The probabilities are rounded to q's
+    dtype for their product with V; sums are fp32.  Infinities and NaN in the K / V of new tokens
+    reach the queries that see them and no others; earlier tokens' are taken to be finite.
+    Forward only (inference), like ``varlen_attention_kv``: the result has no gradient.  Returns
+    an Array on q's offsets (and the LSE (T, heads) fp32 when ``return_lse``)."""
     qt, pools = q.values, cache._pools
     _require_cuda(qt, "paged_attention")
     if q.ragged_dim != 0:
@@ -278,7 +282,7 @@ def paged_attention(q: Array, cache: PagedCache, layer: int, slots, mask=None, r
     if sd != 1 or sr % 8 or sh % 8 or sr * sh == 0 or qt.data_ptr() % 16:
         qt = qt.clone(memory_format=torch.contiguous_format)  # contiguous() would keep a misaligned base
         sr, sh, _ = qt.stride()
-    out = torch.empty_like(qt, memory_format=torch.contiguous_format)  # (half the time of empty)
+    out = torch.empty_like(qt, memory_format=torch.contiguous_format)  # (1.3 us, empty 1.6)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T:
         lib = _lib.load()
